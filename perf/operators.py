@@ -110,7 +110,7 @@ def draw(rng):
         B = max(1, min(size(1, 32), (1 << 24) // (W * V)))
         Hkv, length = size(1, 8), size(1, 600)
         layer = B * W * (length // 2 + 2 * page) * Hkv * D * 4  # bytes of one layer's cache
-        layers = min(rng.choice((0, 1, size(2, 24))), (1 << 30) // layer)
+        layers = min(rng.choice((0, 1, size(2, 24))), (1 << 29) // layer)
         c = beam("", B, W, V, layers, Hkv, D, page, length, dtype, rng.choice((HALF, HALF, SINGLE)))
     del c["name"]
     return c
