@@ -269,6 +269,143 @@ WGX_API int wgx_conv2d_noalloc(const wgx_conv2d_params *p, const void *in, const
                                const void *bias, void *out, void *stream);
 
 /* ------------------------------------------------------------------ */
+/* text decoding over a paged key/value cache. No counterpart in the    */
+/* reference (its programs are vision models).                          */
+/* ------------------------------------------------------------------ */
+/* One layer's cache, or `layers` of them (only wgx_beam_search_step reads
+ * more than the first): K and V rows of head_dim elements (unit stride) in
+ * pages of page_size slots. Slot s of sequence b and head h is the row
+ *   k + page_table[b * table_stride + s / page_size] * k_page_stride
+ *     + h * k_head_stride + (s % page_size) * k_slot_stride   (elements)
+ * Strides are free (head-major and slot-major pages, slices of a larger
+ * pool); rows that start on 16-byte boundaries are moved in 16-byte units.
+ * Page ids and lengths are device data: a page id outside [0, pages), or a
+ * length outside [0, table_width * page_size], is never followed; what it
+ * names is left out and the device error word gets a bit, which the next
+ * wgx_sync reports as WGX_ERR_DEVICE. */
+typedef struct wgx_kv_cache {
+  void *k, *v;
+  const int32_t *page_table; /* [batch][table_width] */
+  int64_t k_layer_stride, k_page_stride, k_head_stride, k_slot_stride;
+  int64_t v_layer_stride, v_page_stride, v_head_stride, v_slot_stride;
+  int64_t table_stride;
+  int32_t batch, kv_heads, head_dim, dtype; /* WGX_FLOAT32 / WGX_FLOAT16 */
+  int32_t pages, page_size, table_width, layers;
+} wgx_kv_cache;
+
+/* Writes the K and V rows of `tokens` new tokens of every sequence behind
+ * its lengths[b] slots; lengths_out[b] = lengths[b] + tokens (may be the
+ * same array). Optional (NULL): weights, positions [batch][kv_heads][slots]
+ * dense: 0 and seen[b] + t are written at the new slots, and seen_out[b] =
+ * seen[b] + tokens (may be the same array). A sequence whose table has no
+ * room for all of the tokens gets none and keeps its length (error word). */
+typedef struct wgx_kv_append_args {
+  wgx_kv_cache cache;
+  const void *k, *v; /* [batch][tokens][kv_heads][head_dim] */
+  int64_t k_batch_stride, k_token_stride, k_head_stride;
+  int64_t v_batch_stride, v_token_stride, v_head_stride;
+  const int32_t *lengths;
+  int32_t *lengths_out;
+  const int32_t *seen;
+  int32_t *seen_out;
+  float *weights;
+  int32_t *positions;
+  int64_t slots;
+  int32_t tokens, reserved;
+} wgx_kv_append_args;
+WGX_API int wgx_kv_append(const wgx_kv_append_args *a, void *stream);
+
+/* Attention of one new token per sequence over its cache:
+ *   out[b][i] = sum_j softmax_j(scale * q[b][i] . k_j) v_j
+ * over the live slots j of KV head i / (q_heads / kv_heads): j < lengths[b],
+ * j >= lengths[b] - window where window > 0, and mask[b][j] != 0 where there
+ * is a mask (slots at or beyond mask_width are left out). A sequence without
+ * live slots gets zeros; what the cache holds in slots that are not live
+ * (infinities and NaN too) has no effect. With weights_out, dense
+ * [batch][kv_heads][slots], the probabilities are accumulated per slot:
+ *   weights_out[b][h][j] = weights[b][h][j] + sum of the group's p_j
+ * for j < lengths[b] (other slots are not written; may be the same array).
+ * Scores, softmax and sums are fp32, one rounding at the end. scratch:
+ * wgx_paged_attention_scratch_bytes() (its contents need no preparation). */
+typedef struct wgx_paged_attention_args {
+  wgx_kv_cache cache;
+  const void *q; /* [batch][q_heads][head_dim] */
+  void *out;
+  int64_t q_batch_stride, q_head_stride, out_batch_stride, out_head_stride;
+  const int32_t *lengths;
+  const uint8_t *mask; /* [batch][mask_width], NULL: none */
+  int64_t mask_stride;
+  const float *weights;
+  float *weights_out;
+  int64_t slots;
+  void *scratch;
+  uint64_t scratch_bytes;
+  int32_t q_heads, window, mask_width;
+  float scale;
+} wgx_paged_attention_args;
+WGX_API int wgx_paged_attention_scratch_bytes(const wgx_paged_attention_args *a, uint64_t *bytes);
+WGX_API int wgx_paged_attention(const wgx_paged_attention_args *a, void *stream);
+
+/* Shrinks every sequence of more than `budget` slots to `budget` slots, per
+ * KV head, by accumulated attention weight. Slots are ordered by (protected,
+ * weight), largest first, equal ones by slot, NaN weights last; the first
+ * `budget` stay. Protected: position >= seen[b] - recent or position < sinks
+ * (recent + sinks <= budget). The j-th survivor at or behind slot `budget`
+ * moves into the j-th free slot before it (both in slot order); nothing else
+ * moves, so slot order is not token order: positions say which token a slot
+ * holds. weights_out / positions_out (may be the inputs) are written for the
+ * slots that remain; lengths_out[b] = min(lengths[b], budget) (may be
+ * lengths). Sequences must not share the pages that are written. */
+typedef struct wgx_cache_evict_args {
+  wgx_kv_cache cache;
+  const int32_t *lengths;
+  int32_t *lengths_out;
+  const int32_t *seen;
+  const float *weights; /* [batch][kv_heads][slots] dense, as the next three */
+  float *weights_out;
+  const int32_t *positions;
+  int32_t *positions_out;
+  int64_t slots;
+  int32_t budget, recent, sinks, reserved;
+} wgx_cache_evict_args;
+WGX_API int wgx_cache_evict(const wgx_cache_evict_args *a, void *stream);
+
+/* One step of beam search. Every unfinished beam w of item b proposes its
+ * min(beams, vocab) largest logits (equal ones: the lowest token) with
+ *   total = scores[b][w] + logits[b][w][t] - log(sum_t' exp(logits[b][w][t']))
+ * in fp32; a finished beam proposes `eos` with its own score. The `beams`
+ * best proposals by total (equal ones: the lowest beam, then the larger
+ * logit, then the lowest token) become the new beams: scores_out, parents
+ * (beam indices), tokens, finished_out = finished[parent] or token == eos.
+ * NaN logits count as -infinity, NaN totals rank as -infinity.
+ * With a cache (cache.k not NULL; cache.batch = batch * beams sequences, beam
+ * w of item b is sequence b * beams + w) the state is reordered: the child
+ * takes its parent's page table (full pages are shared) and length, and the
+ * used slots of a partly filled last page are copied, in every layer, into
+ * the child's page spare[sequence], which takes that page's place. Spare
+ * pages must be in no table; outputs must not overlap inputs. */
+typedef struct wgx_beam_search_args {
+  wgx_kv_cache cache;
+  const void *logits; /* [batch][beams][vocab] */
+  int64_t logits_batch_stride, logits_beam_stride;
+  const float *scores;     /* [batch][beams] dense, as the next five */
+  const uint8_t *finished;
+  float *scores_out;
+  int32_t *parents, *tokens;
+  uint8_t *finished_out;
+  const int32_t *lengths;  /* [batch * beams] */
+  const int32_t *spare;
+  int32_t *page_table_out; /* [batch * beams][table_width] dense */
+  int32_t *lengths_out;
+  void *scratch;
+  uint64_t scratch_bytes;
+  int32_t batch, beams, vocab, dtype, eos, reserved;
+} wgx_beam_search_args;
+#define WGX_MAX_BEAMS 32
+WGX_API int wgx_beam_search_scratch_bytes(const wgx_beam_search_args *a, uint64_t *bytes);
+WGX_API int wgx_beam_search_step(const wgx_beam_search_args *a, void *stream);
+
+/* ------------------------------------------------------------------ */
 /* kernel timing: when enabled, the hot-path kernels launched outside a */
 /* CUDA graph record a CUDA-event pair on their own stream around the   */
 /* main kernel. read() waits for the recorded pairs and returns the     */

@@ -1,0 +1,50 @@
+// Text decoding over a paged key/value cache: declarations shared by the
+// kernels (decode_attention.cu, decode_cache.cu, decode_beam.cu) and their
+// front end (ops_decode.cu: checks, C entry points, recorders).
+#pragma once
+#include "internal.h"
+
+namespace wgx {
+
+// All enqueue on `stream`, expect checked arguments and throw Error when a
+// launch fails.
+uint64_t paged_attention_scratch_bytes(const wgx_paged_attention_args &a);
+void launch_paged_attention(const wgx_paged_attention_args &a, cudaStream_t stream);
+void launch_kv_append(const wgx_kv_append_args &a, cudaStream_t stream);
+void launch_cache_evict(const wgx_cache_evict_args &a, cudaStream_t stream);
+uint64_t beam_search_scratch_bytes(const wgx_beam_search_args &a);
+void launch_beam_search_step(const wgx_beam_search_args &a, cudaStream_t stream);
+
+// Slots one sequence's table can name.
+inline int64_t cache_capacity(const wgx_kv_cache &c) { return int64_t(c.table_width) * c.page_size; }
+
+// K and V rows can be moved in 16-byte units.
+inline bool cache_rows_16b(const wgx_kv_cache &c) {
+  const int e = c.dtype == WGX_FLOAT16 ? 2 : 4;
+  const int64_t strides[] = {c.k_layer_stride, c.k_page_stride, c.k_head_stride, c.k_slot_stride,
+                             c.v_layer_stride, c.v_page_stride, c.v_head_stride, c.v_slot_stride};
+  int64_t bits = int64_t(c.head_dim) * e;
+  for (int64_t s : strides) bits |= s * e;
+  return ((bits | int64_t(reinterpret_cast<uintptr_t>(c.k)) |
+           int64_t(reinterpret_cast<uintptr_t>(c.v))) & 15) == 0;
+}
+
+int device_sm_count();  // of the current device
+inline int current_device() {
+  int dev = 0;
+  check_cuda(cudaGetDevice(&dev), "cudaGetDevice");
+  return dev;
+}
+
+#ifdef __CUDACC__
+// Slots in use of sequence b, held within [0, capacity].
+__device__ __forceinline__ int slots_in_use(const int32_t *lengths, int b, int64_t capacity,
+                                            uint32_t *err) {
+  const int n = lengths[b];
+  if (n >= 0 && n <= capacity) return n;
+  atomicOr(err, kErrCache);
+  return n < 0 ? 0 : int(capacity);
+}
+#endif
+
+}  // namespace wgx

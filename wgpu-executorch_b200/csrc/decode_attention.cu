@@ -1,0 +1,858 @@
+// Attention of one new token per sequence over a paged K/V cache:
+//   s_j = scale * q . k_j,  p_j = exp(s_j - max s) / sum exp(s - max s),
+//   out = sum_j p_j v_j     over the live slots j of the sequence,
+// for all query heads that share a K/V head at once.
+//
+// Every cached byte is read once and used for 2 * group multiply-adds per
+// element, so the cache's bytes over the HBM rate are the floor. The work is
+// split over the cache's length: a step is TOK slots of one (sequence, K/V
+// head), all steps of the batch stand in one line, and every warp of the grid
+// takes an equal, contiguous share of it, whatever the lengths are. A warp
+// streams its steps through a ring of its own in shared memory (cp.async,
+// rows of slots that are not live are zero-filled instead of read: stale
+// infinities and NaN of a page cannot reach a product), so no block barrier
+// stands between loads and products. The softmax is the running one: maximum
+// and sum in fp32 per head, the result rescaled when the maximum grows.
+//
+// The group's heads are the 16 rows of an mma.sync tile (M = heads, N = slots
+// for the scores, N = channels for the result). tcgen05 would need 64 or 128
+// rows; a decode step has at most a group of them, and its time is the
+// loads'. fp16: m16n8k16, exact products, fp32 sums. fp32: m16n8k8 tf32 with
+// every operand split into a tf32 head and the fp32 tail (3 products).
+//
+// A row of work that lies within one warp's share is finished by it. Rows cut
+// by a share's end leave (max, sum, unnormalised result) in scratch, at most
+// two per warp, and join_kernel combines them; it also accumulates the
+// probabilities per slot from the scores, kept in scratch for it.
+#include <algorithm>
+#include <mutex>
+
+#include "decode.h"
+#include "tcgen05.h"
+
+namespace wgx {
+
+namespace {
+
+constexpr int PA_WARPS = 4;
+constexpr int PA_HEADS = 16;        // rows of an mma tile
+constexpr int PA_MAX_GROUP = 128;   // query heads per K/V head
+constexpr int PA_JOIN_THREADS = 128;
+constexpr int PA_JOIN_SLOTS = 1024;  // slots per join block of the accumulation
+
+struct AttnArgs {
+  wgx_paged_attention_args a;
+  int64_t capacity;   // slots a table can name
+  int group;          // query heads per K/V head
+  int chunks;         // ceil(group / PA_HEADS)
+  int max_workers;    // warps the scratch has room for
+  int min_steps;      // steps a warp takes at least
+  int vec;            // rows move in 16-byte units
+  float scale2;       // scale * log2(e): the softmax runs in base 2
+  float *part_o;      // [worker][2][heads][head_dim]
+  float2 *part_ml;    // [worker][2][heads] (max, sum)
+  float2 *stats;      // [row][heads]: of rows finished by one warp (accumulation only)
+  float *scores;      // [batch][q_heads][score_stride] (accumulation only)
+  int64_t score_stride;
+  int heads;          // min(group, PA_HEADS): rows a partial result has
+  uint32_t *err;
+};
+
+// The line of work: sequence b has steps[b] steps in each of its
+// kv_heads * chunks rows. prefix[b] = sum of steps before b (all rows' line
+// is prefix[batch] * rows long).
+struct Span {
+  int first;  // first step (of TOK slots, from slot 0)
+  int steps;
+  int len;
+  int lo;     // first live slot
+};
+template <int TOK>
+__device__ __forceinline__ Span span_of(const AttnArgs &p, int len) {
+  Span s;
+  s.len = len;
+  s.lo = p.a.window > 0 ? max(0, len - p.a.window) : 0;
+  s.first = s.lo / TOK;
+  s.steps = (len + TOK - 1) / TOK - s.first;
+  return s;
+}
+
+// prefix[0 .. batch] and lens[0 .. batch - 1] into shared memory.
+template <int TOK>
+__device__ void build_prefix(const AttnArgs &p, uint32_t *prefix, int *lens) {
+  const int B = p.a.cache.batch, tid = threadIdx.x, nt = blockDim.x;
+  __shared__ uint32_t warp_sum[32];
+  uint32_t base = 0;
+  for (int b0 = 0; b0 < B; b0 += nt) {
+    const int b = b0 + tid;
+    uint32_t n = 0;
+    if (b < B) {
+      const int len = slots_in_use(p.a.lengths, b, p.capacity, p.err);
+      lens[b] = len;
+      n = uint32_t(span_of<TOK>(p, len).steps);
+    }
+    uint32_t x = n;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const uint32_t y = __shfl_up_sync(~0u, x, d);
+      if ((tid & 31) >= d) x += y;
+    }
+    if ((tid & 31) == 31) warp_sum[tid >> 5] = x;
+    __syncthreads();
+    uint32_t before = base, all = base;
+    for (int w = 0; w < nt / 32; ++w) {
+      if (w < (tid >> 5)) before += warp_sum[w];
+      all += warp_sum[w];
+    }
+    if (b < B) prefix[b] = before + x - n;
+    base = all;
+    __syncthreads();
+  }
+  if (tid == 0) prefix[B] = base;
+  __syncthreads();
+}
+
+__device__ __forceinline__ int worker_count(const AttnArgs &p, uint64_t total) {
+  const uint64_t want = (total + p.min_steps - 1) / p.min_steps;
+  return int(want < uint64_t(p.max_workers) ? (want ? want : 1) : uint64_t(p.max_workers));
+}
+__device__ __forceinline__ uint64_t share_begin(uint64_t total, int worker, int workers) {
+  return total * uint64_t(worker) / uint64_t(workers);
+}
+// the worker whose share holds step s
+__device__ __forceinline__ int worker_of(uint64_t s, uint64_t total, int workers) {
+  return int(((s + 1) * uint64_t(workers) - 1) / total);
+}
+
+// A place in the line of work.
+struct Place {
+  int b, row, step;  // row: kv_head * chunks + chunk; step within the row
+  Span s;
+};
+template <int TOK>
+__device__ __forceinline__ void next_step(const AttnArgs &p, const int *lens, int rows, Place &w) {
+  if (++w.step < w.s.steps) return;
+  w.step = 0;
+  if (++w.row < rows) return;
+  w.row = 0;
+  while (++w.b < p.a.cache.batch) {
+    w.s = span_of<TOK>(p, lens[w.b]);
+    if (w.s.steps > 0) return;
+  }
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(live ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t *r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t *r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void mma16(float *c, const uint32_t *a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma8(float *c, const uint32_t *a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// x = head + tail in tf32's 10 mantissa bits each, both rounded to nearest
+// (adding half of the last kept place to the bits; the tensor core ignores the
+// 13 bits behind it): what is lost is below 2^-22 of x. Cutting instead of
+// rounding left errors of 2e-6 in the result, rounding leaves 4e-7.
+__device__ __forceinline__ void split_tf32(float x, uint32_t &head, uint32_t &tail) {
+  head = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+  tail = __float_as_uint(x - __uint_as_float(head)) + 0x1000u;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ float lds32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+template <typename T, int DP>
+struct Tile {
+  static constexpr bool kHalf = sizeof(T) == 2;
+  static constexpr int TOK = kHalf ? 16 : 8;        // slots per step
+  static constexpr int EPC = 16 / int(sizeof(T));   // elements per 16-byte chunk
+  static constexpr int CPR = DP / EPC;              // chunks per staged row
+  static constexpr int ROW = DP * int(sizeof(T));   // staged row bytes
+  static constexpr int STAGE = 2 * TOK * ROW;       // K and V of one step
+  // fp32 rows of 256 channels: the query's registers would not fit beside
+  // the result's, so it stays in shared memory
+  static constexpr bool kQShared = !kHalf && DP > 128;
+  static constexpr int STAGES = kQShared ? 2 : STAGE > 4096 ? 3 : 4;
+  static_assert(STAGES <= 4, "the live bits of the ring are 4 x 16");
+  static constexpr int QBYTES = kQShared ? PA_HEADS * ROW : 0;
+  static constexpr int RING = STAGES * STAGE + QBYTES;  // per warp
+};
+
+// One warp's whole work. HALF_ROWS: at most 8 heads (rows 8-15 of the tiles
+// are padding and their softmax is left out).
+template <typename T, int DP, bool HALF_ROWS>
+__global__ void __launch_bounds__(PA_WARPS * 32)
+    paged_attention_kernel(const __grid_constant__ AttnArgs p) {
+  using L = Tile<T, DP>;
+  constexpr int TOK = L::TOK, STAGES = L::STAGES, NT = DP / 8;
+  constexpr int HALVES = HALF_ROWS ? 1 : 2;
+  extern __shared__ __align__(128) uint8_t pa_smem[];
+  const wgx_kv_cache &c = p.a.cache;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  uint8_t *ring = pa_smem + size_t(warp) * L::RING;
+  uint32_t *prefix = reinterpret_cast<uint32_t *>(pa_smem + size_t(PA_WARPS) * L::RING);
+  int *lens = reinterpret_cast<int *>(prefix + c.batch + 1);
+  const int D = c.head_dim;
+  build_prefix<TOK>(p, prefix, lens);
+  if (D < DP) {
+    // chunks behind the rows' ends: read by the products (with zero queries),
+    // never loaded
+    for (int i = lane * 16; i < L::RING; i += 512)
+      *reinterpret_cast<uint4 *>(ring + i) = make_uint4(0u, 0u, 0u, 0u);
+    __syncwarp();
+  }
+  const int rows = c.kv_heads * p.chunks;
+  const uint64_t total = uint64_t(prefix[c.batch]) * uint64_t(rows);
+  const int workers = worker_count(p, total);
+  const int me = warp * int(gridDim.x) + int(blockIdx.x);
+  if (total == 0 || me >= workers) return;
+  const uint64_t begin = share_begin(total, me, workers), end = share_begin(total, me + 1, workers);
+  if (begin >= end) return;
+
+  Place ld;
+  {
+    // the sequence whose rows hold `begin`
+    const uint32_t key = uint32_t(begin / uint64_t(rows));
+    int lo = 0, hi = c.batch - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (prefix[mid] <= key) lo = mid;
+      else hi = mid - 1;
+    }
+    ld.b = lo;
+    ld.s = span_of<TOK>(p, lens[lo]);
+    const uint64_t rest = begin - uint64_t(prefix[lo]) * uint64_t(rows);
+    ld.row = int(rest / uint64_t(ld.s.steps));
+    ld.step = int(rest % uint64_t(ld.s.steps));
+  }
+  Place cur = ld;
+  uint32_t to_load = uint32_t(end - begin), to_do = to_load;
+
+  // page id, mask and slot of this lane's row (lane < TOK) of the step to be
+  // loaded next: fetched one step ahead of its use
+  int page = -1, slot = 0;
+  auto fetch = [&]() {
+    page = -1;
+    if (lane < TOK && to_load) {
+      const int t = (ld.s.first + ld.step) * TOK + lane;
+      bool live = t >= ld.s.lo && t < ld.s.len;
+      if (live && p.a.mask)
+        live = t < p.a.mask_width && p.a.mask[int64_t(ld.b) * p.a.mask_stride + t] != 0;
+      if (live) {
+        const int pi = int(uint32_t(t) / uint32_t(c.page_size));
+        slot = t - pi * c.page_size;
+        page = c.page_table[int64_t(ld.b) * c.table_stride + pi];
+        if (page < 0 || page >= c.pages) {
+          atomicOr(p.err, kErrCache);
+          page = -1;
+        }
+      }
+    }
+  };
+  uint64_t live_ring = 0;  // 16 bits of live slots per step in flight, oldest highest
+  const T *kbase = static_cast<const T *>(c.k), *vbase = static_cast<const T *>(c.v);
+  auto issue = [&](int stage) {
+    const uint32_t live = __ballot_sync(~0u, page >= 0);
+    live_ring = (live_ring << 16) | (live & 0xffffu);
+    const int h = ld.row / p.chunks;
+    const int64_t ko = page >= 0 ? int64_t(page) * c.k_page_stride + int64_t(h) * c.k_head_stride +
+                                       int64_t(slot) * c.k_slot_stride : 0;
+    const int64_t vo = page >= 0 ? int64_t(page) * c.v_page_stride + int64_t(h) * c.v_head_stride +
+                                       int64_t(slot) * c.v_slot_stride : 0;
+    uint8_t *sk = ring + stage * L::STAGE, *sv = sk + TOK * L::ROW;
+    if (p.vec) {
+      const uint32_t ska = smem_u32(sk), sva = smem_u32(sv);
+#pragma unroll
+      for (int i = 0; i < TOK * L::CPR / 32; ++i) {
+        const int idx = i * 32 + lane, r = idx / L::CPR, ch = idx % L::CPR;
+        const int64_t kr = __shfl_sync(~0u, ko, r), vr = __shfl_sync(~0u, vo, r);
+        const bool ok = (live >> r) & 1;
+        if (ch * L::EPC < D) {
+          const uint32_t d = uint32_t(r * L::ROW + ((ch ^ (r & 7)) << 4));
+          cp_async16(ska + d, kbase + kr + ch * L::EPC, ok);
+          cp_async16(sva + d, vbase + vr + ch * L::EPC, ok);
+        }
+      }
+    } else {
+      for (int r = 0; r < TOK; ++r) {
+        const int64_t kr = __shfl_sync(~0u, ko, r), vr = __shfl_sync(~0u, vo, r);
+        const bool ok = (live >> r) & 1;
+        for (int e = lane; e < D; e += 32) {
+          const int d = r * L::ROW + (((e / L::EPC) ^ (r & 7)) << 4) + (e % L::EPC) * int(sizeof(T));
+          *reinterpret_cast<T *>(sk + d) = ok ? kbase[kr + e] : T(0.f);
+          *reinterpret_cast<T *>(sv + d) = ok ? vbase[vr + e] : T(0.f);
+        }
+      }
+    }
+  };
+  auto load_next = [&](int stage) {
+    if (to_load) {
+      issue(stage);
+      next_step<TOK>(p, lens, rows, ld);
+      --to_load;
+      fetch();
+    } else {
+      live_ring <<= 16;
+    }
+    cp_commit();
+  };
+  fetch();
+#pragma unroll 1
+  for (int s = 0; s < STAGES - 1; ++s) load_next(s);
+
+  uint32_t qf[L::kQShared ? 1 : (L::kHalf ? DP / 16 : DP / 8)][4];
+  float o[NT][4];
+  float m[HALVES], l[HALVES];
+  bool row_start = true;
+  const uint32_t ring_a = smem_u32(ring);
+  int stage = 0;
+  bool from_begin = cur.step == 0;  // this share holds the row's first step
+
+  while (to_do) {
+    const int h = cur.row / p.chunks, chunk = cur.row % p.chunks;
+    if (row_start) {
+      row_start = false;
+      const int head0 = h * p.group + chunk * PA_HEADS;
+      const int nh = min(p.heads, p.group - chunk * PA_HEADS);
+      const T *q = static_cast<const T *>(p.a.q) + int64_t(cur.b) * p.a.q_batch_stride +
+                   int64_t(head0) * p.a.q_head_stride;
+      auto qv = [&](int g, int d) -> T {
+        return (g < nh && d < D) ? q[int64_t(g) * p.a.q_head_stride + d] : T(0.f);
+      };
+      const int r0 = lane >> 2, kq = lane & 3;
+      if constexpr (L::kHalf) {
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int g = r0 + (j & 1) * 8, d = kk * 16 + 2 * kq + (j >> 1) * 8;
+            const __half2 v = (j & 1) && HALF_ROWS ? __half2(T(0.f), T(0.f))
+                                                   : __half2(qv(g, d), qv(g, d + 1));
+            qf[kk][j] = *reinterpret_cast<const uint32_t *>(&v);
+          }
+      } else if constexpr (!L::kQShared) {
+#pragma unroll
+        for (int kk = 0; kk < DP / 8; ++kk)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            qf[kk][j] = (j & 1) && HALF_ROWS
+                            ? 0u
+                            : __float_as_uint(qv(r0 + (j & 1) * 8, kk * 8 + kq + (j >> 1) * 4));
+      } else {
+        __syncwarp();
+        for (int g = 0; g < PA_HEADS; ++g)
+          for (int d = lane; d < DP; d += 32)
+            *reinterpret_cast<T *>(ring + STAGES * L::STAGE + g * L::ROW +
+                                   (((d / 4) ^ (g & 7)) << 4) + (d % 4) * 4) = qv(g, d);
+        __syncwarp();
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+#pragma unroll
+      for (int x = 0; x < HALVES; ++x) m[x] = -INFINITY, l[x] = 0.f;
+    }
+    cp_wait<STAGES - 2>();
+    __syncwarp();
+    load_next(stage == 0 ? STAGES - 1 : stage - 1);
+
+    const uint32_t ka = ring_a + uint32_t(stage * L::STAGE), va = ka + uint32_t(TOK * L::ROW);
+    // after load_next the ring holds STAGES entries: this step's is the oldest
+    const uint32_t live = uint32_t(live_ring >> (16 * (STAGES - 1))) & 0xffffu;
+    // ---- scores: s[t][.] are slots t * 8 + 2 * (lane % 4) + {0, 1} of head
+    // lane / 4 ([0], [1]) and lane / 4 + 8 ([2], [3])
+    constexpr int ST = TOK / 8;
+    float s[ST][4];
+#pragma unroll
+    for (int t = 0; t < ST; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+    if constexpr (L::kHalf) {
+      const int tr = ((lane >> 4) << 3) + (lane & 7);
+#pragma unroll
+      for (int kk = 0; kk < DP / 16; ++kk) {
+        if (kk * 16 < D) {
+          uint32_t b[4];
+          ldsm4(ka + uint32_t(tr * L::ROW + (((2 * kk + ((lane >> 3) & 1)) ^ (tr & 7)) << 4)), b);
+          mma16(s[0], qf[kk], b[0], b[1]);
+          mma16(s[ST - 1], qf[kk], b[2], b[3]);
+        }
+      }
+    } else {
+      const int r = lane >> 2;
+      // the tensor core cuts its running sums instead of rounding them: the
+      // small products have a sum of their own, and the large ones two
+      float lo[4] = {0.f, 0.f, 0.f, 0.f}, odd[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kk = 0; kk < DP / 8; ++kk) {
+        if (kk * 8 < D) {
+          uint32_t a[4], ah[4], al[4], bh[2], bl[2];
+          if constexpr (L::kQShared) {
+            const uint32_t qa = ring_a + uint32_t(STAGES * L::STAGE);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int g = r + (j & 1) * 8;
+              a[j] = (j & 1) && HALF_ROWS
+                         ? 0u
+                         : __float_as_uint(lds32(qa + uint32_t(g * L::ROW + (((2 * kk + (j >> 1)) ^ (g & 7)) << 4) +
+                                                               (lane & 3) * 4)));
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) a[j] = qf[kk][j];
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if ((j & 1) && HALF_ROWS) ah[j] = al[j] = 0u;
+            else split_tf32(__uint_as_float(a[j]), ah[j], al[j]);
+          }
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            split_tf32(lds32(ka + uint32_t(r * L::ROW + (((2 * kk + j) ^ (r & 7)) << 4) + (lane & 3) * 4)),
+                       bh[j], bl[j]);
+          mma8(lo, al, bh[0], bh[1]);
+          mma8(lo, ah, bl[0], bl[1]);
+          mma8(kk & 1 ? odd : s[0], ah, bh[0], bh[1]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[0][j] += odd[j] + lo[j];
+    }
+    // ---- running softmax
+    bool grew = false;
+    float mn[HALVES];
+#pragma unroll
+    for (int x = 0; x < HALVES; ++x) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < ST; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int bit = t * 8 + 2 * (lane & 3) + e;
+          float &v = s[t][2 * x + e];
+          v = (live >> bit) & 1 ? v * p.scale2 : -INFINITY;
+          mx = fmaxf(mx, v);
+        }
+      mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
+      mn[x] = fmaxf(m[x], mx);
+      grew |= mn[x] > m[x];
+    }
+    if (p.scores) {
+      const int t0 = (cur.s.first + cur.step) * TOK + 2 * (lane & 3);
+#pragma unroll
+      for (int x = 0; x < HALVES; ++x) {
+        const int g = chunk * PA_HEADS + (lane >> 2) + 8 * x;
+        if (g < p.group) {
+          float *w = p.scores + (int64_t(cur.b) * p.a.q_heads + h * p.group + g) * p.score_stride + t0;
+#pragma unroll
+          for (int t = 0; t < ST; ++t)
+            *reinterpret_cast<float2 *>(w + t * 8) = make_float2(s[t][2 * x], s[t][2 * x + 1]);
+        }
+      }
+    }
+    if (__any_sync(~0u, grew)) {
+#pragma unroll
+      for (int x = 0; x < HALVES; ++x) {
+        const float f = mn[x] > m[x] ? exp2_approx(m[x] - mn[x]) : 1.f;
+        l[x] *= f;
+        m[x] = mn[x];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          o[n][2 * x] *= f;
+          o[n][2 * x + 1] *= f;
+        }
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < HALVES; ++x) {
+      const float mu = m[x] == -INFINITY ? 0.f : m[x];
+#pragma unroll
+      for (int t = 0; t < ST; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float &v = s[t][2 * x + e];
+          v = exp2_approx(v - mu);
+          l[x] += v;
+        }
+    }
+    if (HALF_ROWS) {
+#pragma unroll
+      for (int t = 0; t < ST; ++t) s[t][2] = s[t][3] = 0.f;
+    }
+    // ---- result += p v
+    if constexpr (L::kHalf) {
+      // the probabilities go in as a sum of two fp16 numbers: one alone would
+      // add an error as large as the output's own rounding
+      uint32_t ph[4], pl[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int t = (j >> 1) * (ST - 1), x = j & 1;
+        ph[j] = pack2(s[t][2 * x], s[t][2 * x + 1]);
+        const float2 hf = __half22float2(*reinterpret_cast<const __half2 *>(&ph[j]));
+        pl[j] = pack2(s[t][2 * x] - hf.x, s[t][2 * x + 1] - hf.y);
+      }
+      const int tr = (((lane >> 3) & 1) << 3) + (lane & 7);
+#pragma unroll
+      for (int n = 0; n < NT / 2; ++n) {
+        if (n * 16 < D) {
+          uint32_t b[4];
+          ldsm4_t(va + uint32_t(tr * L::ROW + (((2 * n + (lane >> 4)) ^ (tr & 7)) << 4)), b);
+          mma16(o[2 * n], ph, b[0], b[1]);
+          mma16(o[2 * n + 1], ph, b[2], b[3]);
+          mma16(o[2 * n], pl, b[0], b[1]);
+          mma16(o[2 * n + 1], pl, b[2], b[3]);
+        }
+      }
+    } else {
+      // the k index of the product runs over the slots in the order 0, 2, 4,
+      // 6, 1, 3, 5, 7, which is how the scores' accumulator holds them
+      uint32_t ah[4], al[4];
+      split_tf32(s[0][0], ah[0], al[0]);
+      split_tf32(s[0][2], ah[1], al[1]);
+      split_tf32(s[0][1], ah[2], al[2]);
+      split_tf32(s[0][3], ah[3], al[3]);
+      const int t0 = 2 * (lane & 3);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        if (n * 8 < D) {
+          uint32_t bh[2], bl[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int t = t0 + j;
+            split_tf32(lds32(va + uint32_t(t * L::ROW + (((2 * n + (lane >> 4)) ^ (t & 7)) << 4) +
+                                           ((lane >> 2) & 3) * 4)),
+                       bh[j], bl[j]);
+          }
+          // a sum of its own per step, added in fp32 with rounding: cut sums
+          // drift over thousands of slots
+          float acc[4] = {0.f, 0.f, 0.f, 0.f};
+          mma8(acc, al, bh[0], bh[1]);
+          mma8(acc, ah, bl[0], bl[1]);
+          mma8(acc, ah, bh[0], bh[1]);
+#pragma unroll
+          for (int j = 0; j < 2 * HALVES; ++j) o[n][j] += acc[j];
+        }
+      }
+    }
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
+    --to_do;
+    const bool row_end = cur.step + 1 == cur.s.steps;
+    if (row_end || to_do == 0) {
+      const int nh = min(p.heads, p.group - chunk * PA_HEADS);
+      const bool whole = from_begin && row_end;
+#pragma unroll
+      for (int x = 0; x < HALVES; ++x) {
+        float sum = l[x];
+        sum += __shfl_xor_sync(~0u, sum, 1);
+        sum += __shfl_xor_sync(~0u, sum, 2);
+        const int g = (lane >> 2) + 8 * x;
+        if (g >= nh) continue;
+        if (whole) {
+          const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+          T *out = static_cast<T *>(p.a.out) + int64_t(cur.b) * p.a.out_batch_stride +
+                   int64_t(h * p.group + chunk * PA_HEADS + g) * p.a.out_head_stride;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int d = n * 8 + 2 * (lane & 3) + e;
+              if (d < D) out[d] = T(o[n][2 * x + e] * inv);
+            }
+          if (p.stats && (lane & 3) == 0)
+            p.stats[(int64_t(cur.b) * rows + cur.row) * PA_HEADS + g] = make_float2(m[x], sum);
+        } else {
+          const int64_t part = (int64_t(me) * 2 + (from_begin ? 1 : 0)) * p.heads + g;
+          float *po = p.part_o + part * D;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int d = n * 8 + 2 * (lane & 3) + e;
+              if (d < D) po[d] = o[n][2 * x + e];
+            }
+          if ((lane & 3) == 0) p.part_ml[part] = make_float2(m[x], sum);
+        }
+      }
+      row_start = true;
+      from_begin = true;  // the next row begins within this share
+    }
+    next_step<TOK>(p, lens, rows, cur);
+  }
+  cp_wait<0>();
+}
+
+// Rows cut between warps: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i.
+// Block (b * kv_heads + h, y): y < group joins that query head; with
+// accumulation every y also adds the probabilities of its slots.
+template <typename T, int TOK>
+__global__ void __launch_bounds__(PA_JOIN_THREADS) join_kernel(const __grid_constant__ AttnArgs p) {
+  extern __shared__ __align__(16) uint8_t jn_smem[];
+  __shared__ float head_m[PA_MAX_GROUP], head_inv[PA_MAX_GROUP];
+  const wgx_kv_cache &c = p.a.cache;
+  uint32_t *prefix = reinterpret_cast<uint32_t *>(jn_smem);
+  int *lens = reinterpret_cast<int *>(prefix + c.batch + 1);
+  build_prefix<TOK>(p, prefix, lens);
+  const int b = blockIdx.x / c.kv_heads, h = blockIdx.x % c.kv_heads, y = blockIdx.y;
+  const int rows = c.kv_heads * p.chunks, D = c.head_dim;
+  const uint64_t total = uint64_t(prefix[c.batch]) * uint64_t(rows);
+  const int workers = worker_count(p, total);
+  const Span s = span_of<TOK>(p, lens[b]);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+  // where chunk's row lies in the line, and the warps that worked on it
+  auto locate = [&](int chunk, uint64_t &r0, int &w0, int &w1) {
+    r0 = uint64_t(prefix[b]) * uint64_t(rows) + uint64_t(h * p.chunks + chunk) * uint64_t(s.steps);
+    w0 = worker_of(r0, total, workers);
+    w1 = worker_of(r0 + uint64_t(s.steps) - 1, total, workers);
+  };
+  // row `g` of worker w's partial result of the row that starts at r0
+  auto part_of = [&](int w, uint64_t r0, int g) {
+    return (int64_t(w) * 2 + (share_begin(total, w, workers) > r0 ? 0 : 1)) * p.heads + g;
+  };
+
+  if (y < p.group) {
+    const int chunk = y / PA_HEADS, g = y % PA_HEADS;
+    T *out = static_cast<T *>(p.a.out) + int64_t(b) * p.a.out_batch_stride +
+             int64_t(h * p.group + y) * p.a.out_head_stride;
+    if (s.steps <= 0) {
+      for (int d = threadIdx.x; d < D; d += PA_JOIN_THREADS) out[d] = T(0.f);
+    } else {
+      uint64_t r0;
+      int w0, w1;
+      locate(chunk, r0, w0, w1);
+      if (w0 != w1) {
+        float M = -INFINITY;
+        for (int w = w0; w <= w1; ++w) M = fmaxf(M, p.part_ml[part_of(w, r0, g)].x);
+        const float mu = M == -INFINITY ? 0.f : M;
+        float sum = 0.f;
+        for (int w = w0; w <= w1; ++w) {
+          const float2 ml = p.part_ml[part_of(w, r0, g)];
+          sum += ml.y * exp2_approx(ml.x - mu);
+        }
+        const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+        for (int d = threadIdx.x; d < D; d += PA_JOIN_THREADS) {
+          float acc = 0.f;
+          for (int w = w0; w <= w1; ++w) {
+            const int64_t part = part_of(w, r0, g);
+            acc += p.part_o[part * D + d] * exp2_approx(p.part_ml[part].x - mu);
+          }
+          out[d] = T(acc * inv);
+        }
+      }
+    }
+  }
+  if (!p.a.weights_out) return;
+  const int t0 = y * PA_JOIN_SLOTS;
+  const int t1 = min(t0 + PA_JOIN_SLOTS, int(min(int64_t(s.len), p.a.slots)));
+  if (t0 >= t1) return;
+  for (int g = warp; g < p.group; g += PA_JOIN_THREADS / 32) {
+    const int chunk = g / PA_HEADS, gr = g % PA_HEADS;
+    uint64_t r0;
+    int w0, w1;
+    locate(chunk, r0, w0, w1);
+    float M, sum;
+    if (w0 == w1) {
+      const float2 ml = p.stats[(int64_t(b) * rows + h * p.chunks + chunk) * PA_HEADS + gr];
+      M = ml.x;
+      sum = ml.y;
+    } else {
+      M = -INFINITY;
+      for (int w = w0 + lane; w <= w1; w += 32) M = fmaxf(M, p.part_ml[part_of(w, r0, gr)].x);
+#pragma unroll
+      for (int d = 16; d; d /= 2) M = fmaxf(M, __shfl_xor_sync(~0u, M, d));
+      const float mu = M == -INFINITY ? 0.f : M;
+      sum = 0.f;
+      for (int w = w0 + lane; w <= w1; w += 32) {
+        const float2 ml = p.part_ml[part_of(w, r0, gr)];
+        sum += ml.y * exp2_approx(ml.x - mu);
+      }
+#pragma unroll
+      for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
+    }
+    if (lane == 0) {
+      head_m[g] = M == -INFINITY ? 0.f : M;
+      head_inv[g] = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    }
+  }
+  __syncthreads();
+  const int64_t at = (int64_t(b) * c.kv_heads + h) * p.a.slots;
+  const float *sc = p.scores + (int64_t(b) * p.a.q_heads + h * p.group) * p.score_stride;
+  for (int t = t0 + threadIdx.x; t < t1; t += PA_JOIN_THREADS) {
+    float w = p.a.weights[at + t];
+    if (t >= s.lo)
+      for (int g = 0; g < p.group; ++g)
+        w += exp2_approx(sc[int64_t(g) * p.score_stride + t] - head_m[g]) * head_inv[g];
+    p.a.weights_out[at + t] = w;
+  }
+}
+
+struct Config {
+  const void *kernel;
+  int smem, ring, tok, ctas_per_sm;
+};
+
+template <typename T, int DP, bool HALF_ROWS>
+Config make_config() {
+  Config c{};
+  c.kernel = reinterpret_cast<const void *>(paged_attention_kernel<T, DP, HALF_ROWS>);
+  c.ring = PA_WARPS * Tile<T, DP>::RING;
+  c.tok = Tile<T, DP>::TOK;
+  return c;
+}
+
+constexpr int kPaMaxBatch = 2048;
+inline int prefix_bytes(int batch) { return (2 * batch + 1) * 4; }
+
+// The kernel for a call's type, head size and group; its attributes are set
+// and its occupancy read once per device.
+const Config &config_for(int dtype, int head_dim, bool half_rows) {
+  static std::mutex mu;
+  static Config table[64][12];
+  static bool ready[64][12] = {};
+  const int dev = current_device();
+  if (dev >= 64) fail("paged_attention: device ordinal out of range");
+  const int dp = head_dim <= 64 ? 0 : head_dim <= 128 ? 1 : 2;
+  const int k = ((dtype == WGX_FLOAT16 ? 0 : 3) + dp) * 2 + (half_rows ? 1 : 0);
+  std::lock_guard<std::mutex> lock(mu);
+  if (!ready[dev][k]) {
+    Config c{};
+    switch (k) {
+      case 0: c = make_config<__half, 64, false>(); break;
+      case 1: c = make_config<__half, 64, true>(); break;
+      case 2: c = make_config<__half, 128, false>(); break;
+      case 3: c = make_config<__half, 128, true>(); break;
+      case 4: c = make_config<__half, 256, false>(); break;
+      case 5: c = make_config<__half, 256, true>(); break;
+      case 6: c = make_config<float, 64, false>(); break;
+      case 7: c = make_config<float, 64, true>(); break;
+      case 8: c = make_config<float, 128, false>(); break;
+      case 9: c = make_config<float, 128, true>(); break;
+      case 10: c = make_config<float, 256, false>(); break;
+      default: c = make_config<float, 256, true>(); break;
+    }
+    const int most = c.ring + prefix_bytes(kPaMaxBatch);
+    check_cuda(cudaFuncSetAttribute(c.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    std::min(most, 227 * 1024)),
+               "paged_attention smem attr");
+    check_cuda(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&c.ctas_per_sm, c.kernel, PA_WARPS * 32,
+                                                             c.ring + prefix_bytes(256)),
+               "paged_attention occupancy");
+    if (c.ctas_per_sm < 1) c.ctas_per_sm = 1;
+    table[dev][k] = c;
+    ready[dev][k] = true;
+  }
+  return table[dev][k];
+}
+
+uint64_t align256(uint64_t x) { return (x + 255) / 256 * 256; }
+
+struct Layout {
+  AttnArgs p;
+  int grid;
+  const Config *cfg;
+  uint64_t bytes;
+};
+
+Layout layout_of(const wgx_paged_attention_args &a) {
+  Layout l{};
+  AttnArgs &p = l.p;
+  const wgx_kv_cache &c = a.cache;
+  p.a = a;
+  p.capacity = cache_capacity(c);
+  p.group = a.q_heads / c.kv_heads;
+  p.chunks = (p.group + PA_HEADS - 1) / PA_HEADS;
+  p.heads = std::min(p.group, PA_HEADS);
+  p.vec = cache_rows_16b(c);
+  p.scale2 = a.scale * 1.4426950408889634f;
+  l.cfg = &config_for(c.dtype, c.head_dim, p.heads <= 8);
+  p.min_steps = 64 / l.cfg->tok;
+  const uint64_t steps = uint64_t((p.capacity + l.cfg->tok - 1) / l.cfg->tok) * c.batch *
+                         uint64_t(c.kv_heads) * p.chunks;
+  const uint64_t want = (steps + p.min_steps - 1) / p.min_steps;
+  const int resident = device_sm_count() * l.cfg->ctas_per_sm;
+  p.max_workers = int(std::min<uint64_t>(std::max<uint64_t>(want, 1), uint64_t(resident) * PA_WARPS));
+  l.grid = std::min(resident, p.max_workers);
+  uint64_t off = 0;
+  const uint64_t parts = uint64_t(p.max_workers) * 2 * p.heads;
+  auto take = [&](uint64_t bytes) {
+    const uint64_t at = off;
+    off += align256(bytes);
+    return static_cast<uint8_t *>(a.scratch) + at;
+  };
+  p.part_o = reinterpret_cast<float *>(take(parts * c.head_dim * 4));
+  p.part_ml = reinterpret_cast<float2 *>(take(parts * 8));
+  if (a.weights_out) {
+    p.stats = reinterpret_cast<float2 *>(take(uint64_t(c.batch) * c.kv_heads * p.chunks * PA_HEADS * 8));
+    p.score_stride = (p.capacity + 15) / 16 * 16;
+    p.scores = reinterpret_cast<float *>(take(uint64_t(c.batch) * a.q_heads * p.score_stride * 4));
+  }
+  l.bytes = off;
+  return l;
+}
+
+}  // namespace
+
+uint64_t paged_attention_scratch_bytes(const wgx_paged_attention_args &a) { return layout_of(a).bytes; }
+
+void launch_paged_attention(const wgx_paged_attention_args &a, cudaStream_t stream) {
+  Layout l = layout_of(a);
+  if (a.scratch_bytes < l.bytes || (reinterpret_cast<uintptr_t>(a.scratch) & 255))
+    fail("paged_attention: scratch of " + std::to_string(l.bytes) + " bytes, 256-byte aligned, needed");
+  l.p.err = device_error_word(current_device());
+  const wgx_kv_cache &c = a.cache;
+  void *args[] = {&l.p};
+  const int pre = prefix_bytes(c.batch);
+  const int th = timer_begin("paged_attention_kernel", stream);
+  check_cuda(cudaLaunchKernel(l.cfg->kernel, dim3(unsigned(l.grid)), dim3(PA_WARPS * 32), args,
+                              size_t(l.cfg->ring + pre), stream),
+             "paged_attention launch");
+  timer_end(th, stream);
+  int pieces = l.p.group;
+  if (a.weights_out)
+    pieces = std::max<int>(pieces, int((l.p.capacity + PA_JOIN_SLOTS - 1) / PA_JOIN_SLOTS));
+  const dim3 grid(unsigned(c.batch) * unsigned(c.kv_heads), unsigned(pieces));
+  if (c.dtype == WGX_FLOAT16)
+    join_kernel<__half, 16><<<grid, PA_JOIN_THREADS, size_t(pre), stream>>>(l.p);
+  else
+    join_kernel<float, 8><<<grid, PA_JOIN_THREADS, size_t(pre), stream>>>(l.p);
+  check_cuda(cudaGetLastError(), "paged_attention join launch");
+}
+
+}  // namespace wgx

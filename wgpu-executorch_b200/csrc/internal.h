@@ -7,8 +7,10 @@
 
 #include <cmath>
 #include <cstdint>
+#include <exception>
 #include <functional>
 #include <memory>
+#include <new>
 #include <string>
 #include <unordered_map>
 #include <utility>
@@ -33,6 +35,22 @@ struct Error {
 [[noreturn]] void fail(const std::string &msg, int code = WGX_ERR_INVALID);
 void check_cuda(cudaError_t e, const char *what);
 
+// Wrap a C-ABI body: Error -> status code + message.
+template <class F>
+int guarded(F &&f) {
+  try {
+    clear_error();
+    f();
+    return WGX_OK;
+  } catch (const Error &e) {
+    return set_error(e.code, e.msg);
+  } catch (const std::bad_alloc &) {
+    return set_error(WGX_ERR_NOMEM, "host allocation failed");
+  } catch (const std::exception &e) {
+    return set_error(WGX_ERR_INVALID, e.what());
+  }
+}
+
 int dtype_size(int dtype);
 const char *dtype_name(int dtype);
 
@@ -44,6 +62,7 @@ enum DeviceErrorBits : uint32_t {
   kErrEpilogueTimeout = 1u << 2,
   kErrTmemAlloc = 1u << 3,
   kErrBounds = 1u << 4,  // bounds-checking build: an access outside its buffer was skipped
+  kErrCache = 1u << 5,   // a page id or length outside its cache was left out
 };
 
 // Bounds-checking debug build (-DWGX_BOUNDS; `make bounds` builds

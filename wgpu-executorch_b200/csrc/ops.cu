@@ -416,6 +416,8 @@ static void record_conv_with_clamp(wgx_context *ctx, const std::vector<wgx_arg> 
 // ops_elementwise.cu; whole-program data-movement ops in ops_data.cu.
 void register_elementwise_ops(std::unordered_map<std::string, OpRecorder> &reg);
 void register_data_ops(std::unordered_map<std::string, OpRecorder> &reg);
+// Text decoding over a paged cache (ops_decode.cu).
+void register_decode_ops(std::unordered_map<std::string, OpRecorder> &reg);
 
 const std::unordered_map<std::string, OpRecorder> &op_registry() {
   static const std::unordered_map<std::string, OpRecorder> reg = [] {
@@ -427,6 +429,7 @@ const std::unordered_map<std::string, OpRecorder> &op_registry() {
     r["et_vk.conv_with_clamp.default"] = record_conv_with_clamp;
     register_elementwise_ops(r);
     register_data_ops(r);
+    register_decode_ops(r);
     return r;
   }();
   return reg;

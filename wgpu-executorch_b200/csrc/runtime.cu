@@ -166,22 +166,6 @@ void wgx_context::invalidate_graph() {
   graph_valid = false;
 }
 
-// Wrap a C-ABI body: Error -> status code + message.
-template <class F>
-static int guarded(F &&f) {
-  try {
-    clear_error();
-    f();
-    return WGX_OK;
-  } catch (const Error &e) {
-    return set_error(e.code, e.msg);
-  } catch (const std::bad_alloc &) {
-    return set_error(WGX_ERR_NOMEM, "host allocation failed");
-  } catch (const std::exception &e) {
-    return set_error(WGX_ERR_INVALID, e.what());
-  }
-}
-
 static void assert_alive(const wgx_context *ctx) {
   if (!ctx) fail("null context");
   if (ctx->destroyed) fail("WgpuExecutionContext is destroyed", WGX_ERR_DESTROYED);
@@ -556,8 +540,9 @@ int wgx_sync(wgx_context *ctx) {
       uint32_t zero = 0;
       cudaMemcpy(w, &zero, 4, cudaMemcpyHostToDevice);
       fail("device reported error code " + std::to_string(code) +
-               ((code & kErrBounds) ? " (an access outside its buffer was skipped)"
-                                    : " (a bounded wait inside a kernel ran out)"),
+               ((code & kErrBounds)  ? " (an access outside its buffer was skipped)"
+                : (code & kErrCache) ? " (a page id or length outside its cache was left out)"
+                                     : " (a bounded wait inside a kernel ran out)"),
            WGX_ERR_DEVICE);
     }
   });

@@ -253,7 +253,8 @@ _CONV_VARIANTS = {
 
 class _Shaders:
     """``shaders`` namespace (src/shaders/index.ts:39-60): every operator of
-    the reference's registry, recorded through wgx_record_op."""
+    the reference's registry, recorded through wgx_record_op, and the
+    text-decoding operators."""
     mm = _native_shader("aten.mm.default", {"umma": "tcgen05 GEMM (fp16)",
                                             "simt": "FFMA GEMM (fp32)"})
     convolution = _native_shader("aten.convolution.default", _CONV_VARIANTS)
@@ -286,6 +287,13 @@ class _Shaders:
     squeezeCopy = _native_shader("aten.squeeze_copy.dims", {"flatCopy": ""})
     unsqueezeCopy = _native_shader("aten.unsqueeze_copy.default", {"flatCopy": ""})
     prepack = _native_shader("et_vk.prepack.default", {"flatCopy": ""})
+    # text decoding over a paged key/value cache (no counterpart in the
+    # reference's registry); wgx.decode has the same operators as direct calls
+    kvAppend = _native_shader("wgx.kv_append.default", {"vec16": "16-byte rows", "generic": ""})
+    pagedAttention = _native_shader("wgx.paged_attention.default",
+                                    {"f16": "split over the cache, joined", "f32": "3xTF32"})
+    cacheEvict = _native_shader("wgx.cache_evict.default", {"cluster": "radix selection"})
+    beamSearchStep = _native_shader("wgx.beam_search_step.default", {"chunked": ""})
 
     def __iter__(self):
         for k, v in vars(type(self)).items():
