@@ -2,9 +2,19 @@
 // kernels (decode_attention.cu, decode_cache.cu, decode_beam.cu) and their
 // front end (ops_decode.cu: checks, C entry points, recorders).
 #pragma once
+#include <cuda.h>
+
 #include "internal.h"
 
 namespace wgx {
+
+// 5-D map over the rows of a cache's K or V: dimension 0 the channels (all of
+// them, or with panels > 1 one 128-byte panel), 1 a page's slots, 2 the panels,
+// 3 the heads, 4 the pages; box = one panel's width x `rows` slots x panels,
+// 128-byte swizzle, zeros behind a row's end. False when the driver does not
+// take the strides.
+bool encode_rows_tmap(CUtensorMap *map, const void *base, const wgx_kv_cache &c, int64_t page_stride,
+                      int64_t head_stride, int64_t slot_stride, int panels, int rows);
 
 // All enqueue on `stream`, expect checked arguments and throw Error when a
 // launch fails.

@@ -29,6 +29,7 @@
 
 #include "decode.h"
 #include "tcgen05.h"
+#include "tma.h"
 
 namespace wgx {
 
@@ -37,10 +38,11 @@ namespace {
 constexpr int PA_WARPS = 4;
 constexpr int PA_HEADS = 16;        // rows of an mma tile
 constexpr int PA_MAX_GROUP = 128;   // query heads per K/V head
-constexpr int PA_JOIN_THREADS = 128;
+constexpr int PA_JOIN_THREADS = 256;
 constexpr int PA_JOIN_SLOTS = 1024;  // slots per join block of the accumulation
 
 struct AttnArgs {
+  CUtensorMap k_map, v_map;  // where tma: [page][head][slot][channel] in boxes of TOK rows
   wgx_paged_attention_args a;
   int64_t capacity;   // slots a table can name
   int group;          // query heads per K/V head
@@ -48,6 +50,9 @@ struct AttnArgs {
   int max_workers;    // warps the scratch has room for
   int min_steps;      // steps a warp takes at least
   int vec;            // rows move in 16-byte units
+  int tma;            // a step's rows lie in one page and move by TMA
+  int boxes;          // TMA copies per operand and step
+  int q_pairs;        // queries can be read two elements at a time
   float scale2;       // scale * log2(e): the softmax runs in base 2
   float *part_o;      // [worker][2][heads][head_dim]
   float2 *part_ml;    // [worker][2][heads] (max, sum)
@@ -124,32 +129,10 @@ __device__ __forceinline__ int worker_of(uint64_t s, uint64_t total, int workers
   return int(((s + 1) * uint64_t(workers) - 1) / total);
 }
 
-// A place in the line of work.
-struct Place {
-  int b, row, step;  // row: kv_head * chunks + chunk; step within the row
-  Span s;
-};
-template <int TOK>
-__device__ __forceinline__ void next_step(const AttnArgs &p, const int *lens, int rows, Place &w) {
-  if (++w.step < w.s.steps) return;
-  w.step = 0;
-  if (++w.row < rows) return;
-  w.row = 0;
-  while (++w.b < p.a.cache.batch) {
-    w.s = span_of<TOK>(p, lens[w.b]);
-    if (w.s.steps > 0) return;
-  }
-}
-
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
                "r"(live ? 16 : 0)
                : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
@@ -215,6 +198,61 @@ struct Tile {
   static_assert(STAGES <= 4, "the live bits of the ring are 4 x 16");
   static constexpr int QBYTES = kQShared ? PA_HEADS * ROW : 0;
   static constexpr int RING = STAGES * STAGE + QBYTES;  // per warp
+  // Byte of chunk c of row r: panels of 128 bytes x TOK rows, chunks of a row
+  // permuted by the row's low bits (the 128-byte swizzle of a TMA copy), so
+  // that eight rows' equal chunks lie in different banks.
+  __device__ static constexpr uint32_t at(int r, int c) {
+    return uint32_t((c >> 3) * (TOK * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+  }
+};
+
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const void *map, int x, int y, int z, int w,
+                                            int v, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v), "r"(bar)
+      : "memory");
+}
+// arrives on `bar` when this thread's cp.async copies so far have landed
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// The steps of a warp's share, from the line's place `begin` on.
+template <int TOK>
+struct Walk {
+  int b, row, step;  // row: kv_head * chunks + chunk
+  Span s;
+
+  __device__ __forceinline__ void start(const AttnArgs &p, const uint32_t *prefix, const int *lens,
+                                        int rows, uint64_t begin) {
+    // the sequence whose rows hold `begin`
+    const uint32_t key = uint32_t(begin / uint64_t(rows));
+    int lo = 0, hi = p.a.cache.batch - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (prefix[mid] <= key) lo = mid;
+      else hi = mid - 1;
+    }
+    b = lo;
+    s = span_of<TOK>(p, lens[lo]);
+    const uint64_t rest = begin - uint64_t(prefix[lo]) * uint64_t(rows);
+    row = int(rest / uint64_t(s.steps));
+    step = int(rest - uint64_t(row) * uint64_t(s.steps));
+  }
+  __device__ __forceinline__ void next_row(const AttnArgs &p, const int *lens, int rows) {
+    step = 0;
+    if (++row < rows) return;
+    row = 0;
+    while (++b < p.a.cache.batch) {
+      s = span_of<TOK>(p, lens[b]);
+      if (s.steps > 0) return;
+    }
+  }
 };
 
 // One warp's whole work. HALF_ROWS: at most 8 heads (rows 8-15 of the tiles
@@ -225,19 +263,28 @@ __global__ void __launch_bounds__(PA_WARPS * 32)
   using L = Tile<T, DP>;
   constexpr int TOK = L::TOK, STAGES = L::STAGES, NT = DP / 8;
   constexpr int HALVES = HALF_ROWS ? 1 : 2;
-  extern __shared__ __align__(128) uint8_t pa_smem[];
+  constexpr uint32_t FULL = (1u << TOK) - 1;
+  extern __shared__ uint8_t pa_smem_raw[];
+  __shared__ __align__(8) uint64_t bars[PA_WARPS][STAGES];
+  uint8_t *pa_smem = reinterpret_cast<uint8_t *>(
+      (reinterpret_cast<uintptr_t>(pa_smem_raw) + 1023) & ~uintptr_t(1023));
   const wgx_kv_cache &c = p.a.cache;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   uint8_t *ring = pa_smem + size_t(warp) * L::RING;
   uint32_t *prefix = reinterpret_cast<uint32_t *>(pa_smem + size_t(PA_WARPS) * L::RING);
   int *lens = reinterpret_cast<int *>(prefix + c.batch + 1);
   const int D = c.head_dim;
+  if (lane == 0) {
+    for (int s = 0; s < STAGES; ++s) mbar_init(smem_u32(&bars[warp][s]), p.tma ? 1 : 32);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
   build_prefix<TOK>(p, prefix, lens);
   if (D < DP) {
     // chunks behind the rows' ends: read by the products (with zero queries),
     // never loaded
     for (int i = lane * 16; i < L::RING; i += 512)
       *reinterpret_cast<uint4 *>(ring + i) = make_uint4(0u, 0u, 0u, 0u);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncwarp();
   }
   const int rows = c.kv_heads * p.chunks;
@@ -248,92 +295,108 @@ __global__ void __launch_bounds__(PA_WARPS * 32)
   const uint64_t begin = share_begin(total, me, workers), end = share_begin(total, me + 1, workers);
   if (begin >= end) return;
 
-  Place ld;
-  {
-    // the sequence whose rows hold `begin`
-    const uint32_t key = uint32_t(begin / uint64_t(rows));
-    int lo = 0, hi = c.batch - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) / 2;
-      if (prefix[mid] <= key) lo = mid;
-      else hi = mid - 1;
-    }
-    ld.b = lo;
-    ld.s = span_of<TOK>(p, lens[lo]);
-    const uint64_t rest = begin - uint64_t(prefix[lo]) * uint64_t(rows);
-    ld.row = int(rest / uint64_t(ld.s.steps));
-    ld.step = int(rest % uint64_t(ld.s.steps));
-  }
-  Place cur = ld;
+  // ---- loads. The next step's page (and, with scattered rows, this lane's
+  // slot) is fetched one step ahead of its use.
+  Walk<TOK> ld;
+  ld.start(p, prefix, lens, rows, begin);
+  Walk<TOK> cur = ld;
   uint32_t to_load = uint32_t(end - begin), to_do = to_load;
-
-  // page id, mask and slot of this lane's row (lane < TOK) of the step to be
-  // loaded next: fetched one step ahead of its use
+  int head = ld.row / p.chunks;
   int page = -1, slot = 0;
+  uint32_t bits = 0;  // live slots of the next step
   auto fetch = [&]() {
+    if (!to_load) return;
+    const int t0 = (ld.s.first + ld.step) * TOK, t = t0 + lane;
+    bool live = lane < TOK && t >= ld.s.lo && t < ld.s.len;
+    if (p.a.mask && live)
+      live = t < p.a.mask_width && p.a.mask[int64_t(ld.b) * p.a.mask_stride + t] != 0;
+    bits = __ballot_sync(~0u, live);
     page = -1;
-    if (lane < TOK && to_load) {
-      const int t = (ld.s.first + ld.step) * TOK + lane;
-      bool live = t >= ld.s.lo && t < ld.s.len;
-      if (live && p.a.mask)
-        live = t < p.a.mask_width && p.a.mask[int64_t(ld.b) * p.a.mask_stride + t] != 0;
-      if (live) {
-        const int pi = int(uint32_t(t) / uint32_t(c.page_size));
-        slot = t - pi * c.page_size;
-        page = c.page_table[int64_t(ld.b) * c.table_stride + pi];
-        if (page < 0 || page >= c.pages) {
-          atomicOr(p.err, kErrCache);
-          page = -1;
-        }
-      }
+    const int32_t *table = c.page_table + int64_t(ld.b) * c.table_stride;
+    if (p.tma) {
+      const int pi = int(uint32_t(t0) / uint32_t(c.page_size));
+      slot = t0 - pi * c.page_size;
+      if (bits) page = table[pi];
+    } else if (live) {
+      const int pi = int(uint32_t(t) / uint32_t(c.page_size));
+      slot = t - pi * c.page_size;
+      page = table[pi];
     }
   };
   uint64_t live_ring = 0;  // 16 bits of live slots per step in flight, oldest highest
   const T *kbase = static_cast<const T *>(c.k), *vbase = static_cast<const T *>(c.v);
   auto issue = [&](int stage) {
-    const uint32_t live = __ballot_sync(~0u, page >= 0);
-    live_ring = (live_ring << 16) | (live & 0xffffu);
-    const int h = ld.row / p.chunks;
-    const int64_t ko = page >= 0 ? int64_t(page) * c.k_page_stride + int64_t(h) * c.k_head_stride +
-                                       int64_t(slot) * c.k_slot_stride : 0;
-    const int64_t vo = page >= 0 ? int64_t(page) * c.v_page_stride + int64_t(h) * c.v_head_stride +
-                                       int64_t(slot) * c.v_slot_stride : 0;
+    const bool bad = uint32_t(page) >= uint32_t(c.pages);
+    if (p.tma) {
+      if (bad && bits) {
+        if (lane == 0) atomicOr(p.err, kErrCache);
+        bits = 0;
+      }
+    } else {
+      const bool was = (bits >> lane) & 1;
+      if (was && bad) atomicOr(p.err, kErrCache);
+      bits = __ballot_sync(~0u, was && !bad);
+    }
+    live_ring = (live_ring << 16) | bits;
+    if (!bits) return;  // nothing to load: the step is passed over
     uint8_t *sk = ring + stage * L::STAGE, *sv = sk + TOK * L::ROW;
+    const uint32_t bar = smem_u32(&bars[warp][stage]);
+    if (p.tma) {
+      if (lane == 0) {
+        const uint32_t ska = smem_u32(sk), sva = smem_u32(sv);
+        constexpr int PANEL = 128 / int(sizeof(T));
+        // (a box counts in full, its part outside the tensor too)
+        mbar_expect_tx(bar, uint32_t(2 * TOK * 128) * uint32_t((D + PANEL - 1) / PANEL));
+        for (int j = 0; j < p.boxes; ++j) {
+          tma_load_5d(ska + uint32_t(j * TOK * 128), &p.k_map, j * PANEL, slot, 0, head, page, bar);
+          tma_load_5d(sva + uint32_t(j * TOK * 128), &p.v_map, j * PANEL, slot, 0, head, page, bar);
+        }
+      }
+      return;
+    }
+    const bool live = (bits >> lane) & 1;
+    const int64_t ko = live ? int64_t(page) * c.k_page_stride + int64_t(head) * c.k_head_stride +
+                                  int64_t(slot) * c.k_slot_stride : 0;
+    const int64_t vo = live ? int64_t(page) * c.v_page_stride + int64_t(head) * c.v_head_stride +
+                                  int64_t(slot) * c.v_slot_stride : 0;
     if (p.vec) {
       const uint32_t ska = smem_u32(sk), sva = smem_u32(sv);
-#pragma unroll
+#pragma unroll 4
       for (int i = 0; i < TOK * L::CPR / 32; ++i) {
         const int idx = i * 32 + lane, r = idx / L::CPR, ch = idx % L::CPR;
         const int64_t kr = __shfl_sync(~0u, ko, r), vr = __shfl_sync(~0u, vo, r);
-        const bool ok = (live >> r) & 1;
+        const bool ok = (bits >> r) & 1;
         if (ch * L::EPC < D) {
-          const uint32_t d = uint32_t(r * L::ROW + ((ch ^ (r & 7)) << 4));
-          cp_async16(ska + d, kbase + kr + ch * L::EPC, ok);
-          cp_async16(sva + d, vbase + vr + ch * L::EPC, ok);
+          cp_async16(ska + L::at(r, ch), kbase + kr + ch * L::EPC, ok);
+          cp_async16(sva + L::at(r, ch), vbase + vr + ch * L::EPC, ok);
         }
       }
+      cp_async_arrive(bar);
     } else {
       for (int r = 0; r < TOK; ++r) {
         const int64_t kr = __shfl_sync(~0u, ko, r), vr = __shfl_sync(~0u, vo, r);
-        const bool ok = (live >> r) & 1;
+        const bool ok = (bits >> r) & 1;
         for (int e = lane; e < D; e += 32) {
-          const int d = r * L::ROW + (((e / L::EPC) ^ (r & 7)) << 4) + (e % L::EPC) * int(sizeof(T));
+          const uint32_t d = L::at(r, e / L::EPC) + uint32_t(e % L::EPC) * uint32_t(sizeof(T));
           *reinterpret_cast<T *>(sk + d) = ok ? kbase[kr + e] : T(0.f);
           *reinterpret_cast<T *>(sv + d) = ok ? vbase[vr + e] : T(0.f);
         }
       }
+      mbar_arrive(bar);
     }
   };
   auto load_next = [&](int stage) {
-    if (to_load) {
-      issue(stage);
-      next_step<TOK>(p, lens, rows, ld);
-      --to_load;
-      fetch();
-    } else {
+    if (!to_load) {
       live_ring <<= 16;
+      return;
     }
-    cp_commit();
+    issue(stage);
+    --to_load;
+    if (++ld.step == ld.s.steps) {
+      ld.next_row(p, lens, rows);
+      head = ld.row / p.chunks;
+    }
+    fetch();
   };
   fetch();
 #pragma unroll 1
@@ -341,20 +404,19 @@ __global__ void __launch_bounds__(PA_WARPS * 32)
 
   uint32_t qf[L::kQShared ? 1 : (L::kHalf ? DP / 16 : DP / 8)][4];
   float o[NT][4];
-  float m[HALVES], l[HALVES];
-  bool row_start = true;
   const uint32_t ring_a = smem_u32(ring);
   int stage = 0;
-  bool from_begin = cur.step == 0;  // this share holds the row's first step
+  uint32_t phase = 0;  // bit s: parity of stage s's next wait
+  bool ok = true;
 
-  while (to_do) {
-    const int h = cur.row / p.chunks, chunk = cur.row % p.chunks;
-    if (row_start) {
-      row_start = false;
-      const int head0 = h * p.group + chunk * PA_HEADS;
-      const int nh = min(p.heads, p.group - chunk * PA_HEADS);
+  while (to_do && ok) {
+    const int h = cur.row / p.chunks, chunk = cur.row - h * p.chunks;
+    const bool from_begin = cur.step == 0;  // this share holds the row's first step
+    const int nh = min(p.heads, p.group - chunk * PA_HEADS);
+    float m[HALVES], l[HALVES];
+    {
       const T *q = static_cast<const T *>(p.a.q) + int64_t(cur.b) * p.a.q_batch_stride +
-                   int64_t(head0) * p.a.q_head_stride;
+                   int64_t(h * p.group + chunk * PA_HEADS) * p.a.q_head_stride;
       auto qv = [&](int g, int d) -> T {
         return (g < nh && d < D) ? q[int64_t(g) * p.a.q_head_stride + d] : T(0.f);
       };
@@ -365,9 +427,16 @@ __global__ void __launch_bounds__(PA_WARPS * 32)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int g = r0 + (j & 1) * 8, d = kk * 16 + 2 * kq + (j >> 1) * 8;
-            const __half2 v = (j & 1) && HALF_ROWS ? __half2(T(0.f), T(0.f))
-                                                   : __half2(qv(g, d), qv(g, d + 1));
-            qf[kk][j] = *reinterpret_cast<const uint32_t *>(&v);
+            if ((j & 1) && HALF_ROWS) {
+              qf[kk][j] = 0u;
+            } else if (p.q_pairs) {
+              qf[kk][j] = g < nh && d < D ? *reinterpret_cast<const uint32_t *>(
+                                                q + int64_t(g) * p.a.q_head_stride + d)
+                                          : 0u;
+            } else {
+              const __half2 v = __half2(qv(g, d), qv(g, d + 1));
+              qf[kk][j] = *reinterpret_cast<const uint32_t *>(&v);
+            }
           }
       } else if constexpr (!L::kQShared) {
 #pragma unroll
@@ -390,251 +459,310 @@ __global__ void __launch_bounds__(PA_WARPS * 32)
 #pragma unroll
       for (int x = 0; x < HALVES; ++x) m[x] = -INFINITY, l[x] = 0.f;
     }
-    cp_wait<STAGES - 2>();
-    __syncwarp();
-    load_next(stage == 0 ? STAGES - 1 : stage - 1);
-
-    const uint32_t ka = ring_a + uint32_t(stage * L::STAGE), va = ka + uint32_t(TOK * L::ROW);
-    // after load_next the ring holds STAGES entries: this step's is the oldest
-    const uint32_t live = uint32_t(live_ring >> (16 * (STAGES - 1))) & 0xffffu;
-    // ---- scores: s[t][.] are slots t * 8 + 2 * (lane % 4) + {0, 1} of head
-    // lane / 4 ([0], [1]) and lane / 4 + 8 ([2], [3])
-    constexpr int ST = TOK / 8;
-    float s[ST][4];
-#pragma unroll
-    for (int t = 0; t < ST; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
-    if constexpr (L::kHalf) {
-      const int tr = ((lane >> 4) << 3) + (lane & 7);
-#pragma unroll
-      for (int kk = 0; kk < DP / 16; ++kk) {
-        if (kk * 16 < D) {
-          uint32_t b[4];
-          ldsm4(ka + uint32_t(tr * L::ROW + (((2 * kk + ((lane >> 3) & 1)) ^ (tr & 7)) << 4)), b);
-          mma16(s[0], qf[kk], b[0], b[1]);
-          mma16(s[ST - 1], qf[kk], b[2], b[3]);
+    const uint32_t here = min(uint32_t(cur.s.steps - cur.step), to_do);
+#pragma unroll 1
+    for (uint32_t i = 0; i < here; ++i) {
+      const uint32_t live = uint32_t(live_ring >> (16 * (STAGES - 2))) & 0xffffu;
+      if (live) {
+        if (!mbar_wait(smem_u32(&bars[warp][stage]), (phase >> stage) & 1)) {
+          if (lane == 0) atomicOr(p.err, kErrLoadTimeout);
+          ok = false;
+          break;
         }
+        phase ^= 1u << stage;
       }
-    } else {
-      const int r = lane >> 2;
-      // the tensor core cuts its running sums instead of rounding them: the
-      // small products have a sum of their own, and the large ones two
-      float lo[4] = {0.f, 0.f, 0.f, 0.f}, odd[4] = {0.f, 0.f, 0.f, 0.f};
+      __syncwarp();  // the stage before this one is free
+      load_next(stage == 0 ? STAGES - 1 : stage - 1);
+      const uint32_t ka = ring_a + uint32_t(stage * L::STAGE), va = ka + uint32_t(TOK * L::ROW);
+      stage = stage + 1 == STAGES ? 0 : stage + 1;
+      constexpr int ST = TOK / 8;
+      if (!live && !p.scores) continue;
+      // ---- scores: s[t][.] are slots t * 8 + 2 * (lane % 4) + {0, 1} of head
+      // lane / 4 ([0], [1]) and lane / 4 + 8 ([2], [3])
+      float s[ST][4];
 #pragma unroll
-      for (int kk = 0; kk < DP / 8; ++kk) {
-        if (kk * 8 < D) {
-          uint32_t a[4], ah[4], al[4], bh[2], bl[2];
-          if constexpr (L::kQShared) {
-            const uint32_t qa = ring_a + uint32_t(STAGES * L::STAGE);
+      for (int t = 0; t < ST; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+      if (live != FULL) {
+        // what the pages hold in other slots must not reach 0 * v
+        for (int r = 0; r < TOK; ++r)
+          if (!((live >> r) & 1))
+            for (int ch = lane; ch < L::CPR; ch += 32)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(va + L::at(r, ch)), "r"(0)
+                           : "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+      }
+      if constexpr (L::kHalf) {
+        const int tr = ((lane >> 4) << 3) + (lane & 7);
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          if (kk * 16 < D) {
+            uint32_t b[4];
+            ldsm4(ka + L::at(tr, 2 * kk + ((lane >> 3) & 1)), b);
+            mma16(s[0], qf[kk], b[0], b[1]);
+            mma16(s[ST - 1], qf[kk], b[2], b[3]);
+          }
+        }
+      } else {
+        const int r = lane >> 2;
+        // the tensor core cuts its running sums instead of rounding them: the
+        // small products have a sum of their own, and the large ones two
+        float lo[4] = {0.f, 0.f, 0.f, 0.f}, odd[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < DP / 8; ++kk) {
+          if (kk * 8 < D) {
+            uint32_t a[4], ah[4], al[4], bh[2], bl[2];
+            if constexpr (L::kQShared) {
+              const uint32_t qa = ring_a + uint32_t(STAGES * L::STAGE);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const int g = r + (j & 1) * 8;
+                a[j] = (j & 1) && HALF_ROWS
+                           ? 0u
+                           : __float_as_uint(lds32(qa + uint32_t(g * L::ROW + (((2 * kk + (j >> 1)) ^ (g & 7)) << 4) +
+                                                                 (lane & 3) * 4)));
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) a[j] = qf[kk][j];
+            }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const int g = r + (j & 1) * 8;
-              a[j] = (j & 1) && HALF_ROWS
-                         ? 0u
-                         : __float_as_uint(lds32(qa + uint32_t(g * L::ROW + (((2 * kk + (j >> 1)) ^ (g & 7)) << 4) +
-                                                               (lane & 3) * 4)));
+              if ((j & 1) && HALF_ROWS) ah[j] = al[j] = 0u;
+              else split_tf32(__uint_as_float(a[j]), ah[j], al[j]);
             }
-          } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) a[j] = qf[kk][j];
+            for (int j = 0; j < 2; ++j)
+              split_tf32(lds32(ka + L::at(r, 2 * kk + j) + uint32_t(lane & 3) * 4), bh[j], bl[j]);
+            mma8(lo, al, bh[0], bh[1]);
+            mma8(lo, ah, bl[0], bl[1]);
+            mma8(kk & 1 ? odd : s[0], ah, bh[0], bh[1]);
           }
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if ((j & 1) && HALF_ROWS) ah[j] = al[j] = 0u;
-            else split_tf32(__uint_as_float(a[j]), ah[j], al[j]);
-          }
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-            split_tf32(lds32(ka + uint32_t(r * L::ROW + (((2 * kk + j) ^ (r & 7)) << 4) + (lane & 3) * 4)),
-                       bh[j], bl[j]);
-          mma8(lo, al, bh[0], bh[1]);
-          mma8(lo, ah, bl[0], bl[1]);
-          mma8(kk & 1 ? odd : s[0], ah, bh[0], bh[1]);
         }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[0][j] += odd[j] + lo[j];
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s[0][j] += odd[j] + lo[j];
-    }
-    // ---- running softmax
-    bool grew = false;
-    float mn[HALVES];
-#pragma unroll
-    for (int x = 0; x < HALVES; ++x) {
-      float mx = -INFINITY;
+      // ---- running softmax, base 2. The reference value m follows the
+      // maximum only when that has grown by more than 2^8: the probabilities
+      // stay below 256, and the result is rescaled a few times per row instead
+      // of at every new maximum of any head.
 #pragma unroll
       for (int t = 0; t < ST; ++t)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int bit = t * 8 + 2 * (lane & 3) + e;
-          float &v = s[t][2 * x + e];
-          v = (live >> bit) & 1 ? v * p.scale2 : -INFINITY;
-          mx = fmaxf(mx, v);
+        for (int e = 0; e < 2 * HALVES; ++e) s[t][e] *= p.scale2;
+      if (live != FULL) {
+#pragma unroll
+        for (int t = 0; t < ST; ++t)
+#pragma unroll
+          for (int e = 0; e < 2 * HALVES; ++e)
+            if (!((live >> (t * 8 + 2 * (lane & 3) + (e & 1))) & 1)) s[t][e] = -INFINITY;
+      }
+      if (p.scores) {
+        const int t0 = (cur.s.first + cur.step + int(i)) * TOK + 2 * (lane & 3);
+#pragma unroll
+        for (int x = 0; x < HALVES; ++x) {
+          const int g = (lane >> 2) + 8 * x;
+          if (g < nh) {
+            float *w = p.scores + (int64_t(cur.b) * p.a.q_heads + h * p.group + chunk * PA_HEADS + g) *
+                                      p.score_stride + t0;
+#pragma unroll
+            for (int t = 0; t < ST; ++t)
+              *reinterpret_cast<float2 *>(w + t * 8) = make_float2(s[t][2 * x], s[t][2 * x + 1]);
+          }
         }
-      mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 2));
-      mn[x] = fmaxf(m[x], mx);
-      grew |= mn[x] > m[x];
-    }
-    if (p.scores) {
-      const int t0 = (cur.s.first + cur.step) * TOK + 2 * (lane & 3);
+        if (!live) continue;
+      }
+      bool grew = false;
+      float mx[HALVES];
 #pragma unroll
       for (int x = 0; x < HALVES; ++x) {
-        const int g = chunk * PA_HEADS + (lane >> 2) + 8 * x;
-        if (g < p.group) {
-          float *w = p.scores + (int64_t(cur.b) * p.a.q_heads + h * p.group + g) * p.score_stride + t0;
+        mx[x] = fmaxf(s[0][2 * x], s[0][2 * x + 1]);
+        if constexpr (ST > 1) mx[x] = fmaxf(mx[x], fmaxf(s[1][2 * x], s[1][2 * x + 1]));
+        mx[x] = fmaxf(mx[x], __shfl_xor_sync(~0u, mx[x], 1));
+        mx[x] = fmaxf(mx[x], __shfl_xor_sync(~0u, mx[x], 2));
+        grew |= mx[x] > m[x] + 8.f;
+      }
+      if (__any_sync(~0u, grew)) {
 #pragma unroll
-          for (int t = 0; t < ST; ++t)
-            *reinterpret_cast<float2 *>(w + t * 8) = make_float2(s[t][2 * x], s[t][2 * x + 1]);
+        for (int x = 0; x < HALVES; ++x) {
+          const float mn = fmaxf(m[x], mx[x]);
+          const float f = mn > m[x] ? exp2_approx(m[x] - mn) : 1.f;
+          l[x] *= f;
+          m[x] = mn;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            o[n][2 * x] *= f;
+            o[n][2 * x + 1] *= f;
+          }
         }
       }
-    }
-    if (__any_sync(~0u, grew)) {
 #pragma unroll
       for (int x = 0; x < HALVES; ++x) {
-        const float f = mn[x] > m[x] ? exp2_approx(m[x] - mn[x]) : 1.f;
-        l[x] *= f;
-        m[x] = mn[x];
+        const float mu = m[x] == -INFINITY ? 0.f : m[x];
+#pragma unroll
+        for (int t = 0; t < ST; ++t)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float &v = s[t][2 * x + e];
+            v = exp2_approx(v - mu);
+            l[x] += v;
+          }
+      }
+      if (HALF_ROWS) {
+#pragma unroll
+        for (int t = 0; t < ST; ++t) s[t][2] = s[t][3] = 0.f;
+      }
+      // ---- result += p v
+      if constexpr (L::kHalf) {
+        // the probabilities go in as a sum of two fp16 numbers: one alone would
+        // add an error as large as the output's own rounding
+        uint32_t ph[4], pl[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int t = (j >> 1) * (ST - 1), x = j & 1;
+          if (x && HALF_ROWS) {
+            ph[j] = pl[j] = 0u;
+            continue;
+          }
+          ph[j] = pack2(s[t][2 * x], s[t][2 * x + 1]);
+          const float2 hf = __half22float2(*reinterpret_cast<const __half2 *>(&ph[j]));
+          pl[j] = pack2(s[t][2 * x] - hf.x, s[t][2 * x + 1] - hf.y);
+        }
+        const int tr = (((lane >> 3) & 1) << 3) + (lane & 7);
+#pragma unroll
+        for (int n = 0; n < NT / 2; ++n) {
+          if (n * 16 < D) {
+            uint32_t b[4];
+            ldsm4_t(va + L::at(tr, 2 * n + (lane >> 4)), b);
+            mma16(o[2 * n], ph, b[0], b[1]);
+            mma16(o[2 * n + 1], ph, b[2], b[3]);
+            mma16(o[2 * n], pl, b[0], b[1]);
+            mma16(o[2 * n + 1], pl, b[2], b[3]);
+          }
+        }
+      } else {
+        // the k index of the product runs over the slots in the order 0, 2, 4,
+        // 6, 1, 3, 5, 7, which is how the scores' accumulator holds them
+        uint32_t ah[4], al[4];
+        split_tf32(s[0][0], ah[0], al[0]);
+        split_tf32(s[0][2], ah[1], al[1]);
+        split_tf32(s[0][1], ah[2], al[2]);
+        split_tf32(s[0][3], ah[3], al[3]);
+        const int t0 = 2 * (lane & 3);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          o[n][2 * x] *= f;
-          o[n][2 * x + 1] *= f;
+          if (n * 8 < D) {
+            uint32_t bh[2], bl[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              split_tf32(lds32(va + L::at(t0 + j, 2 * n + (lane >> 4)) + uint32_t((lane >> 2) & 3) * 4),
+                         bh[j], bl[j]);
+            // a sum of its own per step, added in fp32 with rounding: cut sums
+            // drift over thousands of slots
+            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+            mma8(acc, al, bh[0], bh[1]);
+            mma8(acc, ah, bl[0], bl[1]);
+            mma8(acc, ah, bh[0], bh[1]);
+#pragma unroll
+            for (int j = 0; j < 2 * HALVES; ++j) o[n][j] += acc[j];
+          }
         }
       }
     }
+    if (!ok) break;
+    to_do -= here;
+    const bool whole = from_begin && cur.step + int(here) == cur.s.steps;
 #pragma unroll
     for (int x = 0; x < HALVES; ++x) {
-      const float mu = m[x] == -INFINITY ? 0.f : m[x];
+      float sum = l[x];
+      sum += __shfl_xor_sync(~0u, sum, 1);
+      sum += __shfl_xor_sync(~0u, sum, 2);
+      const int g = (lane >> 2) + 8 * x;
+      if (g >= nh) continue;
+      if (whole) {
+        const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+        T *out = static_cast<T *>(p.a.out) + int64_t(cur.b) * p.a.out_batch_stride +
+                 int64_t(h * p.group + chunk * PA_HEADS + g) * p.a.out_head_stride;
 #pragma unroll
-      for (int t = 0; t < ST; ++t)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float &v = s[t][2 * x + e];
-          v = exp2_approx(v - mu);
-          l[x] += v;
-        }
-    }
-    if (HALF_ROWS) {
-#pragma unroll
-      for (int t = 0; t < ST; ++t) s[t][2] = s[t][3] = 0.f;
-    }
-    // ---- result += p v
-    if constexpr (L::kHalf) {
-      // the probabilities go in as a sum of two fp16 numbers: one alone would
-      // add an error as large as the output's own rounding
-      uint32_t ph[4], pl[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int t = (j >> 1) * (ST - 1), x = j & 1;
-        ph[j] = pack2(s[t][2 * x], s[t][2 * x + 1]);
-        const float2 hf = __half22float2(*reinterpret_cast<const __half2 *>(&ph[j]));
-        pl[j] = pack2(s[t][2 * x] - hf.x, s[t][2 * x + 1] - hf.y);
-      }
-      const int tr = (((lane >> 3) & 1) << 3) + (lane & 7);
-#pragma unroll
-      for (int n = 0; n < NT / 2; ++n) {
-        if (n * 16 < D) {
-          uint32_t b[4];
-          ldsm4_t(va + uint32_t(tr * L::ROW + (((2 * n + (lane >> 4)) ^ (tr & 7)) << 4)), b);
-          mma16(o[2 * n], ph, b[0], b[1]);
-          mma16(o[2 * n + 1], ph, b[2], b[3]);
-          mma16(o[2 * n], pl, b[0], b[1]);
-          mma16(o[2 * n + 1], pl, b[2], b[3]);
-        }
-      }
-    } else {
-      // the k index of the product runs over the slots in the order 0, 2, 4,
-      // 6, 1, 3, 5, 7, which is how the scores' accumulator holds them
-      uint32_t ah[4], al[4];
-      split_tf32(s[0][0], ah[0], al[0]);
-      split_tf32(s[0][2], ah[1], al[1]);
-      split_tf32(s[0][1], ah[2], al[2]);
-      split_tf32(s[0][3], ah[3], al[3]);
-      const int t0 = 2 * (lane & 3);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        if (n * 8 < D) {
-          uint32_t bh[2], bl[2];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int t = t0 + j;
-            split_tf32(lds32(va + uint32_t(t * L::ROW + (((2 * n + (lane >> 4)) ^ (t & 7)) << 4) +
-                                           ((lane >> 2) & 3) * 4)),
-                       bh[j], bl[j]);
+          for (int e = 0; e < 2; ++e) {
+            const int d = n * 8 + 2 * (lane & 3) + e;
+            if (d < D) out[d] = T(o[n][2 * x + e] * inv);
           }
-          // a sum of its own per step, added in fp32 with rounding: cut sums
-          // drift over thousands of slots
-          float acc[4] = {0.f, 0.f, 0.f, 0.f};
-          mma8(acc, al, bh[0], bh[1]);
-          mma8(acc, ah, bl[0], bl[1]);
-          mma8(acc, ah, bh[0], bh[1]);
+        if (p.stats && (lane & 3) == 0)
+          p.stats[(int64_t(cur.b) * rows + cur.row) * PA_HEADS + g] = make_float2(m[x], sum);
+      } else {
+        const int64_t part = (int64_t(me) * 2 + (from_begin ? 1 : 0)) * p.heads + g;
+        float *po = p.part_o + part * D;
 #pragma unroll
-          for (int j = 0; j < 2 * HALVES; ++j) o[n][j] += acc[j];
-        }
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int d = n * 8 + 2 * (lane & 3) + e;
+            if (d < D) po[d] = o[n][2 * x + e];
+          }
+        if ((lane & 3) == 0) p.part_ml[part] = make_float2(m[x], sum);
       }
     }
-    stage = stage + 1 == STAGES ? 0 : stage + 1;
-    --to_do;
-    const bool row_end = cur.step + 1 == cur.s.steps;
-    if (row_end || to_do == 0) {
-      const int nh = min(p.heads, p.group - chunk * PA_HEADS);
-      const bool whole = from_begin && row_end;
-#pragma unroll
-      for (int x = 0; x < HALVES; ++x) {
-        float sum = l[x];
-        sum += __shfl_xor_sync(~0u, sum, 1);
-        sum += __shfl_xor_sync(~0u, sum, 2);
-        const int g = (lane >> 2) + 8 * x;
-        if (g >= nh) continue;
-        if (whole) {
-          const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-          T *out = static_cast<T *>(p.a.out) + int64_t(cur.b) * p.a.out_batch_stride +
-                   int64_t(h * p.group + chunk * PA_HEADS + g) * p.a.out_head_stride;
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int d = n * 8 + 2 * (lane & 3) + e;
-              if (d < D) out[d] = T(o[n][2 * x + e] * inv);
-            }
-          if (p.stats && (lane & 3) == 0)
-            p.stats[(int64_t(cur.b) * rows + cur.row) * PA_HEADS + g] = make_float2(m[x], sum);
-        } else {
-          const int64_t part = (int64_t(me) * 2 + (from_begin ? 1 : 0)) * p.heads + g;
-          float *po = p.part_o + part * D;
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int d = n * 8 + 2 * (lane & 3) + e;
-              if (d < D) po[d] = o[n][2 * x + e];
-            }
-          if ((lane & 3) == 0) p.part_ml[part] = make_float2(m[x], sum);
-        }
-      }
-      row_start = true;
-      from_begin = true;  // the next row begins within this share
-    }
-    next_step<TOK>(p, lens, rows, cur);
+    cur.next_row(p, lens, rows);
   }
-  cp_wait<0>();
+  if (!ok) {
+    // leave with nothing in flight: wait (bounded) for the other stages' copies
+    for (int s = 0; s < STAGES - 1; ++s) {
+      const uint32_t live = uint32_t(live_ring >> (16 * (STAGES - 2 - s))) & 0xffffu;
+      if (live) mbar_wait(smem_u32(&bars[warp][stage]), (phase >> stage) & 1);
+      stage = stage + 1 == STAGES ? 0 : stage + 1;
+    }
+  }
+}
+
+// Block reductions of the join: all threads get the result.
+__device__ __forceinline__ float join_max(float x, float *red) {
+#pragma unroll
+  for (int d = 16; d; d /= 2) x = fmaxf(x, __shfl_xor_sync(~0u, x, d));
+  __syncthreads();
+  if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = x;
+  __syncthreads();
+  x = red[0];
+#pragma unroll
+  for (int w = 1; w < PA_JOIN_THREADS / 32; ++w) x = fmaxf(x, red[w]);
+  return x;
+}
+__device__ __forceinline__ float join_sum(float x, float *red) {
+#pragma unroll
+  for (int d = 16; d; d /= 2) x += __shfl_xor_sync(~0u, x, d);
+  __syncthreads();
+  if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = x;
+  __syncthreads();
+  x = 0.f;
+#pragma unroll
+  for (int w = 0; w < PA_JOIN_THREADS / 32; ++w) x += red[w];
+  return x;
 }
 
 // Rows cut between warps: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i.
 // Block (b * kv_heads + h, y): y < group joins that query head; with
-// accumulation every y also adds the probabilities of its slots.
+// accumulation every y also adds the probabilities of its slots. The partial
+// results (up to one per warp of the grid for a lone long row) are spread over
+// the block's warps, whose lanes take neighbouring channels.
 template <typename T, int TOK>
 __global__ void __launch_bounds__(PA_JOIN_THREADS) join_kernel(const __grid_constant__ AttnArgs p) {
   extern __shared__ __align__(16) uint8_t jn_smem[];
+  constexpr int WARPS = PA_JOIN_THREADS / 32;
   __shared__ float head_m[PA_MAX_GROUP], head_inv[PA_MAX_GROUP];
+  __shared__ float red[WARPS], factor[PA_JOIN_THREADS];
+  __shared__ __align__(16) float sums[WARPS][256];
   const wgx_kv_cache &c = p.a.cache;
   uint32_t *prefix = reinterpret_cast<uint32_t *>(jn_smem);
   int *lens = reinterpret_cast<int *>(prefix + c.batch + 1);
   build_prefix<TOK>(p, prefix, lens);
   const int b = blockIdx.x / c.kv_heads, h = blockIdx.x % c.kv_heads, y = blockIdx.y;
-  const int rows = c.kv_heads * p.chunks, D = c.head_dim;
+  const int rows = c.kv_heads * p.chunks, D = c.head_dim, tid = threadIdx.x;
   const uint64_t total = uint64_t(prefix[c.batch]) * uint64_t(rows);
   const int workers = worker_count(p, total);
   const Span s = span_of<TOK>(p, lens[b]);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = tid / 32, lane = tid % 32;
 
   // where chunk's row lies in the line, and the warps that worked on it
   auto locate = [&](int chunk, uint64_t &r0, int &w0, int &w1) {
@@ -642,9 +770,10 @@ __global__ void __launch_bounds__(PA_JOIN_THREADS) join_kernel(const __grid_cons
     w0 = worker_of(r0, total, workers);
     w1 = worker_of(r0 + uint64_t(s.steps) - 1, total, workers);
   };
-  // row `g` of worker w's partial result of the row that starts at r0
-  auto part_of = [&](int w, uint64_t r0, int g) {
-    return (int64_t(w) * 2 + (share_begin(total, w, workers) > r0 ? 0 : 1)) * p.heads + g;
+  // row `g` of worker w's partial result of the row: only the first worker may
+  // have begun the row (then it is its last one)
+  auto part_of = [&](int w, bool begins, int g) {
+    return (int64_t(w) * 2 + (begins ? 1 : 0)) * p.heads + g;
   };
 
   if (y < p.group) {
@@ -652,28 +781,65 @@ __global__ void __launch_bounds__(PA_JOIN_THREADS) join_kernel(const __grid_cons
     T *out = static_cast<T *>(p.a.out) + int64_t(b) * p.a.out_batch_stride +
              int64_t(h * p.group + y) * p.a.out_head_stride;
     if (s.steps <= 0) {
-      for (int d = threadIdx.x; d < D; d += PA_JOIN_THREADS) out[d] = T(0.f);
+      for (int d = tid; d < D; d += PA_JOIN_THREADS) out[d] = T(0.f);
     } else {
       uint64_t r0;
       int w0, w1;
       locate(chunk, r0, w0, w1);
       if (w0 != w1) {
-        float M = -INFINITY;
-        for (int w = w0; w <= w1; ++w) M = fmaxf(M, p.part_ml[part_of(w, r0, g)].x);
+        float M = -INFINITY, sum = 0.f;
+        for (int w = w0 + tid; w <= w1; w += PA_JOIN_THREADS)
+          M = fmaxf(M, p.part_ml[part_of(w, w == w0, g)].x);
+        M = join_max(M, red);
         const float mu = M == -INFINITY ? 0.f : M;
-        float sum = 0.f;
-        for (int w = w0; w <= w1; ++w) {
-          const float2 ml = p.part_ml[part_of(w, r0, g)];
-          sum += ml.y * exp2_approx(ml.x - mu);
-        }
-        const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-        for (int d = threadIdx.x; d < D; d += PA_JOIN_THREADS) {
-          float acc = 0.f;
-          for (int w = w0; w <= w1; ++w) {
-            const int64_t part = part_of(w, r0, g);
-            acc += p.part_o[part * D + d] * exp2_approx(p.part_ml[part].x - mu);
+        float4 acc[2] = {};
+        const int quads = (D + 3) / 4;
+        for (int base = w0; base <= w1; base += PA_JOIN_THREADS) {
+          __syncthreads();
+          float f = 0.f;
+          if (base + tid <= w1) {
+            const float2 ml = p.part_ml[part_of(base + tid, base + tid == w0, g)];
+            f = exp2_approx(ml.x - mu);
+            sum += f * ml.y;
           }
-          out[d] = T(acc * inv);
+          factor[tid] = f;
+          __syncthreads();
+          const int n = min(PA_JOIN_THREADS, w1 - base + 1);
+#pragma unroll 4
+          for (int i = warp; i < n; i += WARPS) {
+            const float fi = factor[i];
+            const float *po = p.part_o + part_of(base + i, base + i == w0, g) * D;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const int q = lane + 32 * k;
+              if (q >= quads) break;
+              float4 v;
+              if (D % 4 == 0) {
+                v = *reinterpret_cast<const float4 *>(po + 4 * q);
+              } else {
+                v.x = po[4 * q];
+                v.y = 4 * q + 1 < D ? po[4 * q + 1] : 0.f;
+                v.z = 4 * q + 2 < D ? po[4 * q + 2] : 0.f;
+                v.w = 4 * q + 3 < D ? po[4 * q + 3] : 0.f;
+              }
+              acc[k].x += fi * v.x;
+              acc[k].y += fi * v.y;
+              acc[k].z += fi * v.z;
+              acc[k].w += fi * v.w;
+            }
+          }
+        }
+        sum = join_sum(sum, red);
+        const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          if (lane + 32 * k < quads) *reinterpret_cast<float4 *>(&sums[warp][4 * (lane + 32 * k)]) = acc[k];
+        __syncthreads();
+        for (int d = tid; d < D; d += PA_JOIN_THREADS) {
+          float v = 0.f;
+#pragma unroll
+          for (int w = 0; w < WARPS; ++w) v += sums[w][d];
+          out[d] = T(v * inv);
         }
       }
     }
@@ -682,7 +848,7 @@ __global__ void __launch_bounds__(PA_JOIN_THREADS) join_kernel(const __grid_cons
   const int t0 = y * PA_JOIN_SLOTS;
   const int t1 = min(t0 + PA_JOIN_SLOTS, int(min(int64_t(s.len), p.a.slots)));
   if (t0 >= t1) return;
-  for (int g = warp; g < p.group; g += PA_JOIN_THREADS / 32) {
+  for (int g = warp; g < p.group; g += WARPS) {
     const int chunk = g / PA_HEADS, gr = g % PA_HEADS;
     uint64_t r0;
     int w0, w1;
@@ -694,13 +860,13 @@ __global__ void __launch_bounds__(PA_JOIN_THREADS) join_kernel(const __grid_cons
       sum = ml.y;
     } else {
       M = -INFINITY;
-      for (int w = w0 + lane; w <= w1; w += 32) M = fmaxf(M, p.part_ml[part_of(w, r0, gr)].x);
+      for (int w = w0 + lane; w <= w1; w += 32) M = fmaxf(M, p.part_ml[part_of(w, w == w0, gr)].x);
 #pragma unroll
       for (int d = 16; d; d /= 2) M = fmaxf(M, __shfl_xor_sync(~0u, M, d));
       const float mu = M == -INFINITY ? 0.f : M;
       sum = 0.f;
       for (int w = w0 + lane; w <= w1; w += 32) {
-        const float2 ml = p.part_ml[part_of(w, r0, gr)];
+        const float2 ml = p.part_ml[part_of(w, w == w0, gr)];
         sum += ml.y * exp2_approx(ml.x - mu);
       }
 #pragma unroll
@@ -714,11 +880,13 @@ __global__ void __launch_bounds__(PA_JOIN_THREADS) join_kernel(const __grid_cons
   __syncthreads();
   const int64_t at = (int64_t(b) * c.kv_heads + h) * p.a.slots;
   const float *sc = p.scores + (int64_t(b) * p.a.q_heads + h * p.group) * p.score_stride;
-  for (int t = t0 + threadIdx.x; t < t1; t += PA_JOIN_THREADS) {
+  for (int t = t0 + tid; t < t1; t += PA_JOIN_THREADS) {
     float w = p.a.weights[at + t];
-    if (t >= s.lo)
+    if (t >= s.lo) {
+#pragma unroll 4
       for (int g = 0; g < p.group; ++g)
         w += exp2_approx(sc[int64_t(g) * p.score_stride + t] - head_m[g]) * head_inv[g];
+    }
     p.a.weights_out[at + t] = w;
   }
 }
@@ -732,7 +900,7 @@ template <typename T, int DP, bool HALF_ROWS>
 Config make_config() {
   Config c{};
   c.kernel = reinterpret_cast<const void *>(paged_attention_kernel<T, DP, HALF_ROWS>);
-  c.ring = PA_WARPS * Tile<T, DP>::RING;
+  c.ring = PA_WARPS * Tile<T, DP>::RING + 1024;  // + alignment
   c.tok = Tile<T, DP>::TOK;
   return c;
 }
@@ -800,8 +968,19 @@ Layout layout_of(const wgx_paged_attention_args &a) {
   p.chunks = (p.group + PA_HEADS - 1) / PA_HEADS;
   p.heads = std::min(p.group, PA_HEADS);
   p.vec = cache_rows_16b(c);
+  const int es = dtype_size(c.dtype);
+  p.q_pairs = c.dtype == WGX_FLOAT16 && c.head_dim % 2 == 0 && a.q_batch_stride % 2 == 0 &&
+              a.q_head_stride % 2 == 0 && (reinterpret_cast<uintptr_t>(a.q) & 3) == 0;
   p.scale2 = a.scale * 1.4426950408889634f;
   l.cfg = &config_for(c.dtype, c.head_dim, p.heads <= 8);
+  // TMA: a step's rows must lie in one page. Rows of whole 128-byte panels move
+  // as one box per operand, others panel by panel with zeros behind the row.
+  if (p.vec && c.page_size % l.cfg->tok == 0) {
+    const int panel = 128 / es, panels = c.head_dim % panel == 0 ? c.head_dim / panel : 1;
+    p.boxes = panels * panel == c.head_dim ? 1 : (c.head_dim + panel - 1) / panel;
+    p.tma = encode_rows_tmap(&p.k_map, c.k, c, c.k_page_stride, c.k_head_stride, c.k_slot_stride, panels, l.cfg->tok) &&
+            encode_rows_tmap(&p.v_map, c.v, c, c.v_page_stride, c.v_head_stride, c.v_slot_stride, panels, l.cfg->tok);
+  }
   p.min_steps = 64 / l.cfg->tok;
   const uint64_t steps = uint64_t((p.capacity + l.cfg->tok - 1) / l.cfg->tok) * c.batch *
                          uint64_t(c.kv_heads) * p.chunks;

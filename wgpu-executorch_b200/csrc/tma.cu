@@ -2,6 +2,7 @@
 // dependency on libcuda).
 #include <cudaTypedefs.h>
 
+#include "decode.h"
 #include "tma.h"
 
 namespace wgx {
@@ -31,6 +32,28 @@ void encode_nchw_tmap(CUtensorMap *map, const void *base, int B, int C, int HW, 
                                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) fail("conv2d: cuTensorMapEncodeTiled failed (" + std::to_string(int(r)) + ")");
+}
+
+bool encode_rows_tmap(CUtensorMap *map, const void *base, const wgx_kv_cache &c, int64_t page_stride,
+                      int64_t head_stride, int64_t slot_stride, int panels, int rows) {
+  const bool half = c.dtype == WGX_FLOAT16;
+  const int64_t es = half ? 2 : 4, panel = 128 / es;
+  const cuuint64_t dims[5] = {cuuint64_t(panels > 1 ? panel : c.head_dim), cuuint64_t(c.page_size),
+                              cuuint64_t(panels), cuuint64_t(c.kv_heads), cuuint64_t(c.pages)};
+  const int64_t bytes[4] = {slot_stride * es, 128, head_stride * es, page_stride * es};
+  cuuint64_t strides[4];
+  for (int i = 0; i < 4; ++i) {
+    // (an extent of one is never stepped over: any stride will do)
+    const int64_t s = dims[i + 1] == 1 ? 128 : bytes[i];
+    if (s <= 0 || s % 16 || s >= int64_t(1) << 40) return false;
+    strides[i] = cuuint64_t(s);
+  }
+  const cuuint32_t box[5] = {cuuint32_t(panel), cuuint32_t(rows), cuuint32_t(panels), 1, 1};
+  const cuuint32_t estride[5] = {1, 1, 1, 1, 1};
+  return encode_fn()(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 5,
+                     const_cast<void *>(base), dims, strides, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace wgx
