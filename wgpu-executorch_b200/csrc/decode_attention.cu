@@ -264,6 +264,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32)
   constexpr int TOK = L::TOK, STAGES = L::STAGES, NT = DP / 8;
   constexpr int HALVES = HALF_ROWS ? 1 : 2;
   constexpr uint32_t FULL = (1u << TOK) - 1;
+  constexpr int PANEL = 128 / int(sizeof(T)), PANELS = DP / PANEL;  // channels per 128 bytes
   extern __shared__ uint8_t pa_smem_raw[];
   __shared__ __align__(8) uint64_t bars[PA_WARPS][STAGES];
   uint8_t *pa_smem = reinterpret_cast<uint8_t *>(
@@ -301,27 +302,40 @@ __global__ void __launch_bounds__(PA_WARPS * 32)
   ld.start(p, prefix, lens, rows, begin);
   Walk<TOK> cur = ld;
   uint32_t to_load = uint32_t(end - begin), to_do = to_load;
-  int head = ld.row / p.chunks;
-  int page = -1, slot = 0;
-  uint32_t bits = 0;  // live slots of the next step
-  auto fetch = [&]() {
-    if (!to_load) return;
-    const int t0 = (ld.s.first + ld.step) * TOK, t = t0 + lane;
-    bool live = lane < TOK && t >= ld.s.lo && t < ld.s.len;
-    if (p.a.mask && live)
-      live = t < p.a.mask_width && p.a.mask[int64_t(ld.b) * p.a.mask_stride + t] != 0;
-    bits = __ballot_sync(~0u, live);
-    page = -1;
-    const int32_t *table = c.page_table + int64_t(ld.b) * c.table_stride;
+  int head = 0, left = 0;              // K/V head and steps left of the row being loaded
+  int t0 = 0, slot = 0, page = -1;     // next step: first slot, its place in its page
+  const int32_t *entry = nullptr;      // its page table entry (of its first slot)
+  uint32_t bits = 0;                   // its live slots
+  auto fetch_live = [&]() {
+    if (t0 >= ld.s.lo && t0 + TOK <= ld.s.len && !p.a.mask) {
+      bits = FULL;
+    } else {
+      const int t = t0 + lane;
+      bool live = lane < TOK && t >= ld.s.lo && t < ld.s.len;
+      if (p.a.mask && live)
+        live = t < p.a.mask_width && p.a.mask[int64_t(ld.b) * p.a.mask_stride + t] != 0;
+      bits = __ballot_sync(~0u, live);
+    }
+    if (!p.tma) {
+      page = -1;
+      if ((bits >> lane) & 1) {
+        const int t = t0 + lane, pi = int(uint32_t(t) / uint32_t(c.page_size));
+        slot = t - pi * c.page_size;
+        page = c.page_table[int64_t(ld.b) * c.table_stride + pi];
+      }
+    }
+  };
+  auto fetch_row = [&]() {
+    head = ld.row / p.chunks;
+    left = ld.s.steps - ld.step;
+    t0 = (ld.s.first + ld.step) * TOK;
     if (p.tma) {
       const int pi = int(uint32_t(t0) / uint32_t(c.page_size));
       slot = t0 - pi * c.page_size;
-      if (bits) page = table[pi];
-    } else if (live) {
-      const int pi = int(uint32_t(t) / uint32_t(c.page_size));
-      slot = t - pi * c.page_size;
-      page = table[pi];
+      entry = c.page_table + int64_t(ld.b) * c.table_stride + pi;
+      page = *entry;
     }
+    fetch_live();
   };
   uint64_t live_ring = 0;  // 16 bits of live slots per step in flight, oldest highest
   const T *kbase = static_cast<const T *>(c.k), *vbase = static_cast<const T *>(c.v);
@@ -344,7 +358,6 @@ __global__ void __launch_bounds__(PA_WARPS * 32)
     if (p.tma) {
       if (lane == 0) {
         const uint32_t ska = smem_u32(sk), sva = smem_u32(sv);
-        constexpr int PANEL = 128 / int(sizeof(T));
         // (a box counts in full, its part outside the tensor too)
         mbar_expect_tx(bar, uint32_t(2 * TOK * 128) * uint32_t((D + PANEL - 1) / PANEL));
         for (int j = 0; j < p.boxes; ++j) {
@@ -391,20 +404,52 @@ __global__ void __launch_bounds__(PA_WARPS * 32)
       return;
     }
     issue(stage);
-    --to_load;
-    if (++ld.step == ld.s.steps) {
+    if (!--to_load) return;
+    if (--left == 0) {
       ld.next_row(p, lens, rows);
-      head = ld.row / p.chunks;
+      fetch_row();
+    } else {
+      t0 += TOK;
+      if (p.tma) {
+        slot += TOK;
+        if (slot == c.page_size) {
+          slot = 0;
+          page = *++entry;
+        }
+      }
+      fetch_live();
     }
-    fetch();
   };
-  fetch();
+  fetch_row();
 #pragma unroll 1
   for (int s = 0; s < STAGES - 1; ++s) load_next(s);
 
   uint32_t qf[L::kQShared ? 1 : (L::kHalf ? DP / 16 : DP / 8)][4];
   float o[NT][4];
   const uint32_t ring_a = smem_u32(ring);
+  // Bytes of this lane's chunks within a panel of K and of V (L::at): the
+  // permutation is an exclusive or, so a panel's four operand columns cost four
+  // numbers, and panels are constant offsets.
+  uint32_t kx[4], vx[L::kHalf ? 4 : 8];
+  {
+    uint32_t k0, v0, v1 = 0;
+    if constexpr (L::kHalf) {
+      const int kt = ((lane >> 4) << 3) + (lane & 7), vt = (((lane >> 3) & 1) << 3) + (lane & 7);
+      k0 = uint32_t(kt * 128 + ((((lane >> 3) & 1) ^ (kt & 7)) << 4));
+      v0 = uint32_t(vt * 128 + (((lane >> 4) ^ (vt & 7)) << 4));
+    } else {
+      const int kt = lane >> 2, vt = 2 * (lane & 3), in = ((lane >> 2) & 3) * 4;
+      k0 = uint32_t(kt * 128 + (kt << 4) + (lane & 3) * 4);
+      v0 = uint32_t(vt * 128 + (((lane >> 4) ^ vt) << 4) + in);
+      v1 = uint32_t((vt + 1) * 128 + (((lane >> 4) ^ (vt + 1)) << 4) + in);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      kx[i] = k0 ^ uint32_t(32 * i);
+      vx[i] = v0 ^ uint32_t(32 * i);
+      if constexpr (!L::kHalf) vx[4 + i] = v1 ^ uint32_t(32 * i);
+    }
+  }
   int stage = 0;
   uint32_t phase = 0;  // bit s: parity of stage s's next wait
   bool ok = true;
@@ -493,54 +538,58 @@ __global__ void __launch_bounds__(PA_WARPS * 32)
         __syncwarp();
       }
       if constexpr (L::kHalf) {
-        const int tr = ((lane >> 4) << 3) + (lane & 7);
+        float s2[2][4] = {};  // odd columns: sums of their own, for the pipeline
 #pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk) {
-          if (kk * 16 < D) {
-            uint32_t b[4];
-            ldsm4(ka + L::at(tr, 2 * kk + ((lane >> 3) & 1)), b);
-            mma16(s[0], qf[kk], b[0], b[1]);
-            mma16(s[ST - 1], qf[kk], b[2], b[3]);
+        for (int pn = 0; pn < PANELS; ++pn) {
+          if (pn * PANEL < D) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t b[4];
+              ldsm4(ka + kx[i] + uint32_t(pn * TOK * 128), b);
+              mma16(i & 1 ? s2[0] : s[0], qf[pn * 4 + i], b[0], b[1]);
+              mma16(i & 1 ? s2[1] : s[ST - 1], qf[pn * 4 + i], b[2], b[3]);
+            }
           }
         }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 2 * HALVES; ++e) s[t % ST][e] += s2[t][e];
       } else {
         const int r = lane >> 2;
         // the tensor core cuts its running sums instead of rounding them: the
-        // small products have a sum of their own, and the large ones two
-        float lo[4] = {0.f, 0.f, 0.f, 0.f}, odd[4] = {0.f, 0.f, 0.f, 0.f};
+        // small products have sums of their own, and the large ones two
+        float lo[4] = {}, lo2[4] = {}, odd[4] = {};
 #pragma unroll
-        for (int kk = 0; kk < DP / 8; ++kk) {
-          if (kk * 8 < D) {
-            uint32_t a[4], ah[4], al[4], bh[2], bl[2];
-            if constexpr (L::kQShared) {
-              const uint32_t qa = ring_a + uint32_t(STAGES * L::STAGE);
+        for (int pn = 0; pn < PANELS; ++pn) {
+          if (pn * PANEL < D) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int kk = pn * 4 + i;
+              uint32_t ah[4], al[4], bh[2], bl[2];
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
-                const int g = r + (j & 1) * 8;
-                a[j] = (j & 1) && HALF_ROWS
-                           ? 0u
-                           : __float_as_uint(lds32(qa + uint32_t(g * L::ROW + (((2 * kk + (j >> 1)) ^ (g & 7)) << 4) +
-                                                                 (lane & 3) * 4)));
+                if ((j & 1) && HALF_ROWS) {
+                  ah[j] = al[j] = 0u;
+                } else if constexpr (L::kQShared) {
+                  const int g = r + (j & 1) * 8;
+                  const uint32_t qa = ring_a + uint32_t(STAGES * L::STAGE + g * L::ROW + ((g & 7) << 4) + (lane & 3) * 4);
+                  split_tf32(lds32(qa ^ uint32_t((2 * kk + (j >> 1)) << 4)), ah[j], al[j]);
+                } else {
+                  split_tf32(__uint_as_float(qf[kk][j]), ah[j], al[j]);
+                }
               }
-            } else {
 #pragma unroll
-              for (int j = 0; j < 4; ++j) a[j] = qf[kk][j];
+              for (int j = 0; j < 2; ++j)
+                split_tf32(lds32((ka + kx[i] + uint32_t(pn * TOK * 128)) ^ uint32_t(16 * j)), bh[j], bl[j]);
+              mma8(lo, al, bh[0], bh[1]);
+              mma8(lo2, ah, bl[0], bl[1]);
+              mma8(i & 1 ? odd : s[0], ah, bh[0], bh[1]);
             }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              if ((j & 1) && HALF_ROWS) ah[j] = al[j] = 0u;
-              else split_tf32(__uint_as_float(a[j]), ah[j], al[j]);
-            }
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-              split_tf32(lds32(ka + L::at(r, 2 * kk + j) + uint32_t(lane & 3) * 4), bh[j], bl[j]);
-            mma8(lo, al, bh[0], bh[1]);
-            mma8(lo, ah, bl[0], bl[1]);
-            mma8(kk & 1 ? odd : s[0], ah, bh[0], bh[1]);
           }
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[0][j] += odd[j] + lo[j];
+        for (int j = 0; j < 2 * HALVES; ++j) s[0][j] += odd[j] + (lo[j] + lo2[j]);
       }
       // ---- running softmax, base 2. The reference value m follows the
       // maximum only when that has grown by more than 2^8: the probabilities
@@ -628,16 +677,22 @@ __global__ void __launch_bounds__(PA_WARPS * 32)
           const float2 hf = __half22float2(*reinterpret_cast<const __half2 *>(&ph[j]));
           pl[j] = pack2(s[t][2 * x] - hf.x, s[t][2 * x + 1] - hf.y);
         }
-        const int tr = (((lane >> 3) & 1) << 3) + (lane & 7);
 #pragma unroll
-        for (int n = 0; n < NT / 2; ++n) {
-          if (n * 16 < D) {
-            uint32_t b[4];
-            ldsm4_t(va + L::at(tr, 2 * n + (lane >> 4)), b);
-            mma16(o[2 * n], ph, b[0], b[1]);
-            mma16(o[2 * n + 1], ph, b[2], b[3]);
-            mma16(o[2 * n], pl, b[0], b[1]);
-            mma16(o[2 * n + 1], pl, b[2], b[3]);
+        for (int pn = 0; pn < PANELS; ++pn) {
+          if (pn * PANEL < D) {
+            uint32_t b[4][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ldsm4_t(va + vx[i] + uint32_t(pn * TOK * 128), b[i]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              mma16(o[pn * 8 + 2 * i], ph, b[i][0], b[i][1]);
+              mma16(o[pn * 8 + 2 * i + 1], ph, b[i][2], b[i][3]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              mma16(o[pn * 8 + 2 * i], pl, b[i][0], b[i][1]);
+              mma16(o[pn * 8 + 2 * i + 1], pl, b[i][2], b[i][3]);
+            }
           }
         }
       } else {
@@ -648,23 +703,28 @@ __global__ void __launch_bounds__(PA_WARPS * 32)
         split_tf32(s[0][2], ah[1], al[1]);
         split_tf32(s[0][1], ah[2], al[2]);
         split_tf32(s[0][3], ah[3], al[3]);
-        const int t0 = 2 * (lane & 3);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          if (n * 8 < D) {
-            uint32_t bh[2], bl[2];
+        for (int pn = 0; pn < PANELS; ++pn) {
+          if (pn * PANEL < D) {
+            uint32_t bh[4][2], bl[4][2];
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-              split_tf32(lds32(va + L::at(t0 + j, 2 * n + (lane >> 4)) + uint32_t((lane >> 2) & 3) * 4),
-                         bh[j], bl[j]);
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+                split_tf32(lds32(va + vx[4 * j + i] + uint32_t(pn * TOK * 128)), bh[i][j], bl[i][j]);
             // a sum of its own per step, added in fp32 with rounding: cut sums
             // drift over thousands of slots
-            float acc[4] = {0.f, 0.f, 0.f, 0.f};
-            mma8(acc, al, bh[0], bh[1]);
-            mma8(acc, ah, bl[0], bl[1]);
-            mma8(acc, ah, bh[0], bh[1]);
+            float acc[4][4] = {};
 #pragma unroll
-            for (int j = 0; j < 2 * HALVES; ++j) o[n][j] += acc[j];
+            for (int i = 0; i < 4; ++i) mma8(acc[i], al, bh[i][0], bh[i][1]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mma8(acc[i], ah, bl[i][0], bl[i][1]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mma8(acc[i], ah, bh[i][0], bh[i][1]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int j = 0; j < 2 * HALVES; ++j) o[pn * 4 + i][j] += acc[i][j];
           }
         }
       }
