@@ -1,16 +1,18 @@
 // One step of beam search: selection over beams and vocabulary, and the
 // reordering of the paged cache's state.
 //
-// chunk_kernel reads the logits once: a block takes CHUNK tokens of one beam
-// into registers, forms their maximum and sum of exponentials and their
-// `beams` largest logits (a threshold from the lanes' maxima leaves a few
-// candidates, which are ranked by counting). select_kernel joins the chunks of
-// an item's beams: log sums, totals and the `beams` best proposals. With a
-// cache, reorder_kernel then writes the children's page tables and copies the
-// partly filled last pages, all layers in one launch.
+// scan_kernel reads the logits once: each beam's row is cut into a few
+// segments, a block streams its segment tile by tile, every thread with a
+// running maximum and sum of exponentials, and keeps the segment's `beams`
+// largest logits. Nearly all logits fail one comparison with a bound that is
+// shared by the block; the few others go to their warp's list. Warps do not
+// wait for one another until the segment's end. select_kernel joins the segments of an item's beams: log sums, totals
+// and the `beams` best proposals. With a cache, reorder_kernel then writes the
+// children's page tables and copies the partly filled last pages, all layers
+// in one launch.
 //
 // The order of proposals is (total descending, beam, logit descending, token).
-// A beam's proposals are its largest logits, so cutting each chunk's list at
+// A beam's proposals are its largest logits, so cutting each segment's list at
 // `beams` entries by (logit descending, token) loses none of the best.
 #include <algorithm>
 
@@ -22,18 +24,24 @@ namespace {
 
 constexpr int BM_THREADS = 256;
 constexpr int BM_WARPS = BM_THREADS / 32;
-constexpr int BM_ITEMS = 32;                     // logits per thread
-constexpr int BM_CHUNK = BM_THREADS * BM_ITEMS;  // tokens per block
-constexpr int BM_CAND = 1024;                    // candidates ranked by counting
+constexpr int BM_ITEMS = 16;                    // logits per thread and tile
+constexpr int BM_TILE = BM_THREADS * BM_ITEMS;  // tokens per tile
+constexpr int BM_KEEP = 128;                    // a longer list of a warp is cut to the best
+// a warp adds at most beams * BM_ITEMS logits a tile
+constexpr int BM_LIST = BM_KEEP + WGX_MAX_BEAMS * BM_ITEMS;
+constexpr int BM_CAND = 1024;                   // proposals ranked by counting
+constexpr int BM_BLOCKS_PER_SM = 4;             // of scan_kernel: 40 KB of shared memory each
 constexpr int BM_SEL_THREADS = 256;
 constexpr int BM_COPY_THREADS = 256;
+constexpr int BM_UNITS = 4;  // units of K and of V a thread has in flight
 
 struct BeamArgs {
   wgx_beam_search_args a;
   int64_t capacity;
-  int chunks;       // blocks per beam
-  float2 *chunk_ms; // [row][chunk] (max, sum of exp(x - max))
-  float *top_x;     // [row][chunk][beams] logits, best first
+  int tiles;        // of a row
+  int segments;     // blocks per row
+  float2 *seg_ms;   // [row][segment] (max, sum of exp(x - max))
+  float *top_x;     // [row][segment][beams] logits, best first
   int32_t *top_t;   // their tokens; -1: none
   int vec;          // cache rows move in 16-byte units
   uint32_t *err;
@@ -58,18 +66,23 @@ __device__ __forceinline__ float warp_sum(float x) {
   for (int d = 16; d; d /= 2) x += __shfl_xor_sync(~0u, x, d);
   return x;
 }
-// The lanes' values in descending order (bitonic).
-__device__ __forceinline__ float warp_sort(float x) {
+// The lanes' keys in descending order (bitonic).
+__device__ __forceinline__ uint64_t warp_sort(uint64_t x) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int k = 2; k <= 32; k *= 2)
 #pragma unroll
     for (int j = k / 2; j; j /= 2) {
-      const float y = __shfl_xor_sync(~0u, x, j);
-      const bool up = ((lane & k) == 0) == ((lane & j) == 0);
-      x = up ? fmaxf(x, y) : fminf(x, y);
+      const uint64_t y = __shfl_xor_sync(~0u, x, j);
+      const bool larger = ((lane & k) == 0) == ((lane & j) == 0);
+      if ((y > x) == larger) x = y;
     }
   return x;
+}
+
+// Key of a logit: larger logits first, equal ones by token. No two are equal.
+__device__ __forceinline__ uint64_t key_of(float x, int token) {
+  return uint64_t(ordered(x)) << 32 | uint32_t(~uint32_t(token));
 }
 
 // VEC: every beam's logits start on a 16-byte boundary; otherwise (odd
@@ -77,123 +90,160 @@ __device__ __forceinline__ float warp_sort(float x) {
 // for all beams, so that equal logits give equal sums: beams that tie stay
 // tied.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(BM_THREADS) chunk_kernel(const __grid_constant__ BeamArgs p) {
+__global__ void __launch_bounds__(BM_THREADS, BM_BLOCKS_PER_SM) scan_kernel(const __grid_constant__ BeamArgs p) {
   constexpr int EPV = VEC ? 16 / int(sizeof(T)) : 1, VECS = BM_ITEMS / EPV;
-  __shared__ float red_max[BM_WARPS], red_sum[BM_WARPS], own_k[BM_WARPS], low_k[BM_WARPS];
-  __shared__ uint64_t cand[BM_CAND];
-  __shared__ uint32_t n_cand;
-  __shared__ uint64_t best[BM_WARPS];
+  __shared__ float red_max[BM_WARPS], red_sum[BM_WARPS];
+  __shared__ uint64_t lists[BM_WARPS][BM_LIST];
+  __shared__ uint32_t n_lists[BM_WARPS];
+  __shared__ unsigned long long bound;  // keys below it are not among the best
   const wgx_beam_search_args &a = p.a;
-  const int row = blockIdx.y, chunk = blockIdx.x, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int row = blockIdx.y, seg = blockIdx.x, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   if (a.finished[row]) return;  // proposes eos: its logits are not needed
-  const int K = a.beams, t0 = chunk * BM_CHUNK, cnt = min(BM_CHUNK, a.vocab - t0);
+  const int K = a.beams;
   const T *x = static_cast<const T *>(a.logits) + int64_t(row / K) * a.logits_batch_stride +
-               int64_t(row % K) * a.logits_beam_stride + t0;
-  if (tid == 0) n_cand = 0;
-  // ---- the chunk into registers: item i of thread t is token
-  // (i / EPV * BM_THREADS + t) * EPV + i % EPV; -infinity behind the end and
-  // for NaN
-  float v[BM_ITEMS];
-#pragma unroll
-  for (int i = 0; i < VECS; ++i) {
-    const int o = (i * BM_THREADS + tid) * EPV;
-    if (VEC && o + EPV <= cnt) {
-      const uint4 u = __ldcs(reinterpret_cast<const uint4 *>(x + o));
-      const T *e = reinterpret_cast<const T *>(&u);
-#pragma unroll
-      for (int j = 0; j < EPV; ++j) v[i * EPV + j] = float(e[j]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < EPV; ++j) v[i * EPV + j] = o + j < cnt ? float(x[o + j]) : -INFINITY;
-    }
-  }
-  float mx = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < BM_ITEMS; ++i) {
-    if (v[i] != v[i]) v[i] = -INFINITY;
-    mx = fmaxf(mx, v[i]);
-  }
-  // ---- maximum and sum; thresholds: at least `K` logits of the chunk are not
-  // below (i) any one warp's K-th largest lane maximum, (ii) the smallest of
-  // the warps' ceil(K / BM_WARPS)-th largest
-  const float sorted = warp_sort(mx);
-  const float wm = __shfl_sync(~0u, sorted, 0);
-  const float wk = __shfl_sync(~0u, sorted, K - 1);
-  const float wl = __shfl_sync(~0u, sorted, (K + BM_WARPS - 1) / BM_WARPS - 1);
-  if (lane == 0) red_max[warp] = wm, own_k[warp] = wk, low_k[warp] = wl;
+               int64_t(row % K) * a.logits_beam_stride;
+  const int tile0 = int(int64_t(p.tiles) * seg / p.segments);
+  const int tile1 = int(int64_t(p.tiles) * (seg + 1) / p.segments);
+  uint64_t *list = lists[warp];
+  uint32_t *n_list = &n_lists[warp];
+  if (lane == 0) *n_list = 0;
+  if (tid == 0) bound = 0;
   __syncthreads();
-  float m = red_max[0], high = own_k[0], low = low_k[0];
+
+  // ---- item i of thread t of a tile is its token
+  // (i / EPV * BM_THREADS + t) * EPV + i % EPV; -infinity behind the end
+  union Raw {
+    uint4 u[VEC ? VECS : 1];
+    T e[BM_ITEMS];
+    __device__ Raw() {}
+  };
+  auto load = [&](int tile, Raw &r) {
+    const int t0 = tile * BM_TILE, cnt = a.vocab - t0;
 #pragma unroll
-  for (int w = 1; w < BM_WARPS; ++w) {
-    m = fmaxf(m, red_max[w]);
-    high = fmaxf(high, own_k[w]);
-    low = fminf(low, low_k[w]);
-  }
-  const float tau = fmaxf(high, low);
-  const float mu = m == -INFINITY ? 0.f : m;
-  float s = 0.f;
+    for (int i = 0; i < VECS; ++i) {
+      const int o = (i * BM_THREADS + tid) * EPV;
+      if (VEC && o + EPV <= cnt) {
+        r.u[VEC ? i : 0] = __ldcs(reinterpret_cast<const uint4 *>(x + t0 + o));
+      } else {
 #pragma unroll
-  for (int i = 0; i < BM_ITEMS; ++i) s += __expf(v[i] - mu);
-  s = warp_sum(s);
-  if (lane == 0) red_sum[warp] = s;
-  // ---- candidates: key = (logit, lower token first)
-  auto key_of = [&](float f, int o) { return uint64_t(ordered(f)) << 32 | uint32_t(~uint32_t(o)); };
-  auto offer = [&](float f, int o) {
-    if (f >= tau && o < cnt) {
-      const uint32_t at = atomicAdd(&n_cand, 1u);
-      if (at < BM_CAND) cand[at] = key_of(f, o);
+        for (int j = 0; j < EPV; ++j) r.e[i * EPV + j] = o + j < cnt ? x[t0 + o + j] : T(-INFINITY);
+      }
     }
   };
+  float m = -INFINITY, sum = 0.f;  // of this thread
+  Raw next;
+  load(tile0, next);
+  for (int tile = tile0; tile < tile1; ++tile) {
+    float v[BM_ITEMS];
+    float mx = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < BM_ITEMS; ++i)
-    offer(v[i], (i / EPV * BM_THREADS + tid) * EPV + i % EPV);
-  __syncthreads();
-  const int64_t out = int64_t(row) * p.chunks + chunk;
-  if (tid == 0) {
-    float sum = 0.f;
-    for (int w = 0; w < BM_WARPS; ++w) sum += red_sum[w];
-    p.chunk_ms[out] = make_float2(m, sum);
-  }
-  const int want = min(K, cnt), n = int(n_cand);
-  auto emit = [&](int at, uint64_t key) {
-    p.top_x[out * K + at] = unordered(uint32_t(key >> 32));
-    p.top_t[out * K + at] = t0 + int(~uint32_t(key));
-  };
-  if (tid >= want && tid < K) p.top_t[out * K + tid] = -1;
-  if (n <= BM_CAND) {
-    for (int i = tid; i < n; i += BM_THREADS) {
-      const uint64_t k = cand[i];
-      int rank = 0;
-      for (int j = 0; j < n; ++j) rank += cand[j] > k;
-      if (rank < want) emit(rank, k);
+    for (int i = 0; i < BM_ITEMS; ++i) {
+      v[i] = float(next.e[i]);
+      if (v[i] != v[i]) v[i] = -INFINITY;  // NaN
+      mx = fmaxf(mx, v[i]);
     }
-  } else {
-    // many equal logits at the threshold: one maximum after another
-    uint64_t below = ~uint64_t(0);
-    for (int r = 0; r < want; ++r) {
-      uint64_t k = 0;
+    if (tile + 1 < tile1) load(tile + 1, next);
+    // ---- running maximum and sum
+    if (mx > m) {
+      sum *= __expf(m - mx);
+      m = mx;
+    }
+    const float mu = m == -INFINITY ? 0.f : m;
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int i = 0; i < BM_ITEMS; i += 2) {
+      s0 += __expf(v[i] - mu);
+      s1 += __expf(v[i + 1] - mu);
+    }
+    sum += s0 + s1;
+    // ---- candidates. At least K keys of a warp are not below its K-th largest
+    // lane maximum; it is needed only where more than K lanes have candidates,
+    // and bounds what a warp adds to K lanes' logits.
+    uint64_t tau = *static_cast<volatile unsigned long long *>(&bound);
+    if (!__any_sync(~0u, ordered(mx) >= uint32_t(tau >> 32))) continue;
+    const int t0 = tile * BM_TILE, cnt = a.vocab - t0;
+    auto token = [&](int i) { return (i / EPV * BM_THREADS + tid) * EPV + i % EPV; };
+    uint64_t top = 0;
+#pragma unroll
+    for (int i = BM_ITEMS - 1; i >= 0; --i)  // ends with the first of equal ones
+      if (v[i] == mx && token(i) < cnt) top = key_of(mx, t0 + token(i));
+    // (lanes may have read different bounds)
+    bool has = top >= tau && top;
+    if (__popc(__ballot_sync(~0u, has)) > K) {
+      const uint64_t kth = __shfl_sync(~0u, warp_sort(has ? top : 0), K - 1);
+      if (kth > tau) tau = kth;
+      if (lane == 0) atomicMax(&bound, static_cast<unsigned long long>(kth));
+      has = top >= tau && top;
+    }
+    if (has) {
 #pragma unroll
       for (int i = 0; i < BM_ITEMS; ++i) {
-        const int o = (i / EPV * BM_THREADS + tid) * EPV + i % EPV;
-        const uint64_t q = key_of(v[i], o);
-        if (o < cnt && q < below && q > k) k = q;
+        if (ordered(v[i]) >= uint32_t(tau >> 32) && token(i) < cnt) {
+          const uint64_t k = key_of(v[i], t0 + token(i));
+          if (k >= tau) list[atomicAdd(n_list, 1u)] = k;
+        }
       }
-#pragma unroll
-      for (int d = 16; d; d /= 2) {
-        const uint64_t y = __shfl_xor_sync(~0u, k, d);
-        if (y > k) k = y;
+    }
+    __syncwarp();
+    const int n = int(*static_cast<volatile uint32_t *>(n_list));
+    if (n > BM_KEEP) {
+      // cut to the K best: lane r keeps the one with r larger ones
+      uint64_t mine = 0;
+      for (int i0 = 0; i0 < n; i0 += 32) {
+        const uint64_t k = i0 + lane < n ? list[i0 + lane] : 0;
+        int r = 0;
+        for (int j = 0; j < n; ++j) r += list[j] > k;
+        for (int w = 0; w < K; ++w) {
+          const uint32_t who = __ballot_sync(~0u, k && r == w);
+          if (who) {
+            const uint64_t y = __shfl_sync(~0u, k, __ffs(int(who)) - 1);
+            if (lane == w) mine = y;
+          }
+        }
       }
-      if (lane == 0) best[warp] = k;
-      __syncthreads();
-      k = best[0];
-#pragma unroll
-      for (int w = 1; w < BM_WARPS; ++w)
-        if (best[w] > k) k = best[w];
-      __syncthreads();
-      if (tid == 0) emit(r, k);
-      below = k;
+      __syncwarp();
+      if (lane < K) list[lane] = mine;
+      if (lane == 0) *n_list = uint32_t(K);
+      const uint64_t kth = __shfl_sync(~0u, mine, K - 1);
+      if (lane == 0) atomicMax(&bound, static_cast<unsigned long long>(kth));
+      __syncwarp();
     }
   }
+  // ---- join the threads
+  const float wm = warp_max(m);
+  const float wmu = wm == -INFINITY ? 0.f : wm;
+  const float ws = warp_sum(sum * __expf(m - wmu));
+  if (lane == 0) red_max[warp] = wm, red_sum[warp] = ws;
+  __syncthreads();
+  const int64_t out = int64_t(row) * p.segments + seg;
+  if (tid == 0) {
+    float M = red_max[0], all = 0.f;
+    for (int w = 1; w < BM_WARPS; ++w) M = fmaxf(M, red_max[w]);
+    const float mu = M == -INFINITY ? 0.f : M;
+    for (int w = 0; w < BM_WARPS; ++w) all += red_sum[w] * __expf(red_max[w] - mu);
+    p.seg_ms[out] = make_float2(M, all);
+  }
+  // ---- the lists' best, in order: a key not below the bound counts the larger
+  // ones of all lists
+  const uint64_t tau = bound;
+  int n = 0;
+  for (int w = 0; w < BM_WARPS; ++w) n += int(n_lists[w]);
+  for (int i = tid; i < n; i += BM_THREADS) {
+    int w = 0, e = i;
+    while (e >= int(n_lists[w])) e -= int(n_lists[w++]);
+    const uint64_t k = lists[w][e];
+    if (k < tau) continue;
+    int r = 0;
+    for (int o = 0; o < BM_WARPS; ++o) {
+      const int m = int(n_lists[o]);
+      for (int j = 0; j < m; ++j) r += lists[o][j] > k;
+    }
+    if (r < K) {
+      p.top_x[out * K + r] = unordered(uint32_t(k >> 32));
+      p.top_t[out * K + r] = int(~uint32_t(k));
+    }
+  }
+  if (tid >= n && tid < K) p.top_t[out * K + tid] = -1;
 }
 
 struct Proposal {
@@ -217,26 +267,28 @@ __global__ void __launch_bounds__(BM_SEL_THREADS) select_kernel(const __grid_con
   __shared__ Proposal best[BM_SEL_THREADS / 32];
   __shared__ uint32_t n_cand;
   const int b = blockIdx.x, W = a.beams, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  const int list = p.chunks * W, all = W * list;
+  const int list = p.segments * W, all = W * list;
   if (tid == 0) n_cand = 0;
   for (int w = warp; w < W; w += BM_SEL_THREADS / 32) {
     const int row = b * W + w;
     const bool done = a.finished[row] != 0;
+    const float score = a.scores[row];
     float m = -INFINITY, s = 0.f;
     if (!done) {
-      for (int c = lane; c < p.chunks; c += 32) m = fmaxf(m, p.chunk_ms[int64_t(row) * p.chunks + c].x);
+      const float2 *ms = p.seg_ms + int64_t(row) * p.segments;
+      const float2 mine = lane < p.segments ? ms[lane] : make_float2(-INFINITY, 0.f);
+      m = mine.x;
+      for (int c = lane + 32; c < p.segments; c += 32) m = fmaxf(m, ms[c].x);
       m = warp_max(m);
       const float mu = m == -INFINITY ? 0.f : m;
-      for (int c = lane; c < p.chunks; c += 32) {
-        const float2 ms = p.chunk_ms[int64_t(row) * p.chunks + c];
-        s += ms.y * __expf(ms.x - mu);
-      }
+      s = mine.y * __expf(mine.x - mu);
+      for (int c = lane + 32; c < p.segments; c += 32) s += ms[c].y * __expf(ms[c].x - mu);
       s = warp_sum(s);
     }
     if (lane == 0) {
       row_max[w] = m;
       row_log[w] = logf(s);
-      row_score[w] = a.scores[row];
+      row_score[w] = score;
       row_done[w] = done;
     }
   }
@@ -261,7 +313,7 @@ __global__ void __launch_bounds__(BM_SEL_THREADS) select_kernel(const __grid_con
     return true;
   };
   // ---- threshold: at least W proposals are not below the W-th entry of any
-  // one chunk's list
+  // one segment's list
   float tau = -INFINITY;
   for (int i = W - 1 + tid * W; i < all; i += BM_SEL_THREADS * W) {
     Proposal q;
@@ -328,18 +380,18 @@ __global__ void __launch_bounds__(BM_SEL_THREADS) select_kernel(const __grid_con
 }
 
 // Block (sequence, piece): the child's table and counters (piece 0), and a
-// share of its copied page: units of 16 bytes (or elements) of K and V over
-// (layer, head, slot).
-template <typename U, bool VEC>
+// share of its copied page: units U (16 bytes, or one element; STEP elements)
+// of K and V over (layer, head, slot), BM_UNITS at a time.
+template <typename U, int STEP>
 __global__ void __launch_bounds__(BM_COPY_THREADS) reorder_kernel(const __grid_constant__ BeamArgs p) {
   const wgx_beam_search_args &a = p.a;
   const wgx_kv_cache &c = a.cache;
   const int child = blockIdx.y, tid = threadIdx.x;
   const int from = child / a.beams * a.beams + a.parents[child];
+  const int spare = a.spare[child];
   const int len = slots_in_use(a.lengths, from, p.capacity, p.err);
   const int full = len / c.page_size, tail = len - full * c.page_size;
   const int32_t *src_table = c.page_table + int64_t(from) * c.table_stride;
-  const int spare = a.spare[child];
   if (blockIdx.x == 0) {
     int32_t *dst = a.page_table_out + int64_t(child) * c.table_width;
     for (int i = tid; i < c.table_width; i += BM_COPY_THREADS)
@@ -352,24 +404,39 @@ __global__ void __launch_bounds__(BM_COPY_THREADS) reorder_kernel(const __grid_c
     if (tid == 0 && blockIdx.x == 0) atomicOr(p.err, kErrCache);
     return;
   }
-  const int es = c.dtype == WGX_FLOAT16 ? 2 : 4;
-  const int units = VEC ? c.head_dim * es / 16 : c.head_dim;
-  const int64_t step = VEC ? 16 / es : 1;
-  const uint64_t all = uint64_t(c.layers) * c.kv_heads * tail * units;
-  U *k = static_cast<U *>(c.k), *v = static_cast<U *>(c.v);
-  for (uint64_t i = uint64_t(blockIdx.x) * BM_COPY_THREADS + tid; i < all;
-       i += uint64_t(gridDim.x) * BM_COPY_THREADS) {
-    const int u = int(i % units);
-    uint64_t r = i / units;
-    const int t = int(r % tail);
-    r /= tail;
-    const int h = int(r % c.kv_heads), layer = int(r / c.kv_heads);
-    const int64_t ko = int64_t(layer) * c.k_layer_stride + int64_t(h) * c.k_head_stride + int64_t(t) * c.k_slot_stride;
-    const int64_t vo = int64_t(layer) * c.v_layer_stride + int64_t(h) * c.v_head_stride + int64_t(t) * c.v_slot_stride;
-    const U x = k[(ko + int64_t(old) * c.k_page_stride) / step + u];
-    const U y = v[(vo + int64_t(old) * c.v_page_stride) / step + u];
-    k[(ko + int64_t(spare) * c.k_page_stride) / step + u] = x;
-    v[(vo + int64_t(spare) * c.v_page_stride) / step + u] = y;
+  const uint32_t units = uint32_t(c.head_dim / STEP), heads = uint32_t(c.kv_heads);
+  const uint32_t row = uint32_t(tail) * units;  // units of a (layer, head)
+  const U *ks = static_cast<const U *>(c.k) + int64_t(old) * c.k_page_stride / STEP;
+  const U *vs = static_cast<const U *>(c.v) + int64_t(old) * c.v_page_stride / STEP;
+  U *kd = static_cast<U *>(c.k) + int64_t(spare) * c.k_page_stride / STEP;
+  U *vd = static_cast<U *>(c.v) + int64_t(spare) * c.v_page_stride / STEP;
+  // a (layer, head) of the page per turn of this block's share
+  const uint32_t planes = uint32_t(c.layers) * heads;
+  const uint32_t per = row < BM_COPY_THREADS * BM_UNITS ? BM_COPY_THREADS * BM_UNITS / row : 1;  // planes a turn
+  for (uint32_t p0 = blockIdx.x * per; p0 < planes; p0 += gridDim.x * per) {
+    const uint32_t n = min(per, planes - p0) * row;
+    for (uint32_t i0 = tid; i0 < n; i0 += BM_COPY_THREADS * BM_UNITS) {
+      U x[BM_UNITS], y[BM_UNITS];
+      int64_t ko[BM_UNITS], vo[BM_UNITS];
+#pragma unroll
+      for (int e = 0; e < BM_UNITS; ++e) {
+        const uint32_t i = i0 + e * BM_COPY_THREADS;
+        ko[e] = -1;
+        if (i >= n) continue;
+        const uint32_t pl = i / row, in = i - pl * row, t = in / units, u = in - t * units;
+        const uint32_t layer = (p0 + pl) / heads, h = (p0 + pl) - layer * heads;
+        ko[e] = (int64_t(layer) * c.k_layer_stride + int64_t(h) * c.k_head_stride + int64_t(t) * c.k_slot_stride) / STEP + u;
+        vo[e] = (int64_t(layer) * c.v_layer_stride + int64_t(h) * c.v_head_stride + int64_t(t) * c.v_slot_stride) / STEP + u;
+        x[e] = ks[ko[e]];
+        y[e] = vs[vo[e]];
+      }
+#pragma unroll
+      for (int e = 0; e < BM_UNITS; ++e) {
+        if (ko[e] < 0) continue;
+        kd[ko[e]] = x[e];
+        vd[vo[e]] = y[e];
+      }
+    }
   }
 }
 
@@ -377,8 +444,11 @@ uint64_t align256(uint64_t x) { return (x + 255) / 256 * 256; }
 
 uint64_t layout(const wgx_beam_search_args &a, BeamArgs *p) {
   const uint64_t rows = uint64_t(a.batch) * a.beams;
-  const int chunks = (a.vocab + BM_CHUNK - 1) / BM_CHUNK;
-  const uint64_t lists = rows * chunks;
+  const int tiles = (a.vocab + BM_TILE - 1) / BM_TILE;
+  // segments: one wave of blocks over the GPU
+  const int segments = int(std::min<uint64_t>(
+      uint64_t(tiles), std::max<uint64_t>(1, uint64_t(device_sm_count()) * BM_BLOCKS_PER_SM / rows)));
+  const uint64_t lists = rows * segments;
   uint8_t *base = static_cast<uint8_t *>(a.scratch);
   uint64_t off = 0;
   auto take = [&](uint64_t bytes) {
@@ -388,8 +458,9 @@ uint64_t layout(const wgx_beam_search_args &a, BeamArgs *p) {
   };
   uint8_t *ms = take(lists * 8), *x = take(lists * a.beams * 4), *t = take(lists * a.beams * 4);
   if (p) {
-    p->chunks = chunks;
-    p->chunk_ms = reinterpret_cast<float2 *>(ms);
+    p->tiles = tiles;
+    p->segments = segments;
+    p->seg_ms = reinterpret_cast<float2 *>(ms);
     p->top_x = reinterpret_cast<float *>(x);
     p->top_t = reinterpret_cast<int32_t *>(t);
   }
@@ -411,17 +482,17 @@ void launch_beam_search_step(const wgx_beam_search_args &a, cudaStream_t stream)
   p.vec = c.k && cache_rows_16b(c);
   p.err = device_error_word(current_device());
   const unsigned rows = unsigned(a.batch) * unsigned(a.beams);
-  const dim3 grid(unsigned(p.chunks), rows);
-  const int th = timer_begin("chunk_kernel", stream);
+  const dim3 grid(unsigned(p.segments), rows);
+  const int th = timer_begin("scan_kernel", stream);
   const int ls = dtype_size(a.dtype);
   const bool vec = ((a.logits_batch_stride * ls) | (a.logits_beam_stride * ls) |
                     int64_t(reinterpret_cast<uintptr_t>(a.logits))) % 16 == 0;
   if (a.dtype == WGX_FLOAT16) {
-    if (vec) chunk_kernel<__half, true><<<grid, BM_THREADS, 0, stream>>>(p);
-    else chunk_kernel<__half, false><<<grid, BM_THREADS, 0, stream>>>(p);
+    if (vec) scan_kernel<__half, true><<<grid, BM_THREADS, 0, stream>>>(p);
+    else scan_kernel<__half, false><<<grid, BM_THREADS, 0, stream>>>(p);
   } else {
-    if (vec) chunk_kernel<float, true><<<grid, BM_THREADS, 0, stream>>>(p);
-    else chunk_kernel<float, false><<<grid, BM_THREADS, 0, stream>>>(p);
+    if (vec) scan_kernel<float, true><<<grid, BM_THREADS, 0, stream>>>(p);
+    else scan_kernel<float, false><<<grid, BM_THREADS, 0, stream>>>(p);
   }
   check_cuda(cudaGetLastError(), "beam_search_step launch");
   timer_end(th, stream);
@@ -431,16 +502,18 @@ void launch_beam_search_step(const wgx_beam_search_args &a, cudaStream_t stream)
   const int es = dtype_size(c.dtype);
   const uint64_t units = uint64_t(c.layers) * c.kv_heads * c.page_size *
                          uint64_t(p.vec ? c.head_dim * es / 16 : c.head_dim);
-  // about eight units per thread, at most sixteen blocks per SM
-  const uint64_t want = (units + BM_COPY_THREADS * 8 - 1) / (BM_COPY_THREADS * 8);
+  // one turn of BM_UNITS units a thread, at most sixteen blocks per SM
+  const uint64_t want = (units + BM_COPY_THREADS * BM_UNITS - 1) / (BM_COPY_THREADS * BM_UNITS);
   const uint64_t most = std::max<uint64_t>(1, uint64_t(device_sm_count()) * 16 / rows);
-  const dim3 cgrid(unsigned(std::max<uint64_t>(1, std::min(want, most))), rows);
-  if (p.vec)
-    reorder_kernel<uint4, true><<<cgrid, BM_COPY_THREADS, 0, stream>>>(p);
+  const dim3 cgrid(unsigned(std::min(want, most)), rows);
+  if (p.vec && es == 2)
+    reorder_kernel<uint4, 8><<<cgrid, BM_COPY_THREADS, 0, stream>>>(p);
+  else if (p.vec)
+    reorder_kernel<uint4, 4><<<cgrid, BM_COPY_THREADS, 0, stream>>>(p);
   else if (es == 2)
-    reorder_kernel<uint16_t, false><<<cgrid, BM_COPY_THREADS, 0, stream>>>(p);
+    reorder_kernel<uint16_t, 1><<<cgrid, BM_COPY_THREADS, 0, stream>>>(p);
   else
-    reorder_kernel<uint32_t, false><<<cgrid, BM_COPY_THREADS, 0, stream>>>(p);
+    reorder_kernel<uint32_t, 1><<<cgrid, BM_COPY_THREADS, 0, stream>>>(p);
   check_cuda(cudaGetLastError(), "beam_search_step reorder launch");
 }
 

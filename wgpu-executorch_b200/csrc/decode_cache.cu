@@ -16,68 +16,81 @@ namespace {
 
 // ------------------------------------------------------------------ append
 constexpr int AP_THREADS = 256;
+constexpr int AP_UNITS = 4;  // units of K and of V a thread has in flight
 
 struct AppendArgs {
   wgx_kv_append_args a;
   int64_t capacity;
-  int fused;  // one block per sequence: it writes the counters itself
+  int counters;  // this kernel writes the counters (their outputs are not its inputs, or one
+                 // block per sequence)
   uint32_t *err;
 };
 
-// The counters of sequence b, after its rows (lengths_out may be lengths).
-__device__ __forceinline__ void advance(const wgx_kv_append_args &a, int b, int len, bool fits) {
+// The counters of sequence b (lengths_out may be lengths).
+__device__ __forceinline__ void advance(const wgx_kv_append_args &a, int b, int len, int seen, bool fits) {
   a.lengths_out[b] = len + (fits ? a.tokens : 0);
-  if (a.seen_out) a.seen_out[b] = a.seen[b] + (fits ? a.tokens : 0);
+  if (a.seen_out) a.seen_out[b] = seen + (fits ? a.tokens : 0);
 }
 
-// VEC: rows in 16-byte units; otherwise element by element. Thread: one unit
-// of K and of V; consecutive threads take consecutive units of a row.
-template <typename U, bool VEC>
+// U: the unit that is moved (16 bytes of a row, or one element); STEP elements
+// each. Thread: AP_UNITS units of K and of V at a time, consecutive threads on
+// consecutive units. I: index type of a sequence's units.
+template <typename U, int STEP, typename I>
 __global__ void __launch_bounds__(AP_THREADS) append_kernel(const __grid_constant__ AppendArgs p) {
   const wgx_kv_append_args &a = p.a;
   const wgx_kv_cache &c = a.cache;
   const int b = blockIdx.y;
   const int len = slots_in_use(a.lengths, b, p.capacity, p.err);
+  const int seen = a.seen ? a.seen[b] : 0;
   const bool fits = int64_t(len) + a.tokens <= p.capacity;
   if (!fits && threadIdx.x == 0 && blockIdx.x == 0) atomicOr(p.err, kErrCache);
-  const int es = c.dtype == WGX_FLOAT16 ? 2 : 4;
-  const uint32_t units = uint32_t(VEC ? c.head_dim * es / 16 : c.head_dim);
-  const int64_t step = VEC ? 16 / es : 1;  // elements per unit
-  const uint64_t all = uint64_t(a.tokens) * c.kv_heads * units;
+  const uint32_t units = uint32_t(c.head_dim / STEP), heads = uint32_t(c.kv_heads);
+  const I all = I(a.tokens) * heads * units;
   if (fits) {
-    const U *k = static_cast<const U *>(a.k), *v = static_cast<const U *>(a.v);
+    const U *k = static_cast<const U *>(a.k) + int64_t(b) * a.k_batch_stride / STEP;
+    const U *v = static_cast<const U *>(a.v) + int64_t(b) * a.v_batch_stride / STEP;
     U *kc = static_cast<U *>(c.k), *vc = static_cast<U *>(c.v);
-    for (uint64_t i = uint64_t(blockIdx.x) * AP_THREADS + threadIdx.x; i < all;
-         i += uint64_t(gridDim.x) * AP_THREADS) {
-      const uint32_t row = uint32_t(i / units), u = uint32_t(i % units);
-      const int t = int(row / uint32_t(c.kv_heads)), h = int(row % uint32_t(c.kv_heads));
-      const int slot = len + t, pi = slot / c.page_size, in = slot - pi * c.page_size;
-      const int page = c.page_table[int64_t(b) * c.table_stride + pi];
-      if (page < 0 || page >= c.pages) {
-        atomicOr(p.err, kErrCache);
-        continue;
+    const int32_t *table = c.page_table + int64_t(b) * c.table_stride;
+    const I stride = I(gridDim.x) * AP_THREADS;
+    for (I i0 = I(blockIdx.x) * AP_THREADS + threadIdx.x; i0 < all; i0 += stride * AP_UNITS) {
+      U x[AP_UNITS], y[AP_UNITS];
+      int64_t kd[AP_UNITS], vd[AP_UNITS];
+#pragma unroll
+      for (int e = 0; e < AP_UNITS; ++e) {
+        const I i = i0 + I(e) * stride;
+        kd[e] = -1;
+        if (i >= all) continue;
+        const I row = i / units;
+        const uint32_t u = uint32_t(i - row * units);
+        const uint32_t t = uint32_t(row / heads), h = uint32_t(row - I(t) * heads);
+        const uint32_t at = uint32_t(len) + t, pi = at / uint32_t(c.page_size);
+        const int page = table[pi];
+        x[e] = __ldcs(k + (int64_t(t) * a.k_token_stride + int64_t(h) * a.k_head_stride) / STEP + u);
+        y[e] = __ldcs(v + (int64_t(t) * a.v_token_stride + int64_t(h) * a.v_head_stride) / STEP + u);
+        if (page < 0 || page >= c.pages) {
+          atomicOr(p.err, kErrCache);
+          continue;
+        }
+        const int64_t in = int64_t(at - pi * uint32_t(c.page_size));
+        kd[e] = (int64_t(page) * c.k_page_stride + int64_t(h) * c.k_head_stride + in * c.k_slot_stride) / STEP + u;
+        vd[e] = (int64_t(page) * c.v_page_stride + int64_t(h) * c.v_head_stride + in * c.v_slot_stride) / STEP + u;
+        if (u == 0 && at < a.slots) {
+          const int64_t w = (int64_t(b) * c.kv_heads + h) * a.slots + at;
+          if (a.weights) a.weights[w] = 0.f;
+          if (a.positions) a.positions[w] = seen + int(t);
+        }
       }
-      const int64_t ks = int64_t(b) * a.k_batch_stride + int64_t(t) * a.k_token_stride +
-                         int64_t(h) * a.k_head_stride;
-      const int64_t vs = int64_t(b) * a.v_batch_stride + int64_t(t) * a.v_token_stride +
-                         int64_t(h) * a.v_head_stride;
-      const int64_t kd = int64_t(page) * c.k_page_stride + int64_t(h) * c.k_head_stride +
-                         int64_t(in) * c.k_slot_stride;
-      const int64_t vd = int64_t(page) * c.v_page_stride + int64_t(h) * c.v_head_stride +
-                         int64_t(in) * c.v_slot_stride;
-      const U x = k[ks / step + u], y = v[vs / step + u];
-      kc[kd / step + u] = x;
-      vc[vd / step + u] = y;
-      if (u == 0 && slot < a.slots) {
-        const int64_t at = (int64_t(b) * c.kv_heads + h) * a.slots + slot;
-        if (a.weights) a.weights[at] = 0.f;
-        if (a.positions) a.positions[at] = a.seen[b] + t;
+#pragma unroll
+      for (int e = 0; e < AP_UNITS; ++e) {
+        if (kd[e] < 0) continue;
+        kc[kd[e]] = x[e];
+        vc[vd[e]] = y[e];
       }
     }
   }
-  if (p.fused) {
+  if (p.counters && blockIdx.x == 0) {
     __syncthreads();
-    if (threadIdx.x == 0) advance(a, b, len, fits);
+    if (threadIdx.x == 0) advance(a, b, len, seen, fits);
   }
 }
 
@@ -85,18 +98,25 @@ __global__ void advance_kernel(const __grid_constant__ AppendArgs p) {
   const int b = blockIdx.x * blockDim.x + threadIdx.x;
   if (b >= p.a.cache.batch) return;
   const int len = slots_in_use(p.a.lengths, b, p.capacity, p.err);
-  advance(p.a, b, len, int64_t(len) + p.a.tokens <= p.capacity);
+  advance(p.a, b, len, p.a.seen ? p.a.seen[b] : 0, int64_t(len) + p.a.tokens <= p.capacity);
 }
 
 // ------------------------------------------------------------------- evict
-// A cluster of CTAs per (sequence, K/V head). The budget-th largest key is
-// found by radix selection (8 bits a pass, histograms summed over the cluster
-// through distributed shared memory) on keys held in shared memory: weights
-// and positions are read once. Survivors behind the budget then move into the
-// holes before it, both listed in slot order.
+// A cluster of CTAs per (sequence, K/V head). The order of slots is that of the
+// numbers (weight key << 32 | complement of the slot), all distinct; the
+// budget-th largest is found by radix selection, 11 bits a pass (histograms in
+// shared memory, summed over the cluster through distributed shared memory),
+// until the class it lies in is wholly taken or small enough (256) to be
+// ranked by counting: one or two passes unless weights tie. Keys are held in
+// shared memory, weights and positions are read once. Survivors behind the
+// budget then move into the holes before it, both listed in slot order.
 constexpr int EV_THREADS = 512;
 constexpr int EV_MAX_CLUSTER = 8;
-constexpr int EV_MAX_CHUNK = 36864;  // slots per CTA: 6 bytes of shared memory each
+constexpr int EV_MAX_CHUNK = 32768;  // slots per CTA: 6 bytes of shared memory each
+constexpr int EV_BINS = 2048, EV_BITS = 11;
+constexpr int EV_CLASS = 256;        // slots of a class that are ranked by counting
+static_assert(EV_CLASS <= EV_THREADS, "one thread ranks one member");
+constexpr int EV_FLIGHT = 4;         // rows a warp has in flight
 constexpr uint32_t kProtected = 0xffffffffu;
 
 struct EvictArgs {
@@ -139,14 +159,18 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t *warp_sum, u
   return before + s - x;
 }
 
-__global__ void __launch_bounds__(EV_THREADS) evict_kernel(const __grid_constant__ EvictArgs p) {
+__global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const __grid_constant__ EvictArgs p) {
   extern __shared__ __align__(16) uint8_t ev_smem[];
   uint32_t *keys = reinterpret_cast<uint32_t *>(ev_smem);
   uint16_t *list = reinterpret_cast<uint16_t *>(ev_smem + size_t(p.chunk) * 4);
-  __shared__ uint32_t hist[4][256];
+  // three histograms in turn: while one is read by other CTAs the next is
+  // filled and the one after it cleared
+  __shared__ __align__(16) uint32_t hist[3][EV_BINS];
+  __shared__ uint64_t members[EV_CLASS], all_members[EV_CLASS];
+  __shared__ uint64_t last_kept;     // the budget-th largest number
   __shared__ uint32_t warp_sum[EV_THREADS / 32];
-  __shared__ uint32_t counts[3];     // ties, holes, movers of this CTA
-  __shared__ uint32_t pick[2];       // digit, keys above it
+  __shared__ uint32_t counts[3];     // class members, holes, movers of this CTA
+  __shared__ uint32_t pick[3];       // bin, numbers above it, numbers in it
   __shared__ uint32_t hole_end[EV_MAX_CLUSTER], mover_end[EV_MAX_CLUSTER];
   cg::cluster_group cluster = cg::this_cluster();
   const int S = int(cluster.num_blocks()), rank = int(cluster.block_rank());
@@ -155,6 +179,7 @@ __global__ void __launch_bounds__(EV_THREADS) evict_kernel(const __grid_constant
   const int tid = threadIdx.x, row = int(blockIdx.x) / S;
   const int b = row / c.kv_heads, h = row % c.kv_heads, C = a.budget;
   const int len = slots_in_use(a.lengths, b, p.capacity, p.err);
+  const int recent_from = a.seen[b] - a.recent;
   const int n = int(min(int64_t(len), a.slots));
   const int64_t at = int64_t(row) * a.slots;
   if (p.counters && h == 0 && rank == 0 && tid == 0) a.lengths_out[b] = min(len, C);
@@ -166,72 +191,106 @@ __global__ void __launch_bounds__(EV_THREADS) evict_kernel(const __grid_constant
     return;
   }
   const int per = (n + S - 1) / S, s0 = min(rank * per, n), s1 = min(s0 + per, n), cnt = s1 - s0;
-  const int recent_from = a.seen[b] - a.recent;
 
-  for (int i = tid; i < 4 * 256; i += EV_THREADS) (&hist[0][0])[i] = 0;
+  for (int i = tid; i < 3 * EV_BINS; i += EV_THREADS) (&hist[0][0])[i] = 0;
+  if (tid == 0) counts[0] = 0;
+  const bool w_apart = a.weights_out != a.weights, p_apart = a.positions_out != a.positions;
+#pragma unroll 4
   for (int i = tid; i < cnt; i += EV_THREADS) {
     const float w = a.weights[at + s0 + i];
     const int pos = a.positions[at + s0 + i];
     keys[i] = evict_key(w, pos, recent_from, a.sinks);
     if (s0 + i < C) {  // holes among these are overwritten below
-      if (a.weights_out != a.weights) a.weights_out[at + s0 + i] = w;
-      if (a.positions_out != a.positions) a.positions_out[at + s0 + i] = pos;
+      if (w_apart) a.weights_out[at + s0 + i] = w;
+      if (p_apart) a.positions_out[at + s0 + i] = pos;
     }
   }
   __syncthreads();
+  auto number = [&](int i) { return uint64_t(keys[i]) << 32 | uint32_t(~uint32_t(s0 + i)); };
 
-  // ---- the C-th largest key: `found` digit by digit, `left` of the keys that
-  // equal it so far still to be taken
-  uint32_t found = 0, left = uint32_t(C);
-  for (int pass = 0; pass < 4; ++pass) {
-    const int shift = 24 - 8 * pass;
-    const int rounds = (cnt + EV_THREADS - 1) / EV_THREADS;
-    for (int r = 0; r < rounds; ++r) {
-      const int i = r * EV_THREADS + tid;
-      const bool in = i < cnt && (pass == 0 || (keys[i] >> (shift + 8)) == (found >> (shift + 8)));
-      // equal digits of a warp are counted together: weights share exponents
-      const uint32_t digit = in ? (keys[i] >> shift) & 255u : 256u;
-      const uint32_t peers = __match_any_sync(~0u, digit);
-      if (in && (tid & 31) == __ffs(int(peers)) - 1)
-        atomicAdd(&hist[pass][digit], uint32_t(__popc(peers)));
+  // ---- the C-th largest number: its leading bits are those of `found`, and
+  // `left` of the numbers with these bits are still to be taken
+  uint64_t found = 0;
+  uint32_t left = uint32_t(C);
+  int shift = 64;  // bits not yet looked at
+  for (int pass = 0;; ++pass) {
+    const int bits = min(EV_BITS, shift);
+    const int low = shift - bits;
+    uint32_t *mine = hist[pass % 3];
+    for (int i = tid; i < cnt; i += EV_THREADS) {
+      const uint64_t x = number(i);
+      if (shift == 64 || (x >> shift) == (found >> shift))
+        atomicAdd(&mine[uint32_t(x >> low) & (EV_BINS - 1)], 1u);
+    }
+    if (pass) {  // (the first three are clear)
+      uint32_t *next = hist[(pass + 1) % 3];
+      for (int i = tid; i < EV_BINS; i += EV_THREADS) next[i] = 0;
     }
     cluster.sync();
-    uint32_t mine = 0;
-    if (tid < 256)  // thread t: digit 255 - t, so that larger digits come first
-      for (int r = 0; r < S; ++r) mine += cluster.map_shared_rank(&hist[pass][0], r)[255 - tid];
+    // thread t: the four bins from 4 * (511 - t), largest first
+    uint4 q = make_uint4(0, 0, 0, 0);
+    const int bin = EV_BINS - 4 * (tid + 1);
+    for (int r = 0; r < S; ++r) {
+      const uint4 y = *reinterpret_cast<const uint4 *>(cluster.map_shared_rank(mine, r) + bin);
+      q.x += y.x;
+      q.y += y.y;
+      q.z += y.z;
+      q.w += y.w;
+    }
     uint32_t total;
-    const uint32_t above = block_scan(mine, warp_sum, &total);
-    if (tid < 256 && above < left && above + mine >= left) {
-      pick[0] = uint32_t(255 - tid);
-      pick[1] = above;
+    uint32_t above = block_scan(q.x + q.y + q.z + q.w, warp_sum, &total);
+    const uint32_t v[4] = {q.w, q.z, q.y, q.x};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (above < left && above + v[j] >= left) {
+        pick[0] = uint32_t(bin + 3 - j);
+        pick[1] = above;
+        pick[2] = v[j];
+      }
+      above += v[j];
     }
     __syncthreads();
-    found |= pick[0] << shift;
+    shift = low;
+    found |= uint64_t(pick[0]) << shift;
     left -= pick[1];
-    __syncthreads();
+    const uint32_t members_all = pick[2];
+    if (members_all == left) break;  // wholly taken (always so with no bits left)
+    if (members_all <= EV_CLASS) {
+      for (int i = tid; i < cnt; i += EV_THREADS) {
+        const uint64_t x = number(i);
+        if ((x >> shift) == (found >> shift)) members[atomicAdd(&counts[0], 1u)] = x;
+      }
+      cluster.sync();
+      // every CTA ranks them all: thread i counts the members larger than i
+      uint32_t base = 0;
+      for (int r = 0; r < S; ++r) {
+        const uint32_t m = *cluster.map_shared_rank(&counts[0], r);
+        if (uint32_t(tid) < m) all_members[base + tid] = cluster.map_shared_rank(members, r)[tid];
+        base += m;
+      }
+      __syncthreads();
+      if (uint32_t(tid) < members_all) {
+        const uint64_t x = all_members[tid];
+        uint32_t larger = 0;
+#pragma unroll 8
+        for (uint32_t j = 0; j < members_all; ++j) larger += all_members[j] > x;
+        if (larger == left - 1) last_kept = x;
+      }
+      __syncthreads();
+      found = last_kept;
+      break;
+    }
+    __syncthreads();  // pick is written again
   }
 
-  // ---- survivors: keys above `found`, and the first `left` (by slot) of
-  // those equal to it. A thread takes `q` consecutive slots (odd: no bank
+  // ---- holes and movers. A thread takes `q` consecutive slots (odd: no bank
   // conflicts between threads).
   const int q = ((cnt + EV_THREADS - 1) / EV_THREADS) | 1;
   const int i0 = min(tid * q, cnt), i1 = min(i0 + q, cnt);
-  uint32_t ties = 0, total;
-  for (int i = i0; i < i1; ++i) ties += keys[i] == found;
-  uint32_t tie_rank = block_scan(ties, warp_sum, &total);
-  if (tid == 0) counts[0] = total;
-  cluster.sync();
-  for (int r = 0; r < rank; ++r) tie_rank += cluster.map_shared_rank(&counts[0], r)[0];
   const int split = max(0, min(C - s0, cnt));  // local slots before the budget
-  uint32_t hm = 0;  // holes (low half) and movers (high half); chunks are below 2^16 slots
-  {
-    uint32_t tr = tie_rank;
-    for (int i = i0; i < i1; ++i) {
-      const uint32_t k = keys[i];
-      const bool keep = k > found || (k == found && tr++ < left);
-      hm += keep == (i < split) ? 0u : (i < split ? 1u : 0x10000u);
-    }
-  }
+  uint32_t hm = 0, total;  // holes (low half) and movers (high half); chunks are below 2^16 slots
+  for (int i = i0; i < i1; ++i)
+    if ((number(i) >= found) != (i < split)) hm += i < split ? 1u : 0x10000u;
   uint32_t at_list = block_scan(hm, warp_sum, &total);
   if (tid == 0) {
     counts[1] = total & 0xffffu;
@@ -239,11 +298,10 @@ __global__ void __launch_bounds__(EV_THREADS) evict_kernel(const __grid_constant
   }
   // holes from the front of the list, movers behind the place of slot C
   for (int i = i0; i < i1; ++i) {
-    const uint32_t k = keys[i];
-    const bool keep = k > found || (k == found && tie_rank++ < left);
+    if ((number(i) >= found) == (i < split)) continue;
     if (i < split) {
-      if (!keep) list[at_list++ & 0xffffu] = uint16_t(i);
-    } else if (keep) {
+      list[at_list++ & 0xffffu] = uint16_t(i);
+    } else {
       list[split + (at_list >> 16)] = uint16_t(i);
       at_list += 0x10000u;
     }
@@ -296,28 +354,45 @@ __global__ void __launch_bounds__(EV_THREADS) evict_kernel(const __grid_constant
     }
     uint8_t *kb = static_cast<uint8_t *>(c.k), *vb = static_cast<uint8_t *>(c.v);
     const int pairs = min(32, moves - j0);
-    for (int x = 0; x < pairs; ++x) {
-      const int64_t xkd = __shfl_sync(~0u, kd, x), xks = __shfl_sync(~0u, ks, x);
-      const int64_t xvd = __shfl_sync(~0u, vd, x), xvs = __shfl_sync(~0u, vs, x);
-      if (xkd < 0) continue;
-      if (p.vec) {
-        const int units = c.head_dim * es / 16;
-        for (int i = lane; i < 2 * units; i += 32) {
-          const bool isv = i >= units;
+    if (p.vec) {
+      // a unit of EV_FLIGHT rows at a time: loads first, then stores
+      const int units = c.head_dim * es / 16;
+      for (int x0 = 0; x0 < pairs; x0 += EV_FLIGHT) {
+        for (int i0 = 0; i0 < 2 * units; i0 += 32) {
+          const int i = i0 + lane;
+          const bool isv = i >= units, on = i < 2 * units;
           const int o = (isv ? i - units : i) * 16;
-          const uint8_t *src = isv ? vb + xvs + o : kb + xks + o;
-          *reinterpret_cast<uint4 *>(isv ? vb + xvd + o : kb + xkd + o) =
-              *reinterpret_cast<const uint4 *>(src);
+          uint8_t *base = (isv ? vb : kb) + o;
+          uint4 v[EV_FLIGHT];
+          uint8_t *to[EV_FLIGHT];
+#pragma unroll
+          for (int e = 0; e < EV_FLIGHT; ++e) {
+            const int64_t xkd = __shfl_sync(~0u, kd, x0 + e), xks = __shfl_sync(~0u, ks, x0 + e);
+            const int64_t xvd = __shfl_sync(~0u, vd, x0 + e), xvs = __shfl_sync(~0u, vs, x0 + e);
+            to[e] = nullptr;
+            if (on && xkd >= 0) {  // (lanes without a pair hold -1)
+              v[e] = *reinterpret_cast<const uint4 *>(base + (isv ? xvs : xks));
+              to[e] = base + (isv ? xvd : xkd);
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < EV_FLIGHT; ++e)
+            if (to[e]) *reinterpret_cast<uint4 *>(to[e]) = v[e];
         }
-      } else if (es == 2) {
+      }
+    } else {
+      for (int x = 0; x < pairs; ++x) {
+        const int64_t xkd = __shfl_sync(~0u, kd, x), xks = __shfl_sync(~0u, ks, x);
+        const int64_t xvd = __shfl_sync(~0u, vd, x), xvs = __shfl_sync(~0u, vs, x);
+        if (xkd < 0) continue;
         for (int i = lane; i < c.head_dim; i += 32) {
-          reinterpret_cast<uint16_t *>(kb + xkd)[i] = reinterpret_cast<const uint16_t *>(kb + xks)[i];
-          reinterpret_cast<uint16_t *>(vb + xvd)[i] = reinterpret_cast<const uint16_t *>(vb + xvs)[i];
-        }
-      } else {
-        for (int i = lane; i < c.head_dim; i += 32) {
-          reinterpret_cast<uint32_t *>(kb + xkd)[i] = reinterpret_cast<const uint32_t *>(kb + xks)[i];
-          reinterpret_cast<uint32_t *>(vb + xvd)[i] = reinterpret_cast<const uint32_t *>(vb + xvs)[i];
+          if (es == 2) {
+            reinterpret_cast<uint16_t *>(kb + xkd)[i] = reinterpret_cast<const uint16_t *>(kb + xks)[i];
+            reinterpret_cast<uint16_t *>(vb + xvd)[i] = reinterpret_cast<const uint16_t *>(vb + xvs)[i];
+          } else {
+            reinterpret_cast<uint32_t *>(kb + xkd)[i] = reinterpret_cast<const uint32_t *>(kb + xks)[i];
+            reinterpret_cast<uint32_t *>(vb + xvd)[i] = reinterpret_cast<const uint32_t *>(vb + xvs)[i];
+          }
         }
       }
     }
@@ -346,23 +421,27 @@ void launch_kv_append(const wgx_kv_append_args &a, cudaStream_t stream) {
   for (int64_t s : strides) vec = vec && (s * es) % 16 == 0;
   vec = vec && ((reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v)) & 15) == 0;
   const uint64_t units = uint64_t(a.tokens) * c.kv_heads * (vec ? c.head_dim * es / 16 : c.head_dim);
-  // enough blocks to fill the GPU; a sequence's few rows stay in one block,
-  // which then writes the counters too
-  const uint64_t want = (units + AP_THREADS - 1) / AP_THREADS;
+  // enough blocks for AP_UNITS units a thread, at most sixteen per SM; a
+  // sequence's few rows stay in one block
+  const uint64_t want = (units + AP_THREADS * AP_UNITS - 1) / (AP_THREADS * AP_UNITS);
   const uint64_t most = std::max<uint64_t>(1, uint64_t(device_sm_count()) * 16 / uint64_t(c.batch));
-  const unsigned gx = want <= 4 ? 1u : unsigned(std::min(want, most));
-  p.fused = gx == 1;
-  const dim3 grid(gx, unsigned(c.batch));
+  const dim3 grid(unsigned(std::min(want, most)), unsigned(c.batch));
+  p.counters = grid.x == 1 || (a.lengths_out != a.lengths && (!a.seen || a.seen_out != a.seen));
+  const bool wide = units >= 1ull << 30;  // 32-bit unit indices would run over
   const int th = timer_begin("append_kernel", stream);
-  if (vec)
-    append_kernel<uint4, true><<<grid, AP_THREADS, 0, stream>>>(p);
-  else if (es == 2)
-    append_kernel<uint16_t, false><<<grid, AP_THREADS, 0, stream>>>(p);
-  else
-    append_kernel<uint32_t, false><<<grid, AP_THREADS, 0, stream>>>(p);
+#define WGX_APPEND(U, STEP)                                                          \
+  do {                                                                               \
+    if (wide) append_kernel<U, STEP, uint64_t><<<grid, AP_THREADS, 0, stream>>>(p);  \
+    else append_kernel<U, STEP, uint32_t><<<grid, AP_THREADS, 0, stream>>>(p);       \
+  } while (0)
+  if (vec && es == 2) WGX_APPEND(uint4, 8);
+  else if (vec) WGX_APPEND(uint4, 4);
+  else if (es == 2) WGX_APPEND(uint16_t, 1);
+  else WGX_APPEND(uint32_t, 1);
+#undef WGX_APPEND
   check_cuda(cudaGetLastError(), "kv_append launch");
   timer_end(th, stream);
-  if (!p.fused) {
+  if (!p.counters) {
     advance_kernel<<<unsigned(c.batch + 127) / 128, 128, 0, stream>>>(p);
     check_cuda(cudaGetLastError(), "kv_append counters launch");
   }
