@@ -1,13 +1,13 @@
 // One step of beam search: selection over beams and vocabulary, and the
 // reordering of the paged cache's state.
 //
-// scan_kernel reads the logits once: each beam's row is cut into a few
-// segments, a block streams its segment tile by tile, every thread with a
-// running maximum and sum of exponentials, and keeps the segment's `beams`
-// largest logits. Nearly all logits fail one comparison with a bound that is
-// shared by the block; the few others go to their warp's list. Warps do not
-// wait for one another until the segment's end. select_kernel joins the segments of an item's beams: log sums, totals
-// and the `beams` best proposals. With a cache, reorder_kernel then writes the
+// scan_kernel streams the logits: each beam's row is cut into a few segments,
+// one wave of blocks over the GPU; a thread only keeps a running maximum and sum
+// of exponentials (8 instructions a logit). The segment's `beams` best lie with
+// the `beams` threads of the largest maxima, and are not below the smallest of
+// these: only those threads' logits are looked at again (from L2).
+// select_kernel joins the segments of an item's beams: log sums, totals and the
+// `beams` best proposals. With a cache, reorder_kernel then writes the
 // children's page tables and copies the partly filled last pages, all layers
 // in one launch.
 //
@@ -26,9 +26,7 @@ constexpr int BM_THREADS = 256;
 constexpr int BM_WARPS = BM_THREADS / 32;
 constexpr int BM_ITEMS = 16;                    // logits per thread and tile
 constexpr int BM_TILE = BM_THREADS * BM_ITEMS;  // tokens per tile
-constexpr int BM_KEEP = 128;                    // a longer list of a warp is cut to the best
-// a warp adds at most beams * BM_ITEMS logits a tile
-constexpr int BM_LIST = BM_KEEP + WGX_MAX_BEAMS * BM_ITEMS;
+constexpr int BM_LIST = 1024;                   // logits of a segment ranked by counting
 constexpr int BM_CAND = 1024;                   // proposals ranked by counting
 constexpr int BM_BLOCKS_PER_SM = 4;             // of scan_kernel: 40 KB of shared memory each
 constexpr int BM_SEL_THREADS = 256;
@@ -66,18 +64,28 @@ __device__ __forceinline__ float warp_sum(float x) {
   for (int d = 16; d; d /= 2) x += __shfl_xor_sync(~0u, x, d);
   return x;
 }
-// The lanes' keys in descending order (bitonic).
-__device__ __forceinline__ uint64_t warp_sort(uint64_t x) {
+// The lanes' keys in descending order (bitonic), each with its tag.
+__device__ __forceinline__ void warp_sort(uint64_t &x, int &tag) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int k = 2; k <= 32; k *= 2)
 #pragma unroll
     for (int j = k / 2; j; j /= 2) {
       const uint64_t y = __shfl_xor_sync(~0u, x, j);
+      const int t = __shfl_xor_sync(~0u, tag, j);
       const bool larger = ((lane & k) == 0) == ((lane & j) == 0);
-      if ((y > x) == larger) x = y;
+      // (equal keys: threads without tokens; either order will do, but both
+      // lanes must agree)
+      if (larger ? y > x : y < x) {
+        x = y;
+        tag = t;
+      }
     }
-  return x;
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // Key of a logit: larger logits first, equal ones by token. No two are equal.
@@ -93,9 +101,11 @@ template <typename T, bool VEC>
 __global__ void __launch_bounds__(BM_THREADS, BM_BLOCKS_PER_SM) scan_kernel(const __grid_constant__ BeamArgs p) {
   constexpr int EPV = VEC ? 16 / int(sizeof(T)) : 1, VECS = BM_ITEMS / EPV;
   __shared__ float red_max[BM_WARPS], red_sum[BM_WARPS];
-  __shared__ uint64_t lists[BM_WARPS][BM_LIST];
-  __shared__ uint32_t n_lists[BM_WARPS];
-  __shared__ unsigned long long bound;  // keys below it are not among the best
+  __shared__ uint64_t tops[BM_THREADS];       // the warps' sorted thread maxima
+  __shared__ uint16_t top_tid[BM_THREADS], hit[WGX_MAX_BEAMS];
+  __shared__ uint64_t bound, best[BM_WARPS];
+  __shared__ uint64_t list[BM_LIST];
+  __shared__ uint32_t n_list;
   const wgx_beam_search_args &a = p.a;
   const int row = blockIdx.y, seg = blockIdx.x, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   if (a.finished[row]) return;  // proposes eos: its logits are not needed
@@ -104,14 +114,10 @@ __global__ void __launch_bounds__(BM_THREADS, BM_BLOCKS_PER_SM) scan_kernel(cons
                int64_t(row % K) * a.logits_beam_stride;
   const int tile0 = int(int64_t(p.tiles) * seg / p.segments);
   const int tile1 = int(int64_t(p.tiles) * (seg + 1) / p.segments);
-  uint64_t *list = lists[warp];
-  uint32_t *n_list = &n_lists[warp];
-  if (lane == 0) *n_list = 0;
-  if (tid == 0) bound = 0;
-  __syncthreads();
+  if (tid == 0) n_list = 0;
 
-  // ---- item i of thread t of a tile is its token
-  // (i / EPV * BM_THREADS + t) * EPV + i % EPV; -infinity behind the end
+  // ---- unit i of thread t of a tile is its EPV tokens from
+  // (i * BM_THREADS + t) * EPV on; -infinity behind the end
   union Raw {
     uint4 u[VEC ? VECS : 1];
     T e[BM_ITEMS];
@@ -123,127 +129,150 @@ __global__ void __launch_bounds__(BM_THREADS, BM_BLOCKS_PER_SM) scan_kernel(cons
     for (int i = 0; i < VECS; ++i) {
       const int o = (i * BM_THREADS + tid) * EPV;
       if (VEC && o + EPV <= cnt) {
-        r.u[VEC ? i : 0] = __ldcs(reinterpret_cast<const uint4 *>(x + t0 + o));
+        r.u[VEC ? i : 0] = *reinterpret_cast<const uint4 *>(x + t0 + o);
       } else {
 #pragma unroll
         for (int j = 0; j < EPV; ++j) r.e[i * EPV + j] = o + j < cnt ? x[t0 + o + j] : T(-INFINITY);
       }
     }
   };
+  // NaN counts as -infinity (fmaxf takes its other operand)
+  auto value = [](T e) { return fmaxf(float(e), -INFINITY); };
+  constexpr float kLog2e = 1.4426950408889634f;
   float m = -INFINITY, sum = 0.f;  // of this thread
+  int top_tile = tile0;            // the first tile with its maximum
   Raw next;
   load(tile0, next);
+#pragma unroll 1
   for (int tile = tile0; tile < tile1; ++tile) {
     float v[BM_ITEMS];
     float mx = -INFINITY;
 #pragma unroll
     for (int i = 0; i < BM_ITEMS; ++i) {
-      v[i] = float(next.e[i]);
-      if (v[i] != v[i]) v[i] = -INFINITY;  // NaN
+      v[i] = value(next.e[i]);
       mx = fmaxf(mx, v[i]);
     }
     if (tile + 1 < tile1) load(tile + 1, next);
-    // ---- running maximum and sum
     if (mx > m) {
-      sum *= __expf(m - mx);
+      sum *= exp2_approx((m - mx) * kLog2e);
       m = mx;
+      top_tile = tile;
     }
     const float mu = m == -INFINITY ? 0.f : m;
     float s0 = 0.f, s1 = 0.f;
 #pragma unroll
     for (int i = 0; i < BM_ITEMS; i += 2) {
-      s0 += __expf(v[i] - mu);
-      s1 += __expf(v[i + 1] - mu);
+      s0 += exp2_approx((v[i] - mu) * kLog2e);  // (the difference is exact near the maximum)
+      s1 += exp2_approx((v[i + 1] - mu) * kLog2e);
     }
     sum += s0 + s1;
-    // ---- candidates. At least K keys of a warp are not below its K-th largest
-    // lane maximum; it is needed only where more than K lanes have candidates,
-    // and bounds what a warp adds to K lanes' logits.
-    uint64_t tau = *static_cast<volatile unsigned long long *>(&bound);
-    if (!__any_sync(~0u, ordered(mx) >= uint32_t(tau >> 32))) continue;
-    const int t0 = tile * BM_TILE, cnt = a.vocab - t0;
-    auto token = [&](int i) { return (i / EPV * BM_THREADS + tid) * EPV + i % EPV; };
-    uint64_t top = 0;
+  }
+  // ---- this thread's largest key: the first token with its maximum
+  uint64_t top = 0;
+  {
+    load(top_tile, next);
+    const int t0 = top_tile * BM_TILE;
 #pragma unroll
-    for (int i = BM_ITEMS - 1; i >= 0; --i)  // ends with the first of equal ones
-      if (v[i] == mx && token(i) < cnt) top = key_of(mx, t0 + token(i));
-    // (lanes may have read different bounds)
-    bool has = top >= tau && top;
-    if (__popc(__ballot_sync(~0u, has)) > K) {
-      const uint64_t kth = __shfl_sync(~0u, warp_sort(has ? top : 0), K - 1);
-      if (kth > tau) tau = kth;
-      if (lane == 0) atomicMax(&bound, static_cast<unsigned long long>(kth));
-      has = top >= tau && top;
-    }
-    if (has) {
-#pragma unroll
-      for (int i = 0; i < BM_ITEMS; ++i) {
-        if (ordered(v[i]) >= uint32_t(tau >> 32) && token(i) < cnt) {
-          const uint64_t k = key_of(v[i], t0 + token(i));
-          if (k >= tau) list[atomicAdd(n_list, 1u)] = k;
-        }
-      }
-    }
-    __syncwarp();
-    const int n = int(*static_cast<volatile uint32_t *>(n_list));
-    if (n > BM_KEEP) {
-      // cut to the K best: lane r keeps the one with r larger ones
-      uint64_t mine = 0;
-      for (int i0 = 0; i0 < n; i0 += 32) {
-        const uint64_t k = i0 + lane < n ? list[i0 + lane] : 0;
-        int r = 0;
-        for (int j = 0; j < n; ++j) r += list[j] > k;
-        for (int w = 0; w < K; ++w) {
-          const uint32_t who = __ballot_sync(~0u, k && r == w);
-          if (who) {
-            const uint64_t y = __shfl_sync(~0u, k, __ffs(int(who)) - 1);
-            if (lane == w) mine = y;
-          }
-        }
-      }
-      __syncwarp();
-      if (lane < K) list[lane] = mine;
-      if (lane == 0) *n_list = uint32_t(K);
-      const uint64_t kth = __shfl_sync(~0u, mine, K - 1);
-      if (lane == 0) atomicMax(&bound, static_cast<unsigned long long>(kth));
-      __syncwarp();
+    for (int i = BM_ITEMS - 1; i >= 0; --i) {
+      const int t = t0 + (i / EPV * BM_THREADS + tid) * EPV + i % EPV;
+      if (value(next.e[i]) == m && t < a.vocab) top = key_of(m, t);
     }
   }
-  // ---- join the threads
   const float wm = warp_max(m);
   const float wmu = wm == -INFINITY ? 0.f : wm;
-  const float ws = warp_sum(sum * __expf(m - wmu));
+  const float ws = warp_sum(sum * exp2_approx((m - wmu) * kLog2e));
   if (lane == 0) red_max[warp] = wm, red_sum[warp] = ws;
+  // ---- the K threads with the largest keys: they are among the K first of
+  // their warps
+  int who = tid;
+  warp_sort(top, who);
+  tops[tid] = top;
+  top_tid[tid] = uint16_t(who);
+  if (tid == 0) bound = 0;
   __syncthreads();
   const int64_t out = int64_t(row) * p.segments + seg;
   if (tid == 0) {
     float M = red_max[0], all = 0.f;
     for (int w = 1; w < BM_WARPS; ++w) M = fmaxf(M, red_max[w]);
     const float mu = M == -INFINITY ? 0.f : M;
-    for (int w = 0; w < BM_WARPS; ++w) all += red_sum[w] * __expf(red_max[w] - mu);
+    for (int w = 0; w < BM_WARPS; ++w) all += red_sum[w] * exp2_approx((red_max[w] - mu) * kLog2e);
     p.seg_ms[out] = make_float2(M, all);
   }
-  // ---- the lists' best, in order: a key not below the bound counts the larger
-  // ones of all lists
-  const uint64_t tau = bound;
-  int n = 0;
-  for (int w = 0; w < BM_WARPS; ++w) n += int(n_lists[w]);
-  for (int i = tid; i < n; i += BM_THREADS) {
-    int w = 0, e = i;
-    while (e >= int(n_lists[w])) e -= int(n_lists[w++]);
-    const uint64_t k = lists[w][e];
-    if (k < tau) continue;
+  if (tid < BM_WARPS * K) {
+    const int w = tid / K, e = tid % K;
+    const uint64_t k = tops[w * 32 + e];
     int r = 0;
-    for (int o = 0; o < BM_WARPS; ++o) {
-      const int m = int(n_lists[o]);
-      for (int j = 0; j < m; ++j) r += lists[o][j] > k;
-    }
-    if (r < K) {
-      p.top_x[out * K + r] = unordered(uint32_t(k >> 32));
-      p.top_t[out * K + r] = int(~uint32_t(k));
+    for (int o = 0; o < BM_WARPS; ++o)
+      for (int j = 0; j < K; ++j) r += tops[o * 32 + j] > k;
+    if (k && r < K) {  // (0: a thread without tokens)
+      hit[r] = top_tid[w * 32 + e];
+      if (r == K - 1) bound = k;
     }
   }
-  if (tid >= n && tid < K) p.top_t[out * K + tid] = -1;
+  const int hits = min(K, __syncthreads_count(top != 0));
+  // ---- their logits that are not below the bound
+  const int units = (tile1 - tile0) * VECS, all = hits * units;
+  const uint64_t tau = bound;
+  auto each = [&](auto &&f) {
+    for (int q = tid; q < all; q += BM_THREADS) {
+      const int r = q / units, u = q - r * units, tile = tile0 + u / VECS;
+      const int t = tile * BM_TILE + (u % VECS * BM_THREADS + hit[r]) * EPV;
+      if (VEC && t + EPV <= a.vocab) {
+        const uint4 raw = *reinterpret_cast<const uint4 *>(x + t);
+        const T *e = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+        for (int j = 0; j < EPV; ++j) f(key_of(value(e[j]), t + j));
+      } else {
+        for (int j = 0; j < EPV; ++j)
+          if (t + j < a.vocab) f(key_of(value(x[t + j]), t + j));
+      }
+    }
+  };
+  each([&](uint64_t k) {
+    if (k >= tau) {
+      const uint32_t at = atomicAdd(&n_list, 1u);
+      if (at < BM_LIST) list[at] = k;
+    }
+  });
+  __syncthreads();
+  const int n = int(n_list), want = min(n, K);
+  auto emit = [&](int r, uint64_t k) {
+    p.top_x[out * K + r] = unordered(uint32_t(k >> 32));
+    p.top_t[out * K + r] = int(~uint32_t(k));
+  };
+  if (tid >= want && tid < K) p.top_t[out * K + tid] = -1;
+  if (n <= BM_LIST) {
+    for (int i = tid; i < n; i += BM_THREADS) {
+      const uint64_t k = list[i];
+      int r = 0;
+      for (int j = 0; j < n; ++j) r += list[j] > k;
+      if (r < K) emit(r, k);
+    }
+  } else {
+    // a few threads hold very many of the largest logits: one maximum after
+    // another
+    uint64_t below = ~uint64_t(0);
+    for (int r = 0; r < want; ++r) {
+      uint64_t k = 0;
+      each([&](uint64_t y) {
+        if (y < below && y > k) k = y;
+      });
+#pragma unroll
+      for (int d = 16; d; d /= 2) {
+        const uint64_t y = __shfl_xor_sync(~0u, k, d);
+        if (y > k) k = y;
+      }
+      if (lane == 0) best[warp] = k;
+      __syncthreads();
+      k = best[0];
+#pragma unroll
+      for (int w = 1; w < BM_WARPS; ++w)
+        if (best[w] > k) k = best[w];
+      __syncthreads();
+      if (tid == 0) emit(r, k);
+      below = k;
+    }
+  }
 }
 
 struct Proposal {
