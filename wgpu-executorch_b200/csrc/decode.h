@@ -47,6 +47,24 @@ inline int current_device() {
 }
 
 #ifdef __CUDACC__
+// Launches a kernel that may be set up while the stream's previous kernel ends
+// (it calls griddepcontrol.wait before it touches what that one writes).
+template <typename... P, typename... A>
+void launch_dependent(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t stream,
+                      const char *what, const A &...args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(unsigned(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  check_cuda(cudaLaunchKernelEx(&cfg, kernel, args...), what);
+}
+
 // Slots in use of sequence b, held within [0, capacity].
 __device__ __forceinline__ int slots_in_use(const int32_t *lengths, int b, int64_t capacity,
                                             uint32_t *err) {

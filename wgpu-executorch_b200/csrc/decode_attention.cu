@@ -35,11 +35,10 @@ namespace wgx {
 
 namespace {
 
-constexpr int PA_WARPS = 4;
 constexpr int PA_HEADS = 16;        // rows of an mma tile
 constexpr int PA_MAX_GROUP = 128;   // query heads per K/V head
 constexpr int PA_JOIN_THREADS = 256;
-constexpr int PA_JOIN_SLOTS = 1024;  // slots per join block of the accumulation
+constexpr int PA_JOIN_SLOTS = 2048;  // slots per join block of the accumulation
 
 struct AttnArgs {
   CUtensorMap k_map, v_map;  // where tma: [page][head][slot][channel] in boxes of TOK rows
@@ -59,6 +58,7 @@ struct AttnArgs {
   float2 *stats;      // [row][heads]: of rows finished by one warp (accumulation only)
   float *scores;      // [batch][q_heads][score_stride] (accumulation only)
   int64_t score_stride;
+  int weights_quads;  // weights move four slots at a time
   int heads;          // min(group, PA_HEADS): rows a partial result has
   uint32_t *err;
 };
@@ -117,23 +117,37 @@ __device__ void build_prefix(const AttnArgs &p, uint32_t *prefix, int *lens) {
   __syncthreads();
 }
 
-__device__ __forceinline__ int worker_count(const AttnArgs &p, uint64_t total) {
-  const uint64_t want = (total + p.min_steps - 1) / p.min_steps;
-  return int(want < uint64_t(p.max_workers) ? (want ? want : 1) : uint64_t(p.max_workers));
+__device__ __forceinline__ uint32_t worker_count(const AttnArgs &p, uint32_t total) {
+  const uint32_t want = (total + uint32_t(p.min_steps) - 1) / uint32_t(p.min_steps);
+  return max(1u, min(want, uint32_t(p.max_workers)));
 }
-__device__ __forceinline__ uint64_t share_begin(uint64_t total, int worker, int workers) {
-  return total * uint64_t(worker) / uint64_t(workers);
-}
-// the worker whose share holds step s
-__device__ __forceinline__ int worker_of(uint64_t s, uint64_t total, int workers) {
-  return int(((s + 1) * uint64_t(workers) - 1) / total);
-}
+// Equal shares of the line: the first `extra` workers take base + 1 steps.
+struct Shares {
+  uint32_t base, extra;
+  __device__ __forceinline__ Shares(uint32_t total, uint32_t workers) {
+    base = total / workers;
+    extra = total - base * workers;
+  }
+  __device__ __forceinline__ uint32_t begin(uint32_t worker) const { return base * worker + min(worker, extra); }
+  // the worker whose share holds step s (base is at least 1: there are no more
+  // workers than steps)
+  __device__ __forceinline__ uint32_t of(uint32_t s) const {
+    const uint32_t cut = extra * (base + 1);
+    return s < cut ? s / (base + 1) : extra + (s - cut) / base;
+  }
+};
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
                "r"(live ? 16 : 0)
                : "memory");
 }
+// Programmatic dependent launch: the join's blocks may be set up while the
+// attention's work ends; wait() returns when all of it is done and visible.
+__device__ __forceinline__ void let_dependents_launch() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void wait_for_prior_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -187,17 +201,13 @@ template <typename T, int DP>
 struct Tile {
   static constexpr bool kHalf = sizeof(T) == 2;
   static constexpr int TOK = kHalf ? 16 : 8;        // slots per step
+  static constexpr uint32_t FULL = (1u << TOK) - 1;
   static constexpr int EPC = 16 / int(sizeof(T));   // elements per 16-byte chunk
   static constexpr int CPR = DP / EPC;              // chunks per staged row
   static constexpr int ROW = DP * int(sizeof(T));   // staged row bytes
   static constexpr int STAGE = 2 * TOK * ROW;       // K and V of one step
-  // fp32 rows of 256 channels: the query's registers would not fit beside
-  // the result's, so it stays in shared memory
-  static constexpr bool kQShared = !kHalf && DP > 128;
-  static constexpr int STAGES = kQShared ? 2 : STAGE > 4096 ? 3 : 4;
-  static_assert(STAGES <= 4, "the live bits of the ring are 4 x 16");
-  static constexpr int QBYTES = kQShared ? PA_HEADS * ROW : 0;
-  static constexpr int RING = STAGES * STAGE + QBYTES;  // per warp
+  static constexpr int PANEL = 128 / int(sizeof(T));  // channels per 128 bytes
+  static constexpr int PANELS = DP / PANEL;
   // Byte of chunk c of row r: panels of 128 bytes x TOK rows, chunks of a row
   // permuted by the row's low bits (the 128-byte swizzle of a TMA copy), so
   // that eight rows' equal chunks lie in different banks.
@@ -229,9 +239,9 @@ struct Walk {
   Span s;
 
   __device__ __forceinline__ void start(const AttnArgs &p, const uint32_t *prefix, const int *lens,
-                                        int rows, uint64_t begin) {
+                                        int rows, uint32_t begin) {
     // the sequence whose rows hold `begin`
-    const uint32_t key = uint32_t(begin / uint64_t(rows));
+    const uint32_t key = begin / uint32_t(rows);
     int lo = 0, hi = p.a.cache.batch - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) / 2;
@@ -240,9 +250,9 @@ struct Walk {
     }
     b = lo;
     s = span_of<TOK>(p, lens[lo]);
-    const uint64_t rest = begin - uint64_t(prefix[lo]) * uint64_t(rows);
-    row = int(rest / uint64_t(s.steps));
-    step = int(rest - uint64_t(row) * uint64_t(s.steps));
+    const uint32_t rest = begin - prefix[lo] * uint32_t(rows);
+    row = int(rest / uint32_t(s.steps));
+    step = int(rest) - row * s.steps;
   }
   __device__ __forceinline__ void next_row(const AttnArgs &p, const int *lens, int rows) {
     step = 0;
@@ -255,114 +265,96 @@ struct Walk {
   }
 };
 
-// One warp's whole work. HALF_ROWS: at most 8 heads (rows 8-15 of the tiles
-// are padding and their softmax is left out).
-template <typename T, int DP, bool HALF_ROWS>
-__global__ void __launch_bounds__(PA_WARPS * 32)
-    paged_attention_kernel(const __grid_constant__ AttnArgs p) {
+// A worker's loads: its share of the line of work through a ring of STAGES
+// steps in shared memory. Every warp of the worker keeps this state; the leader
+// issues the copies. What a step needs to know (with scattered rows its page and
+// slot per lane, its mask) is fetched one step ahead of its use, page table
+// entries 32 pages ahead.
+template <typename T, int DP, int STAGES>
+struct Loader {
   using L = Tile<T, DP>;
-  constexpr int TOK = L::TOK, STAGES = L::STAGES, NT = DP / 8;
-  constexpr int HALVES = HALF_ROWS ? 1 : 2;
-  constexpr uint32_t FULL = (1u << TOK) - 1;
-  constexpr int PANEL = 128 / int(sizeof(T)), PANELS = DP / PANEL;  // channels per 128 bytes
-  extern __shared__ uint8_t pa_smem_raw[];
-  __shared__ __align__(8) uint64_t bars[PA_WARPS][STAGES];
-  uint8_t *pa_smem = reinterpret_cast<uint8_t *>(
-      (reinterpret_cast<uintptr_t>(pa_smem_raw) + 1023) & ~uintptr_t(1023));
-  const wgx_kv_cache &c = p.a.cache;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  uint8_t *ring = pa_smem + size_t(warp) * L::RING;
-  uint32_t *prefix = reinterpret_cast<uint32_t *>(pa_smem + size_t(PA_WARPS) * L::RING);
-  int *lens = reinterpret_cast<int *>(prefix + c.batch + 1);
-  const int D = c.head_dim;
-  if (lane == 0) {
-    for (int s = 0; s < STAGES; ++s) mbar_init(smem_u32(&bars[warp][s]), p.tma ? 1 : 32);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  build_prefix<TOK>(p, prefix, lens);
-  if (D < DP) {
-    // chunks behind the rows' ends: read by the products (with zero queries),
-    // never loaded
-    for (int i = lane * 16; i < L::RING; i += 512)
-      *reinterpret_cast<uint4 *>(ring + i) = make_uint4(0u, 0u, 0u, 0u);
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    __syncwarp();
-  }
-  const int rows = c.kv_heads * p.chunks;
-  const uint64_t total = uint64_t(prefix[c.batch]) * uint64_t(rows);
-  const int workers = worker_count(p, total);
-  const int me = warp * int(gridDim.x) + int(blockIdx.x);
-  if (total == 0 || me >= workers) return;
-  const uint64_t begin = share_begin(total, me, workers), end = share_begin(total, me + 1, workers);
-  if (begin >= end) return;
-
-  // ---- loads. The next step's page (and, with scattered rows, this lane's
-  // slot) is fetched one step ahead of its use.
+  static constexpr int TOK = L::TOK;
+  static_assert(STAGES <= 4, "the live bits of the ring are 4 x 16");
   Walk<TOK> ld;
-  ld.start(p, prefix, lens, rows, begin);
-  Walk<TOK> cur = ld;
-  uint32_t to_load = uint32_t(end - begin), to_do = to_load;
-  int head = 0, left = 0;              // K/V head and steps left of the row being loaded
-  int t0 = 0, slot = 0, page = -1;     // next step: first slot, its place in its page
-  const int32_t *entry = nullptr;      // its page table entry (of its first slot)
-  uint32_t bits = 0;                   // its live slots
-  auto fetch_live = [&]() {
-    if (t0 >= ld.s.lo && t0 + TOK <= ld.s.len && !p.a.mask) {
-      bits = FULL;
-    } else {
-      const int t = t0 + lane;
-      bool live = lane < TOK && t >= ld.s.lo && t < ld.s.len;
-      if (p.a.mask && live)
-        live = t < p.a.mask_width && p.a.mask[int64_t(ld.b) * p.a.mask_stride + t] != 0;
-      bits = __ballot_sync(~0u, live);
-    }
+  uint32_t to_load;
+  int head, left;            // K/V head and steps left of the row being loaded
+  int t0, slot, page;        // next step: first slot, its place in its page, page
+  // the row's page table, 32 entries in a register (one per lane) and the next
+  // 32 in another: entry `at` of the first is the next step's
+  const int32_t *entries;
+  int pages_now, pages_next, at, known;  // known: first entry not yet loaded
+  uint32_t mine;             // lane < TOK: its slot `lane` is live
+  uint64_t live_ring;        // 16 bits of live slots per step in flight, oldest highest
+
+  __device__ __forceinline__ void fetch_live(const AttnArgs &p, int lane) {
+    const int t = t0 + lane;
+    mine = lane < TOK && t >= ld.s.lo && t < ld.s.len;
+    if (p.a.mask && mine)  // (looked at when the step is issued)
+      mine = t < p.a.mask_width ? p.a.mask[int64_t(ld.b) * p.a.mask_stride + t] : 0;
     if (!p.tma) {
       page = -1;
-      if ((bits >> lane) & 1) {
-        const int t = t0 + lane, pi = int(uint32_t(t) / uint32_t(c.page_size));
-        slot = t - pi * c.page_size;
-        page = c.page_table[int64_t(ld.b) * c.table_stride + pi];
+      if (lane < TOK && t >= ld.s.lo && t < ld.s.len) {
+        const int pi = int(uint32_t(t) / uint32_t(p.a.cache.page_size));
+        slot = t - pi * p.a.cache.page_size;
+        page = p.a.cache.page_table[int64_t(ld.b) * p.a.cache.table_stride + pi];
       }
     }
-  };
-  auto fetch_row = [&]() {
+  }
+  __device__ __forceinline__ int more_pages(const AttnArgs &p, int lane) {
+    const int i = known + lane;
+    known += 32;
+    return i < p.a.cache.table_width ? entries[i] : -1;
+  }
+  __device__ __forceinline__ void fetch_row(const AttnArgs &p, int lane) {
     head = ld.row / p.chunks;
     left = ld.s.steps - ld.step;
     t0 = (ld.s.first + ld.step) * TOK;
     if (p.tma) {
-      const int pi = int(uint32_t(t0) / uint32_t(c.page_size));
-      slot = t0 - pi * c.page_size;
-      entry = c.page_table + int64_t(ld.b) * c.table_stride + pi;
-      page = *entry;
+      const int pi = int(uint32_t(t0) / uint32_t(p.a.cache.page_size));
+      slot = t0 - pi * p.a.cache.page_size;
+      entries = p.a.cache.page_table + int64_t(ld.b) * p.a.cache.table_stride;
+      known = pi;
+      at = 0;
+      pages_now = more_pages(p, lane);
+      pages_next = more_pages(p, lane);
     }
-    fetch_live();
-  };
-  uint64_t live_ring = 0;  // 16 bits of live slots per step in flight, oldest highest
-  const T *kbase = static_cast<const T *>(c.k), *vbase = static_cast<const T *>(c.v);
-  auto issue = [&](int stage) {
-    const bool bad = uint32_t(page) >= uint32_t(c.pages);
-    if (p.tma) {
-      if (bad && bits) {
-        if (lane == 0) atomicOr(p.err, kErrCache);
-        bits = 0;
-      }
-    } else {
-      const bool was = (bits >> lane) & 1;
-      if (was && bad) atomicOr(p.err, kErrCache);
-      bits = __ballot_sync(~0u, was && !bad);
+    fetch_live(p, lane);
+  }
+  __device__ __forceinline__ void start(const AttnArgs &p, const Walk<TOK> &from, uint32_t steps, int lane) {
+    ld = from;
+    to_load = steps;
+    slot = 0;
+    page = -1;
+    live_ring = 0;
+    fetch_row(p, lane);
+  }
+  // the live slots of the step that is to be used next
+  __device__ __forceinline__ uint32_t oldest() const {
+    return uint32_t(live_ring >> (16 * (STAGES - 2))) & 0xffffu;
+  }
+  __device__ __forceinline__ void issue(const AttnArgs &p, uint8_t *stage_p, uint32_t bar, int lane,
+                                        bool leader) {
+    const wgx_kv_cache &c = p.a.cache;
+    if (p.tma) page = __shfl_sync(~0u, pages_now, at);
+    bool on = mine != 0;
+    if (on && uint32_t(page) >= uint32_t(c.pages)) {
+      atomicOr(p.err, kErrCache);
+      on = false;
     }
+    const uint32_t bits = __ballot_sync(~0u, on);
     live_ring = (live_ring << 16) | bits;
-    if (!bits) return;  // nothing to load: the step is passed over
-    uint8_t *sk = ring + stage * L::STAGE, *sv = sk + TOK * L::ROW;
-    const uint32_t bar = smem_u32(&bars[warp][stage]);
+    if (!bits || !leader) return;  // (no live slot: the step is passed over)
+    uint8_t *sk = stage_p, *sv = sk + TOK * L::ROW;
+    const T *kbase = static_cast<const T *>(c.k), *vbase = static_cast<const T *>(c.v);
+    const int D = c.head_dim;
     if (p.tma) {
       if (lane == 0) {
         const uint32_t ska = smem_u32(sk), sva = smem_u32(sv);
         // (a box counts in full, its part outside the tensor too)
-        mbar_expect_tx(bar, uint32_t(2 * TOK * 128) * uint32_t((D + PANEL - 1) / PANEL));
+        mbar_expect_tx(bar, uint32_t(2 * TOK * 128) * uint32_t((D + L::PANEL - 1) / L::PANEL));
         for (int j = 0; j < p.boxes; ++j) {
-          tma_load_5d(ska + uint32_t(j * TOK * 128), &p.k_map, j * PANEL, slot, 0, head, page, bar);
-          tma_load_5d(sva + uint32_t(j * TOK * 128), &p.v_map, j * PANEL, slot, 0, head, page, bar);
+          tma_load_5d(ska + uint32_t(j * TOK * 128), &p.k_map, j * L::PANEL, slot, 0, head, page, bar);
+          tma_load_5d(sva + uint32_t(j * TOK * 128), &p.v_map, j * L::PANEL, slot, 0, head, page, bar);
         }
       }
       return;
@@ -397,36 +389,161 @@ __global__ void __launch_bounds__(PA_WARPS * 32)
       }
       mbar_arrive(bar);
     }
-  };
-  auto load_next = [&](int stage) {
+  }
+  __device__ __forceinline__ void next(const AttnArgs &p, const int *lens, int rows, uint8_t *ring,
+                                       uint64_t *bars, int stage, int lane, bool leader) {
     if (!to_load) {
       live_ring <<= 16;
       return;
     }
-    issue(stage);
+    issue(p, ring + stage * L::STAGE, smem_u32(&bars[stage]), lane, leader);
     if (!--to_load) return;
     if (--left == 0) {
       ld.next_row(p, lens, rows);
-      fetch_row();
+      fetch_row(p, lane);
     } else {
       t0 += TOK;
       if (p.tma) {
         slot += TOK;
-        if (slot == c.page_size) {
+        if (slot == p.a.cache.page_size) {
           slot = 0;
-          page = *++entry;
+          if (++at == 32) {
+            at = 0;
+            pages_now = pages_next;
+            pages_next = more_pages(p, lane);
+          }
         }
       }
-      fetch_live();
+      fetch_live(p, lane);
+    }
+  }
+};
+
+// What the pages hold in slots that are not live must not reach 0 * v.
+template <typename T, int DP>
+__device__ __forceinline__ void clear_dead_rows(uint32_t va, uint32_t live, int lane) {
+  using L = Tile<T, DP>;
+  for (int r = 0; r < L::TOK; ++r)
+    if (!((live >> r) & 1))
+      for (int ch = lane; ch < L::CPR; ch += 32)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(va + L::at(r, ch)), "r"(0) : "memory");
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+}
+
+// A worker after a wait ran out: nothing may be in flight when it leaves, so it
+// waits (bounded) for the stages behind the one that did not arrive.
+template <int STAGES>
+__device__ void drain(uint64_t live_ring, uint64_t *bars, int stage, uint32_t phase) {
+  stage = stage + 1 == STAGES ? 0 : stage + 1;
+  for (int s = 1; s < STAGES - 1; ++s) {
+    const uint32_t live = uint32_t(live_ring >> (16 * (STAGES - 2 - s))) & 0xffffu;
+    if (live) mbar_wait(smem_u32(&bars[stage]), (phase >> stage) & 1);
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
+  }
+}
+
+// Shared memory of a block: the workers' rings (1024-byte aligned), then the
+// sequences' prefix and lengths.
+struct BlockSmem {
+  uint8_t *ring;
+  uint32_t *prefix;
+  int *lens;
+};
+__device__ __forceinline__ BlockSmem block_smem(uint8_t *raw, int worker, int ring_bytes, int workers, int batch) {
+  uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  BlockSmem m;
+  m.ring = base + size_t(worker) * ring_bytes;
+  m.prefix = reinterpret_cast<uint32_t *>(base + size_t(workers) * ring_bytes);
+  m.lens = reinterpret_cast<int *>(m.prefix + batch + 1);
+  return m;
+}
+
+constexpr int PA_BLOCK_WORKERS = 4;
+
+// Tensor-core form: the worker's heads are the 16 rows of an mma tile.
+// HALF_ROWS: at most 8 heads (rows 8-15 are padding and their softmax is left
+// out). Heads of 256 channels: two warps share a worker; both form the scores,
+// each the result of its half of the channels (one warp's 128 result registers
+// beside 64 of the query left room for one warp per scheduler).
+template <typename T, int DP>
+struct MmaShape {
+  static constexpr int WARPS = DP > 128 ? 2 : 1;  // per worker
+  // fp32 rows of 256 channels: the query's registers would not fit beside the
+  // result's, so it stays in shared memory
+  static constexpr bool kQShared = sizeof(T) == 4 && DP > 128;
+  static constexpr int STAGES = kQShared ? 2 : Tile<T, DP>::STAGE > 4096 ? 3 : 4;
+  static constexpr int QBYTES = kQShared ? PA_HEADS * Tile<T, DP>::ROW : 0;
+  static constexpr int RING = STAGES * Tile<T, DP>::STAGE + QBYTES;
+  static constexpr int THREADS = PA_BLOCK_WORKERS * WARPS * 32;
+  static_assert(PA_BLOCK_WORKERS * RING + 1024 + (2 * 2048 + 1) * 4 <= 227 * 1024, "shared memory of a block");
+};
+
+template <typename T, int DP, bool HALF_ROWS>
+__global__ void __launch_bounds__(MmaShape<T, DP>::THREADS)
+    paged_attention_kernel(const __grid_constant__ AttnArgs p) {
+  using L = Tile<T, DP>;
+  using M = MmaShape<T, DP>;
+  constexpr int TOK = L::TOK, STAGES = M::STAGES, PANEL = L::PANEL;
+  constexpr int WP = L::PANELS / M::WARPS, NT = DP / 8 / M::WARPS;  // this warp's panels and tiles of the result
+  constexpr int HALVES = HALF_ROWS ? 1 : 2, ST = TOK / 8;
+  extern __shared__ uint8_t pa_smem_raw[];
+  __shared__ __align__(8) uint64_t all_bars[PA_BLOCK_WORKERS][STAGES];
+  const wgx_kv_cache &c = p.a.cache;
+  const int lane = threadIdx.x % 32, worker = threadIdx.x / (32 * M::WARPS);
+  const int part = threadIdx.x / 32 % M::WARPS;  // of the worker
+  let_dependents_launch();
+  const BlockSmem sm = block_smem(pa_smem_raw, worker, M::RING, PA_BLOCK_WORKERS, c.batch);
+  uint64_t *bars = all_bars[worker];
+  const int D = c.head_dim;
+  // barrier among the worker's warps; true when all of their threads say so
+  auto worker_all = [&](bool mine) -> bool {
+    if constexpr (M::WARPS == 1) {
+      return __all_sync(~0u, mine);
+    } else {
+      uint32_t all;
+      asm volatile(
+          "{\n\t.reg .pred a, b;\n\t"
+          "setp.ne.u32 a, %1, 0;\n\t"
+          "barrier.cta.red.and.pred b, %2, %3, a;\n\t"
+          "selp.u32 %0, 1, 0, b;\n\t}"
+          : "=r"(all)
+          : "r"(uint32_t(mine)), "r"(worker + 1), "n"(M::WARPS * 32)
+          : "memory");
+      return all != 0;
     }
   };
-  fetch_row();
-#pragma unroll 1
-  for (int s = 0; s < STAGES - 1; ++s) load_next(s);
+  if (part == 0 && lane == 0) {
+    for (int s = 0; s < STAGES; ++s) mbar_init(smem_u32(&bars[s]), p.tma ? 1 : 32);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (D < DP && part == 0) {
+    // chunks behind the rows' ends: read by the products (with zero queries),
+    // never loaded
+    for (int i = lane * 16; i < M::RING; i += 512)
+      *reinterpret_cast<uint4 *>(sm.ring + i) = make_uint4(0u, 0u, 0u, 0u);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  build_prefix<TOK>(p, sm.prefix, sm.lens);  // (ends with a block barrier)
+  const int rows = c.kv_heads * p.chunks;
+  const uint32_t total = sm.prefix[c.batch] * uint32_t(rows);
+  const uint32_t workers = worker_count(p, total);
+  const uint32_t me = uint32_t(worker) * gridDim.x + blockIdx.x;
+  if (total == 0 || me >= workers) return;
+  const Shares shares(total, workers);
+  const uint32_t begin = shares.begin(me), end = shares.begin(me + 1);
 
-  uint32_t qf[L::kQShared ? 1 : (L::kHalf ? DP / 16 : DP / 8)][4];
+  Walk<TOK> cur;
+  cur.start(p, sm.prefix, sm.lens, rows, begin);
+  uint32_t to_do = end - begin;
+  Loader<T, DP, STAGES> loader;
+  loader.start(p, cur, to_do, lane);
+#pragma unroll 1
+  for (int s = 0; s < STAGES - 1; ++s) loader.next(p, sm.lens, rows, sm.ring, bars, s, lane, part == 0);
+
+  uint32_t qf[M::kQShared ? 1 : (L::kHalf ? DP / 16 : DP / 8)][4];
   float o[NT][4];
-  const uint32_t ring_a = smem_u32(ring);
+  const uint32_t ring_a = smem_u32(sm.ring);
   // Bytes of this lane's chunks within a panel of K and of V (L::at): the
   // permutation is an exclusive or, so a panel's four operand columns cost four
   // numbers, and panels are constant offsets.
@@ -443,13 +560,15 @@ __global__ void __launch_bounds__(PA_WARPS * 32)
       v0 = uint32_t(vt * 128 + (((lane >> 4) ^ vt) << 4) + in);
       v1 = uint32_t((vt + 1) * 128 + (((lane >> 4) ^ (vt + 1)) << 4) + in);
     }
+    const uint32_t mine = uint32_t(part * WP * TOK * 128);  // this warp's panels of V
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       kx[i] = k0 ^ uint32_t(32 * i);
-      vx[i] = v0 ^ uint32_t(32 * i);
-      if constexpr (!L::kHalf) vx[4 + i] = v1 ^ uint32_t(32 * i);
+      vx[i] = (v0 ^ uint32_t(32 * i)) + mine;
+      if constexpr (!L::kHalf) vx[4 + i] = (v1 ^ uint32_t(32 * i)) + mine;
     }
   }
+  const int d0 = part * WP * PANEL;  // this warp's first channel of the result
   int stage = 0;
   uint32_t phase = 0;  // bit s: parity of stage s's next wait
   bool ok = true;
@@ -483,21 +602,19 @@ __global__ void __launch_bounds__(PA_WARPS * 32)
               qf[kk][j] = *reinterpret_cast<const uint32_t *>(&v);
             }
           }
-      } else if constexpr (!L::kQShared) {
+      } else if constexpr (!M::kQShared) {
 #pragma unroll
         for (int kk = 0; kk < DP / 8; ++kk)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            qf[kk][j] = (j & 1) && HALF_ROWS
-                            ? 0u
-                            : __float_as_uint(qv(r0 + (j & 1) * 8, kk * 8 + kq + (j >> 1) * 4));
+            qf[kk][j] = __float_as_uint(qv(r0 + (j & 1) * 8, kk * 8 + kq + (j >> 1) * 4));
       } else {
-        __syncwarp();
-        for (int g = 0; g < PA_HEADS; ++g)
+        worker_all(true);
+        for (int g = part; g < PA_HEADS; g += M::WARPS)
           for (int d = lane; d < DP; d += 32)
-            *reinterpret_cast<T *>(ring + STAGES * L::STAGE + g * L::ROW +
+            *reinterpret_cast<T *>(sm.ring + STAGES * L::STAGE + g * L::ROW +
                                    (((d / 4) ^ (g & 7)) << 4) + (d % 4) * 4) = qv(g, d);
-        __syncwarp();
+        worker_all(true);
       }
 #pragma unroll
       for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
@@ -507,40 +624,31 @@ __global__ void __launch_bounds__(PA_WARPS * 32)
     const uint32_t here = min(uint32_t(cur.s.steps - cur.step), to_do);
 #pragma unroll 1
     for (uint32_t i = 0; i < here; ++i) {
-      const uint32_t live = uint32_t(live_ring >> (16 * (STAGES - 2))) & 0xffffu;
+      const uint32_t live = loader.oldest();
       if (live) {
-        if (!mbar_wait(smem_u32(&bars[warp][stage]), (phase >> stage) & 1)) {
-          if (lane == 0) atomicOr(p.err, kErrLoadTimeout);
-          ok = false;
-          break;
-        }
+        ok = mbar_wait(smem_u32(&bars[stage]), (phase >> stage) & 1);
         phase ^= 1u << stage;
       }
-      __syncwarp();  // the stage before this one is free
-      load_next(stage == 0 ? STAGES - 1 : stage - 1);
+      // (also: the stage before this one is free)
+      if (!worker_all(ok)) {
+        if (lane == 0) atomicOr(p.err, kErrLoadTimeout);
+        ok = false;
+        break;
+      }
+      loader.next(p, sm.lens, rows, sm.ring, bars, stage == 0 ? STAGES - 1 : stage - 1, lane, part == 0);
       const uint32_t ka = ring_a + uint32_t(stage * L::STAGE), va = ka + uint32_t(TOK * L::ROW);
       stage = stage + 1 == STAGES ? 0 : stage + 1;
-      constexpr int ST = TOK / 8;
       if (!live && !p.scores) continue;
+      if (live != L::FULL) clear_dead_rows<T, DP>(va, live, lane);
       // ---- scores: s[t][.] are slots t * 8 + 2 * (lane % 4) + {0, 1} of head
       // lane / 4 ([0], [1]) and lane / 4 + 8 ([2], [3])
       float s[ST][4];
 #pragma unroll
       for (int t = 0; t < ST; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
-      if (live != FULL) {
-        // what the pages hold in other slots must not reach 0 * v
-        for (int r = 0; r < TOK; ++r)
-          if (!((live >> r) & 1))
-            for (int ch = lane; ch < L::CPR; ch += 32)
-              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(va + L::at(r, ch)), "r"(0)
-                           : "memory");
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-      }
       if constexpr (L::kHalf) {
         float s2[2][4] = {};  // odd columns: sums of their own, for the pipeline
 #pragma unroll
-        for (int pn = 0; pn < PANELS; ++pn) {
+        for (int pn = 0; pn < L::PANELS; ++pn) {
           if (pn * PANEL < D) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -561,7 +669,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32)
         // small products have sums of their own, and the large ones two
         float lo[4] = {}, lo2[4] = {}, odd[4] = {};
 #pragma unroll
-        for (int pn = 0; pn < PANELS; ++pn) {
+        for (int pn = 0; pn < L::PANELS; ++pn) {
           if (pn * PANEL < D) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -569,9 +677,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32)
               uint32_t ah[4], al[4], bh[2], bl[2];
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
-                if ((j & 1) && HALF_ROWS) {
-                  ah[j] = al[j] = 0u;
-                } else if constexpr (L::kQShared) {
+                if constexpr (M::kQShared) {
                   const int g = r + (j & 1) * 8;
                   const uint32_t qa = ring_a + uint32_t(STAGES * L::STAGE + g * L::ROW + ((g & 7) << 4) + (lane & 3) * 4);
                   split_tf32(lds32(qa ^ uint32_t((2 * kk + (j >> 1)) << 4)), ah[j], al[j]);
@@ -599,7 +705,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32)
       for (int t = 0; t < ST; ++t)
 #pragma unroll
         for (int e = 0; e < 2 * HALVES; ++e) s[t][e] *= p.scale2;
-      if (live != FULL) {
+      if (live != L::FULL) {
 #pragma unroll
         for (int t = 0; t < ST; ++t)
 #pragma unroll
@@ -608,15 +714,17 @@ __global__ void __launch_bounds__(PA_WARPS * 32)
       }
       if (p.scores) {
         const int t0 = (cur.s.first + cur.step + int(i)) * TOK + 2 * (lane & 3);
+        if (part == 0) {
 #pragma unroll
-        for (int x = 0; x < HALVES; ++x) {
-          const int g = (lane >> 2) + 8 * x;
-          if (g < nh) {
-            float *w = p.scores + (int64_t(cur.b) * p.a.q_heads + h * p.group + chunk * PA_HEADS + g) *
-                                      p.score_stride + t0;
+          for (int x = 0; x < HALVES; ++x) {
+            const int g = (lane >> 2) + 8 * x;
+            if (g < nh) {
+              float *w = p.scores + (int64_t(cur.b) * p.a.q_heads + h * p.group + chunk * PA_HEADS + g) *
+                                        p.score_stride + t0;
 #pragma unroll
-            for (int t = 0; t < ST; ++t)
-              *reinterpret_cast<float2 *>(w + t * 8) = make_float2(s[t][2 * x], s[t][2 * x + 1]);
+              for (int t = 0; t < ST; ++t)
+                *reinterpret_cast<float2 *>(w + t * 8) = make_float2(s[t][2 * x], s[t][2 * x + 1]);
+            }
           }
         }
         if (!live) continue;
@@ -678,8 +786,8 @@ __global__ void __launch_bounds__(PA_WARPS * 32)
           pl[j] = pack2(s[t][2 * x] - hf.x, s[t][2 * x + 1] - hf.y);
         }
 #pragma unroll
-        for (int pn = 0; pn < PANELS; ++pn) {
-          if (pn * PANEL < D) {
+        for (int pn = 0; pn < WP; ++pn) {
+          if (d0 + pn * PANEL < D) {
             uint32_t b[4][4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) ldsm4_t(va + vx[i] + uint32_t(pn * TOK * 128), b[i]);
@@ -704,8 +812,8 @@ __global__ void __launch_bounds__(PA_WARPS * 32)
         split_tf32(s[0][1], ah[2], al[2]);
         split_tf32(s[0][3], ah[3], al[3]);
 #pragma unroll
-        for (int pn = 0; pn < PANELS; ++pn) {
-          if (pn * PANEL < D) {
+        for (int pn = 0; pn < WP; ++pn) {
+          if (d0 + pn * PANEL < D) {
             uint32_t bh[4][2], bl[4][2];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -729,7 +837,6 @@ __global__ void __launch_bounds__(PA_WARPS * 32)
         }
       }
     }
-    if (!ok) break;
     to_do -= here;
     const bool whole = from_begin && cur.step + int(here) == cur.s.steps;
 #pragma unroll
@@ -738,7 +845,7 @@ __global__ void __launch_bounds__(PA_WARPS * 32)
       sum += __shfl_xor_sync(~0u, sum, 1);
       sum += __shfl_xor_sync(~0u, sum, 2);
       const int g = (lane >> 2) + 8 * x;
-      if (g >= nh) continue;
+      if (g >= nh || !ok) continue;
       if (whole) {
         const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
         T *out = static_cast<T *>(p.a.out) + int64_t(cur.b) * p.a.out_batch_stride +
@@ -747,34 +854,289 @@ __global__ void __launch_bounds__(PA_WARPS * 32)
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const int d = n * 8 + 2 * (lane & 3) + e;
+            const int d = d0 + n * 8 + 2 * (lane & 3) + e;
             if (d < D) out[d] = T(o[n][2 * x + e] * inv);
           }
-        if (p.stats && (lane & 3) == 0)
+        if (p.stats && part == 0 && (lane & 3) == 0)
           p.stats[(int64_t(cur.b) * rows + cur.row) * PA_HEADS + g] = make_float2(m[x], sum);
       } else {
-        const int64_t part = (int64_t(me) * 2 + (from_begin ? 1 : 0)) * p.heads + g;
-        float *po = p.part_o + part * D;
+        const int64_t at = (int64_t(me) * 2 + (from_begin ? 1 : 0)) * p.heads + g;
+        float *po = p.part_o + at * D;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const int d = n * 8 + 2 * (lane & 3) + e;
+            const int d = d0 + n * 8 + 2 * (lane & 3) + e;
             if (d < D) po[d] = o[n][2 * x + e];
           }
-        if ((lane & 3) == 0) p.part_ml[part] = make_float2(m[x], sum);
+        if (part == 0 && (lane & 3) == 0) p.part_ml[at] = make_float2(m[x], sum);
       }
     }
-    cur.next_row(p, lens, rows);
+    cur.next_row(p, sm.lens, rows);
   }
-  if (!ok) {
-    // leave with nothing in flight: wait (bounded) for the other stages' copies
-    for (int s = 0; s < STAGES - 1; ++s) {
-      const uint32_t live = uint32_t(live_ring >> (16 * (STAGES - 2 - s))) & 0xffffu;
-      if (live) mbar_wait(smem_u32(&bars[warp][stage]), (phase >> stage) & 1);
-      stage = stage + 1 == STAGES ? 0 : stage + 1;
+  if (!ok) drain<STAGES>(loader.live_ring, bars, stage, phase);
+}
+
+// CUDA-core form for fp32 caches and groups of at most 8 heads (G: the group
+// rounded up to 1, 2, 4, 8): 2 * G multiply-adds per cached element, exact
+// products. On the tensor cores a step of 8 slots costs the same whatever the
+// group (about 450 instructions and the operands' splitting); here 80 * G and
+// about 100 more.
+template <int DP, int G>
+struct SimtShape {
+  static constexpr int STAGES = DP > 128 && G > 2 ? 2 : Tile<float, DP>::STAGE > 4096 ? 3 : 4;
+  static constexpr int QBYTES = G * DP * 4;
+  static constexpr int PBYTES = 8 * G * 4;
+  static constexpr int RING = (STAGES * Tile<float, DP>::STAGE + QBYTES + PBYTES + 1023) / 1024 * 1024;
+  static constexpr int THREADS = PA_BLOCK_WORKERS * 32;
+  static_assert(PA_BLOCK_WORKERS * RING + 1024 + (2 * 2048 + 1) * 4 <= 227 * 1024, "shared memory of a block");
+};
+
+__device__ __forceinline__ float4 lds128(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+
+template <int DP, int G>
+__global__ void __launch_bounds__(SimtShape<DP, G>::THREADS)
+    paged_attention_simt_kernel(const __grid_constant__ AttnArgs p) {
+  using L = Tile<float, DP>;
+  using M = SimtShape<DP, G>;
+  constexpr int TOK = 8, STAGES = M::STAGES, CHUNKS = DP / 4;
+  constexpr int LANES = CHUNKS < 32 ? CHUNKS : 32;  // lanes over a row of V
+  constexpr int SPLIT = 32 / LANES;                 // slots at a time
+  constexpr int OV = CHUNKS / LANES;                // chunks of the result per lane
+  extern __shared__ uint8_t pa_smem_raw[];
+  __shared__ __align__(8) uint64_t all_bars[PA_BLOCK_WORKERS][STAGES];
+  const wgx_kv_cache &c = p.a.cache;
+  const int lane = threadIdx.x % 32, worker = threadIdx.x / 32;
+  let_dependents_launch();
+  const BlockSmem sm = block_smem(pa_smem_raw, worker, M::RING, PA_BLOCK_WORKERS, c.batch);
+  uint64_t *bars = all_bars[worker];
+  const int D = c.head_dim;
+  if (lane == 0) {
+    for (int s = 0; s < STAGES; ++s) mbar_init(smem_u32(&bars[s]), p.tma ? 1 : 32);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (D < DP) {
+    // chunks behind the rows' ends are read but never loaded
+    for (int i = lane * 16; i < M::RING; i += 512)
+      *reinterpret_cast<uint4 *>(sm.ring + i) = make_uint4(0u, 0u, 0u, 0u);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  build_prefix<TOK>(p, sm.prefix, sm.lens);  // (ends with a block barrier)
+  const int rows = c.kv_heads;  // (p.chunks is 1)
+  const uint32_t total = sm.prefix[c.batch] * uint32_t(rows);
+  const uint32_t workers = worker_count(p, total);
+  const uint32_t me = uint32_t(worker) * gridDim.x + blockIdx.x;
+  if (total == 0 || me >= workers) return;
+  const Shares shares(total, workers);
+  const uint32_t begin = shares.begin(me), end = shares.begin(me + 1);
+
+  Walk<TOK> cur;
+  cur.start(p, sm.prefix, sm.lens, rows, begin);
+  uint32_t to_do = end - begin;
+  Loader<float, DP, STAGES> loader;
+  loader.start(p, cur, to_do, lane);
+#pragma unroll 1
+  for (int s = 0; s < STAGES - 1; ++s) loader.next(p, sm.lens, rows, sm.ring, bars, s, lane, true);
+
+  const uint32_t ring_a = smem_u32(sm.ring);
+  const uint32_t q_a = ring_a + uint32_t(STAGES * L::STAGE), p_a = q_a + uint32_t(M::QBYTES);
+  float *q_s = reinterpret_cast<float *>(sm.ring + STAGES * L::STAGE);  // [head][channel]
+  float *p_s = q_s + G * DP;                                            // [slot][head]
+  // scores: lane = quarter * 8 + slot, chunks 4 * i + quarter of the slot's row
+  const int ks = lane & 7, quarter = lane >> 3;
+  const uint32_t k0 = uint32_t(ks * 128 + ((quarter ^ ks) << 4));
+  // result: lane = half * LANES + chunk, slots SPLIT * j + half
+  const int vc = lane % LANES, half = lane / LANES;
+  int stage = 0;
+  uint32_t phase = 0;
+  bool ok = true;
+
+  while (to_do && ok) {
+    const int h = cur.row;
+    const bool from_begin = cur.step == 0;
+    const int nh = p.group;
+    float m[G], l[G];
+    float4 o[OV][G];
+    {
+      const float *q = static_cast<const float *>(p.a.q) + int64_t(cur.b) * p.a.q_batch_stride +
+                       int64_t(h) * nh * p.a.q_head_stride;
+      __syncwarp();
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        for (int d = lane; d < DP; d += 32)
+          q_s[g * DP + d] = g < nh && d < D ? q[int64_t(g) * p.a.q_head_stride + d] * p.scale2 : 0.f;
+        m[g] = -INFINITY;
+        l[g] = 0.f;
+#pragma unroll
+        for (int k = 0; k < OV; ++k) o[k][g] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      __syncwarp();
     }
+    const uint32_t here = min(uint32_t(cur.s.steps - cur.step), to_do);
+#pragma unroll 1
+    for (uint32_t i = 0; i < here; ++i) {
+      const uint32_t live = loader.oldest();
+      if (live) {
+        ok = mbar_wait(smem_u32(&bars[stage]), (phase >> stage) & 1);
+        phase ^= 1u << stage;
+      }
+      // (also: the stage before this one is free)
+      if (!__all_sync(~0u, ok)) {
+        if (lane == 0) atomicOr(p.err, kErrLoadTimeout);
+        ok = false;
+        break;
+      }
+      loader.next(p, sm.lens, rows, sm.ring, bars, stage == 0 ? STAGES - 1 : stage - 1, lane, true);
+      const uint32_t ka = ring_a + uint32_t(stage * L::STAGE), va = ka + uint32_t(TOK * L::ROW);
+      stage = stage + 1 == STAGES ? 0 : stage + 1;
+      if (!live && !p.scores) continue;
+      if (live != L::FULL) clear_dead_rows<float, DP>(va, live, lane);
+      // ---- scores of this lane's slot, a quarter of the channels each
+      float s[G];
+#pragma unroll
+      for (int g = 0; g < G; ++g) s[g] = 0.f;
+#pragma unroll
+      for (int pn = 0; pn < L::PANELS; ++pn) {
+        if (pn * L::PANEL < D) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float4 k = lds128(ka + uint32_t(pn * TOK * 128) + (k0 ^ uint32_t(64 * e)));
+            const uint32_t qc = q_a + uint32_t((pn * 8 + e * 4 + quarter) * 16);
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+              const float4 q = lds128(qc + uint32_t(g * DP * 4));
+              s[g] = fmaf(k.x, q.x, s[g]);
+              s[g] = fmaf(k.y, q.y, s[g]);
+              s[g] = fmaf(k.z, q.z, s[g]);
+              s[g] = fmaf(k.w, q.w, s[g]);
+            }
+          }
+        }
+      }
+      const bool on = (live >> ks) & 1;
+      bool grew = false;
+      float mx[G];
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        s[g] += __shfl_xor_sync(~0u, s[g], 8);
+        s[g] += __shfl_xor_sync(~0u, s[g], 16);
+        s[g] = on ? s[g] : -INFINITY;
+        mx[g] = fmaxf(s[g], __shfl_xor_sync(~0u, s[g], 1));
+        mx[g] = fmaxf(mx[g], __shfl_xor_sync(~0u, mx[g], 2));
+        mx[g] = fmaxf(mx[g], __shfl_xor_sync(~0u, mx[g], 4));
+        grew |= mx[g] > m[g] + 8.f;
+      }
+      if (p.scores) {
+        if (quarter == 0) {
+          float *w = p.scores + (int64_t(cur.b) * p.a.q_heads + h * nh) * p.score_stride +
+                     (cur.s.first + cur.step + int(i)) * TOK + ks;
+          for (int g = 0; g < G; ++g)
+            if (g < nh) w[int64_t(g) * p.score_stride] = s[g];
+        }
+        if (!live) continue;
+      }
+      // ---- running softmax (see paged_attention_kernel)
+      if (grew) {  // (the same in every lane)
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          const float mn = fmaxf(m[g], mx[g]);
+          const float f = mn > m[g] ? exp2_approx(m[g] - mn) : 1.f;
+          l[g] *= f;
+          m[g] = mn;
+#pragma unroll
+          for (int k = 0; k < OV; ++k) {
+            o[k][g].x *= f;
+            o[k][g].y *= f;
+            o[k][g].z *= f;
+            o[k][g].w *= f;
+          }
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        s[g] = exp2_approx(s[g] - (m[g] == -INFINITY ? 0.f : m[g]));
+        l[g] += s[g];
+        if (quarter == 0) p_s[ks * G + g] = s[g];
+      }
+      __syncwarp();
+      // ---- result += p v
+#pragma unroll
+      for (int j = 0; j < TOK / SPLIT; ++j) {
+        const int t = j * SPLIT + half;
+        float pg[G];
+        if constexpr (G >= 4) {
+#pragma unroll
+          for (int g = 0; g < G; g += 4) {
+            const float4 y = lds128(p_a + uint32_t((t * G + g) * 4));
+            pg[g] = y.x;
+            pg[g + 1] = y.y;
+            pg[g + 2] = y.z;
+            pg[g + 3] = y.w;
+          }
+        } else {
+#pragma unroll
+          for (int g = 0; g < G; ++g) pg[g] = lds32(p_a + uint32_t((t * G + g) * 4));
+        }
+#pragma unroll
+        for (int k = 0; k < OV; ++k) {
+          if ((vc + 32 * k) * 4 < D) {
+            const float4 v = lds128(va + L::at(t, vc + 32 * k));
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+              o[k][g].x = fmaf(pg[g], v.x, o[k][g].x);
+              o[k][g].y = fmaf(pg[g], v.y, o[k][g].y);
+              o[k][g].z = fmaf(pg[g], v.z, o[k][g].z);
+              o[k][g].w = fmaf(pg[g], v.w, o[k][g].w);
+            }
+          }
+        }
+      }
+    }
+    to_do -= here;
+    const bool whole = from_begin && cur.step + int(here) == cur.s.steps;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      float sum = l[g];
+      sum += __shfl_xor_sync(~0u, sum, 1);
+      sum += __shfl_xor_sync(~0u, sum, 2);
+      sum += __shfl_xor_sync(~0u, sum, 4);
+      if constexpr (SPLIT == 2) {
+        o[0][g].x += __shfl_xor_sync(~0u, o[0][g].x, 16);
+        o[0][g].y += __shfl_xor_sync(~0u, o[0][g].y, 16);
+        o[0][g].z += __shfl_xor_sync(~0u, o[0][g].z, 16);
+        o[0][g].w += __shfl_xor_sync(~0u, o[0][g].w, 16);
+      }
+      if (g >= nh || !ok) continue;
+      const int64_t at = (int64_t(me) * 2 + (from_begin ? 1 : 0)) * p.heads + g;
+      const float inv = !whole ? 1.f : sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+      float *to = whole ? static_cast<float *>(p.a.out) + int64_t(cur.b) * p.a.out_batch_stride +
+                              int64_t(h * nh + g) * p.a.out_head_stride
+                        : p.part_o + at * D;
+      if (half == 0) {
+#pragma unroll
+        for (int k = 0; k < OV; ++k) {
+          const int d = (vc + 32 * k) * 4;
+          if (d < D) to[d] = o[k][g].x * inv;
+          if (d + 1 < D) to[d + 1] = o[k][g].y * inv;
+          if (d + 2 < D) to[d + 2] = o[k][g].z * inv;
+          if (d + 3 < D) to[d + 3] = o[k][g].w * inv;
+        }
+      }
+      if (lane == 0) {
+        if (!whole) p.part_ml[at] = make_float2(m[g], sum);
+        else if (p.stats) p.stats[(int64_t(cur.b) * rows + cur.row) * PA_HEADS + g] = make_float2(m[g], sum);
+      }
+    }
+    cur.next_row(p, sm.lens, rows);
   }
+  if (!ok) drain<STAGES>(loader.live_ring, bars, stage, phase);
 }
 
 // Block reductions of the join: all threads get the result.
@@ -816,22 +1178,23 @@ __global__ void __launch_bounds__(PA_JOIN_THREADS) join_kernel(const __grid_cons
   const wgx_kv_cache &c = p.a.cache;
   uint32_t *prefix = reinterpret_cast<uint32_t *>(jn_smem);
   int *lens = reinterpret_cast<int *>(prefix + c.batch + 1);
-  build_prefix<TOK>(p, prefix, lens);
+  build_prefix<TOK>(p, prefix, lens);  // (of the call's inputs)
+  wait_for_prior_kernel();
   const int b = blockIdx.x / c.kv_heads, h = blockIdx.x % c.kv_heads, y = blockIdx.y;
   const int rows = c.kv_heads * p.chunks, D = c.head_dim, tid = threadIdx.x;
-  const uint64_t total = uint64_t(prefix[c.batch]) * uint64_t(rows);
-  const int workers = worker_count(p, total);
+  const uint32_t total = prefix[c.batch] * uint32_t(rows);
+  const Shares shares(total, worker_count(p, total));
   const Span s = span_of<TOK>(p, lens[b]);
   const int warp = tid / 32, lane = tid % 32;
 
-  // where chunk's row lies in the line, and the warps that worked on it
-  auto locate = [&](int chunk, uint64_t &r0, int &w0, int &w1) {
-    r0 = uint64_t(prefix[b]) * uint64_t(rows) + uint64_t(h * p.chunks + chunk) * uint64_t(s.steps);
-    w0 = worker_of(r0, total, workers);
-    w1 = worker_of(r0 + uint64_t(s.steps) - 1, total, workers);
+  // the workers that worked on the row of chunk
+  auto locate = [&](int chunk, int &w0, int &w1) {
+    const uint32_t r0 = prefix[b] * uint32_t(rows) + uint32_t(h * p.chunks + chunk) * uint32_t(s.steps);
+    w0 = int(shares.of(r0));
+    w1 = int(shares.of(r0 + uint32_t(s.steps) - 1));
   };
-  // row `g` of worker w's partial result of the row: only the first worker may
-  // have begun the row (then it is its last one)
+  // row `g` of worker w's partial result of the row: the first worker began the
+  // row, the others were in it when their shares began
   auto part_of = [&](int w, bool begins, int g) {
     return (int64_t(w) * 2 + (begins ? 1 : 0)) * p.heads + g;
   };
@@ -843,9 +1206,8 @@ __global__ void __launch_bounds__(PA_JOIN_THREADS) join_kernel(const __grid_cons
     if (s.steps <= 0) {
       for (int d = tid; d < D; d += PA_JOIN_THREADS) out[d] = T(0.f);
     } else {
-      uint64_t r0;
       int w0, w1;
-      locate(chunk, r0, w0, w1);
+      locate(chunk, w0, w1);
       if (w0 != w1) {
         float M = -INFINITY, sum = 0.f;
         for (int w = w0 + tid; w <= w1; w += PA_JOIN_THREADS)
@@ -910,9 +1272,8 @@ __global__ void __launch_bounds__(PA_JOIN_THREADS) join_kernel(const __grid_cons
   if (t0 >= t1) return;
   for (int g = warp; g < p.group; g += WARPS) {
     const int chunk = g / PA_HEADS, gr = g % PA_HEADS;
-    uint64_t r0;
     int w0, w1;
-    locate(chunk, r0, w0, w1);
+    locate(chunk, w0, w1);
     float M, sum;
     if (w0 == w1) {
       const float2 ml = p.stats[(int64_t(b) * rows + h * p.chunks + chunk) * PA_HEADS + gr];
@@ -940,29 +1301,69 @@ __global__ void __launch_bounds__(PA_JOIN_THREADS) join_kernel(const __grid_cons
   __syncthreads();
   const int64_t at = (int64_t(b) * c.kv_heads + h) * p.a.slots;
   const float *sc = p.scores + (int64_t(b) * p.a.q_heads + h * p.group) * p.score_stride;
-  for (int t = t0 + tid; t < t1; t += PA_JOIN_THREADS) {
+  auto one = [&](int t) {
     float w = p.a.weights[at + t];
-    if (t >= s.lo) {
-#pragma unroll 4
+    if (t >= s.first * TOK)  // (masked slots in front of the window have scores of -infinity)
       for (int g = 0; g < p.group; ++g)
         w += exp2_approx(sc[int64_t(g) * p.score_stride + t] - head_m[g]) * head_inv[g];
-    }
     p.a.weights_out[at + t] = w;
+  };
+  int t = t0 + 4 * tid;
+  if (p.weights_quads) {
+    // four slots of four heads at a time
+    for (; t + 4 <= t1; t += 4 * PA_JOIN_THREADS) {
+      float4 w = *reinterpret_cast<const float4 *>(p.a.weights + at + t);
+      if (t >= s.first * TOK) {
+#pragma unroll 4
+        for (int g = 0; g < p.group; ++g) {
+          const float4 x = __ldcs(reinterpret_cast<const float4 *>(sc + int64_t(g) * p.score_stride + t));
+          const float m = head_m[g], inv = head_inv[g];
+          w.x += exp2_approx(x.x - m) * inv;
+          w.y += exp2_approx(x.y - m) * inv;
+          w.z += exp2_approx(x.z - m) * inv;
+          w.w += exp2_approx(x.w - m) * inv;
+        }
+      }
+      *reinterpret_cast<float4 *>(p.a.weights_out + at + t) = w;
+    }
+    // (the row's last one to three slots: t is theirs in one thread)
+    for (; t < t1; ++t) one(t);
+  } else {
+    for (t = t0 + tid; t < t1; t += PA_JOIN_THREADS) one(t);
   }
 }
 
 struct Config {
   const void *kernel;
-  int smem, ring, tok, ctas_per_sm;
+  int ring, tok, threads, ctas_per_sm;
 };
 
 template <typename T, int DP, bool HALF_ROWS>
-Config make_config() {
+Config mma_config() {
   Config c{};
   c.kernel = reinterpret_cast<const void *>(paged_attention_kernel<T, DP, HALF_ROWS>);
-  c.ring = PA_WARPS * Tile<T, DP>::RING + 1024;  // + alignment
+  c.ring = PA_BLOCK_WORKERS * MmaShape<T, DP>::RING + 1024;  // + alignment
   c.tok = Tile<T, DP>::TOK;
+  c.threads = MmaShape<T, DP>::THREADS;
   return c;
+}
+template <int DP, int G>
+Config simt_config() {
+  Config c{};
+  c.kernel = reinterpret_cast<const void *>(paged_attention_simt_kernel<DP, G>);
+  c.ring = PA_BLOCK_WORKERS * SimtShape<DP, G>::RING + 1024;
+  c.tok = 8;
+  c.threads = SimtShape<DP, G>::THREADS;
+  return c;
+}
+template <int DP>
+Config config_of(int dtype, int heads) {
+  if (dtype == WGX_FLOAT16) return heads <= 8 ? mma_config<__half, DP, true>() : mma_config<__half, DP, false>();
+  if (heads <= 1) return simt_config<DP, 1>();
+  if (heads <= 2) return simt_config<DP, 2>();
+  if (heads <= 4) return simt_config<DP, 4>();
+  if (heads <= 8) return simt_config<DP, 8>();
+  return mma_config<float, DP, false>();
 }
 
 constexpr int kPaMaxBatch = 2048;
@@ -970,43 +1371,29 @@ inline int prefix_bytes(int batch) { return (2 * batch + 1) * 4; }
 
 // The kernel for a call's type, head size and group; its attributes are set
 // and its occupancy read once per device.
-const Config &config_for(int dtype, int head_dim, bool half_rows) {
+const Config &config_for(int dtype, int head_dim, int heads) {
   static std::mutex mu;
-  static Config table[64][12];
-  static bool ready[64][12] = {};
+  static Config table[64][2][3][5];
+  static bool ready[64][2][3][5] = {};
   const int dev = current_device();
   if (dev >= 64) fail("paged_attention: device ordinal out of range");
-  const int dp = head_dim <= 64 ? 0 : head_dim <= 128 ? 1 : 2;
-  const int k = ((dtype == WGX_FLOAT16 ? 0 : 3) + dp) * 2 + (half_rows ? 1 : 0);
+  const int dt = dtype == WGX_FLOAT16, dp = head_dim <= 64 ? 0 : head_dim <= 128 ? 1 : 2;
+  const int hk = heads <= 1 ? 0 : heads <= 2 ? 1 : heads <= 4 ? 2 : heads <= 8 ? 3 : 4;
   std::lock_guard<std::mutex> lock(mu);
-  if (!ready[dev][k]) {
-    Config c{};
-    switch (k) {
-      case 0: c = make_config<__half, 64, false>(); break;
-      case 1: c = make_config<__half, 64, true>(); break;
-      case 2: c = make_config<__half, 128, false>(); break;
-      case 3: c = make_config<__half, 128, true>(); break;
-      case 4: c = make_config<__half, 256, false>(); break;
-      case 5: c = make_config<__half, 256, true>(); break;
-      case 6: c = make_config<float, 64, false>(); break;
-      case 7: c = make_config<float, 64, true>(); break;
-      case 8: c = make_config<float, 128, false>(); break;
-      case 9: c = make_config<float, 128, true>(); break;
-      case 10: c = make_config<float, 256, false>(); break;
-      default: c = make_config<float, 256, true>(); break;
-    }
-    const int most = c.ring + prefix_bytes(kPaMaxBatch);
+  if (!ready[dev][dt][dp][hk]) {
+    Config c = dp == 0 ? config_of<64>(dtype, heads)
+                       : dp == 1 ? config_of<128>(dtype, heads) : config_of<256>(dtype, heads);
     check_cuda(cudaFuncSetAttribute(c.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    std::min(most, 227 * 1024)),
+                                    c.ring + prefix_bytes(kPaMaxBatch)),
                "paged_attention smem attr");
-    check_cuda(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&c.ctas_per_sm, c.kernel, PA_WARPS * 32,
+    check_cuda(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&c.ctas_per_sm, c.kernel, c.threads,
                                                              c.ring + prefix_bytes(256)),
                "paged_attention occupancy");
     if (c.ctas_per_sm < 1) c.ctas_per_sm = 1;
-    table[dev][k] = c;
-    ready[dev][k] = true;
+    table[dev][dt][dp][hk] = c;
+    ready[dev][dt][dp][hk] = true;
   }
-  return table[dev][k];
+  return table[dev][dt][dp][hk];
 }
 
 uint64_t align256(uint64_t x) { return (x + 255) / 256 * 256; }
@@ -1032,7 +1419,7 @@ Layout layout_of(const wgx_paged_attention_args &a) {
   p.q_pairs = c.dtype == WGX_FLOAT16 && c.head_dim % 2 == 0 && a.q_batch_stride % 2 == 0 &&
               a.q_head_stride % 2 == 0 && (reinterpret_cast<uintptr_t>(a.q) & 3) == 0;
   p.scale2 = a.scale * 1.4426950408889634f;
-  l.cfg = &config_for(c.dtype, c.head_dim, p.heads <= 8);
+  l.cfg = &config_for(c.dtype, c.head_dim, p.heads);
   // TMA: a step's rows must lie in one page. Rows of whole 128-byte panels move
   // as one box per operand, others panel by panel with zeros behind the row.
   if (p.vec && c.page_size % l.cfg->tok == 0) {
@@ -1041,12 +1428,14 @@ Layout layout_of(const wgx_paged_attention_args &a) {
     p.tma = encode_rows_tmap(&p.k_map, c.k, c, c.k_page_stride, c.k_head_stride, c.k_slot_stride, panels, l.cfg->tok) &&
             encode_rows_tmap(&p.v_map, c.v, c, c.v_page_stride, c.v_head_stride, c.v_slot_stride, panels, l.cfg->tok);
   }
-  p.min_steps = 64 / l.cfg->tok;
+  if (getenv("PA_NOTMA")) p.tma = 0;
+  p.min_steps = getenv("PA_MIN") ? atoi(getenv("PA_MIN")) : 64 / l.cfg->tok;
   const uint64_t steps = uint64_t((p.capacity + l.cfg->tok - 1) / l.cfg->tok) * c.batch *
                          uint64_t(c.kv_heads) * p.chunks;
+  if (steps >= uint64_t(1) << 31) fail("paged_attention: too many slots");
   const uint64_t want = (steps + p.min_steps - 1) / p.min_steps;
   const int resident = device_sm_count() * l.cfg->ctas_per_sm;
-  p.max_workers = int(std::min<uint64_t>(std::max<uint64_t>(want, 1), uint64_t(resident) * PA_WARPS));
+  p.max_workers = int(std::min<uint64_t>(std::max<uint64_t>(want, 1), uint64_t(resident) * PA_BLOCK_WORKERS));
   l.grid = std::min(resident, p.max_workers);
   uint64_t off = 0;
   const uint64_t parts = uint64_t(p.max_workers) * 2 * p.heads;
@@ -1060,6 +1449,8 @@ Layout layout_of(const wgx_paged_attention_args &a) {
   if (a.weights_out) {
     p.stats = reinterpret_cast<float2 *>(take(uint64_t(c.batch) * c.kv_heads * p.chunks * PA_HEADS * 8));
     p.score_stride = (p.capacity + 15) / 16 * 16;
+    p.weights_quads = a.slots % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.weights) |
+                                            reinterpret_cast<uintptr_t>(a.weights_out)) & 15) == 0;
     p.scores = reinterpret_cast<float *>(take(uint64_t(c.batch) * a.q_heads * p.score_stride * 4));
   }
   l.bytes = off;
@@ -1079,7 +1470,7 @@ void launch_paged_attention(const wgx_paged_attention_args &a, cudaStream_t stre
   void *args[] = {&l.p};
   const int pre = prefix_bytes(c.batch);
   const int th = timer_begin("paged_attention_kernel", stream);
-  check_cuda(cudaLaunchKernel(l.cfg->kernel, dim3(unsigned(l.grid)), dim3(PA_WARPS * 32), args,
+  check_cuda(cudaLaunchKernel(l.cfg->kernel, dim3(unsigned(l.grid)), dim3(unsigned(l.cfg->threads)), args,
                               size_t(l.cfg->ring + pre), stream),
              "paged_attention launch");
   timer_end(th, stream);
@@ -1087,11 +1478,8 @@ void launch_paged_attention(const wgx_paged_attention_args &a, cudaStream_t stre
   if (a.weights_out)
     pieces = std::max<int>(pieces, int((l.p.capacity + PA_JOIN_SLOTS - 1) / PA_JOIN_SLOTS));
   const dim3 grid(unsigned(c.batch) * unsigned(c.kv_heads), unsigned(pieces));
-  if (c.dtype == WGX_FLOAT16)
-    join_kernel<__half, 16><<<grid, PA_JOIN_THREADS, size_t(pre), stream>>>(l.p);
-  else
-    join_kernel<float, 8><<<grid, PA_JOIN_THREADS, size_t(pre), stream>>>(l.p);
-  check_cuda(cudaGetLastError(), "paged_attention join launch");
+  launch_dependent(c.dtype == WGX_FLOAT16 ? join_kernel<__half, 16> : join_kernel<float, 8>, grid,
+                   PA_JOIN_THREADS, size_t(pre), stream, "paged_attention join launch", l.p);
 }
 
 }  // namespace wgx
