@@ -1405,7 +1405,7 @@ struct Layout {
   uint64_t bytes;
 };
 
-Layout layout_of(const wgx_paged_attention_args &a) {
+Layout layout_of(const wgx_paged_attention_args &a, bool for_launch) {
   Layout l{};
   AttnArgs &p = l.p;
   const wgx_kv_cache &c = a.cache;
@@ -1422,14 +1422,13 @@ Layout layout_of(const wgx_paged_attention_args &a) {
   l.cfg = &config_for(c.dtype, c.head_dim, p.heads);
   // TMA: a step's rows must lie in one page. Rows of whole 128-byte panels move
   // as one box per operand, others panel by panel with zeros behind the row.
-  if (p.vec && c.page_size % l.cfg->tok == 0) {
+  if (for_launch && p.vec && c.page_size % l.cfg->tok == 0) {
     const int panel = 128 / es, panels = c.head_dim % panel == 0 ? c.head_dim / panel : 1;
     p.boxes = panels * panel == c.head_dim ? 1 : (c.head_dim + panel - 1) / panel;
     p.tma = encode_rows_tmap(&p.k_map, c.k, c, c.k_page_stride, c.k_head_stride, c.k_slot_stride, panels, l.cfg->tok) &&
             encode_rows_tmap(&p.v_map, c.v, c, c.v_page_stride, c.v_head_stride, c.v_slot_stride, panels, l.cfg->tok);
   }
-  if (getenv("PA_NOTMA")) p.tma = 0;
-  p.min_steps = getenv("PA_MIN") ? atoi(getenv("PA_MIN")) : 64 / l.cfg->tok;
+  p.min_steps = 1;
   const uint64_t steps = uint64_t((p.capacity + l.cfg->tok - 1) / l.cfg->tok) * c.batch *
                          uint64_t(c.kv_heads) * p.chunks;
   if (steps >= uint64_t(1) << 31) fail("paged_attention: too many slots");
@@ -1459,10 +1458,10 @@ Layout layout_of(const wgx_paged_attention_args &a) {
 
 }  // namespace
 
-uint64_t paged_attention_scratch_bytes(const wgx_paged_attention_args &a) { return layout_of(a).bytes; }
+uint64_t paged_attention_scratch_bytes(const wgx_paged_attention_args &a) { return layout_of(a, false).bytes; }
 
 void launch_paged_attention(const wgx_paged_attention_args &a, cudaStream_t stream) {
-  Layout l = layout_of(a);
+  Layout l = layout_of(a, true);
   if (a.scratch_bytes < l.bytes || (reinterpret_cast<uintptr_t>(a.scratch) & 255))
     fail("paged_attention: scratch of " + std::to_string(l.bytes) + " bytes, 256-byte aligned, needed");
   l.p.err = device_error_word(current_device());

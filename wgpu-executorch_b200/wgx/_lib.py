@@ -105,13 +105,14 @@ SIGNATURES = {
                     c_uint64, c_void_p], c_int),
     "wgx_conv2d_noalloc": ([POINTER(ConvParams), c_void_p, c_void_p, c_void_p, c_void_p,
                             c_void_p], c_int),
-    # argument structs of the decoding operators: packed by wgx.decode
-    "wgx_kv_append": ([c_char_p, c_void_p], c_int),
-    "wgx_paged_attention_scratch_bytes": ([c_char_p, POINTER(c_uint64)], c_int),
-    "wgx_paged_attention": ([c_char_p, c_void_p], c_int),
-    "wgx_cache_evict": ([c_char_p, c_void_p], c_int),
-    "wgx_beam_search_scratch_bytes": ([c_char_p, POINTER(c_uint64)], c_int),
-    "wgx_beam_search_step": ([c_char_p, c_void_p], c_int),
+    # the decoding operators take their structs' addresses (wgx.decode calls
+    # them through its own binding, csrc/torch_binding.cpp)
+    "wgx_kv_append": ([c_void_p, c_void_p], c_int),
+    "wgx_paged_attention_scratch_bytes": ([c_void_p, POINTER(c_uint64)], c_int),
+    "wgx_paged_attention": ([c_void_p, c_void_p], c_int),
+    "wgx_cache_evict": ([c_void_p, c_void_p], c_int),
+    "wgx_beam_search_scratch_bytes": ([c_void_p, POINTER(c_uint64)], c_int),
+    "wgx_beam_search_step": ([c_void_p, c_void_p], c_int),
     "wgx_device_error": ([c_int, POINTER(c_uint32), c_int], c_int),
     "wgx_debug_inject": ([c_uint32], c_int),
     "wgx_build_flags": ([POINTER(c_uint32)], c_int),
