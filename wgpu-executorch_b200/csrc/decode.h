@@ -47,6 +47,13 @@ inline int current_device() {
 }
 
 #ifdef __CUDACC__
+// Programmatic dependent launch: the next kernel's blocks may be set up while
+// this one's work ends (every block of this kernel has started); wait returns
+// when all of the prior kernel's work is done and visible.
+__device__ __forceinline__ void let_dependents_launch() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void wait_for_prior_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // Launches a kernel that may be set up while the stream's previous kernel ends
 // (it calls griddepcontrol.wait before it touches what that one writes).
 template <typename... P, typename... A>

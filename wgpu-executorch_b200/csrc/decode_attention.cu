@@ -38,7 +38,7 @@ namespace {
 constexpr int PA_HEADS = 16;        // rows of an mma tile
 constexpr int PA_MAX_GROUP = 128;   // query heads per K/V head
 constexpr int PA_JOIN_THREADS = 256;
-constexpr int PA_JOIN_SLOTS = 2048;  // slots per join block of the accumulation
+constexpr int PA_JOIN_SLOTS = 4096;  // slots per join block of the accumulation
 
 struct AttnArgs {
   CUtensorMap k_map, v_map;  // where tma: [page][head][slot][channel] in boxes of TOK rows
@@ -53,13 +53,17 @@ struct AttnArgs {
   int boxes;          // TMA copies per operand and step
   int q_pairs;        // queries can be read two elements at a time
   float scale2;       // scale * log2(e): the softmax runs in base 2
-  float *part_o;      // [worker][2][heads][head_dim]
+  float *part_o;      // [worker][2][heads][part_stride]
+  int part_stride;    // head_dim rounded up to 4
   float2 *part_ml;    // [worker][2][heads] (max, sum)
   float2 *stats;      // [row][heads]: of rows finished by one warp (accumulation only)
   float *scores;      // [batch][q_heads][score_stride] (accumulation only)
   int64_t score_stride;
   int weights_quads;  // weights move four slots at a time
   int heads;          // min(group, PA_HEADS): rows a partial result has
+  uint32_t *prefix;   // [batch + 1] steps of a row before each sequence (for the join)
+  int o_blocks;       // of the join: blocks for the result
+  int join_warps;     // of the join: warps per query head
   uint32_t *err;
 };
 
@@ -83,8 +87,9 @@ __device__ __forceinline__ Span span_of(const AttnArgs &p, int len) {
 }
 
 // prefix[0 .. batch] and lens[0 .. batch - 1] into shared memory.
+// Where `leave`, block 0 also leaves the prefix in scratch.
 template <int TOK>
-__device__ void build_prefix(const AttnArgs &p, uint32_t *prefix, int *lens) {
+__device__ void build_prefix(const AttnArgs &p, uint32_t *prefix, int *lens, bool leave) {
   const int B = p.a.cache.batch, tid = threadIdx.x, nt = blockDim.x;
   __shared__ uint32_t warp_sum[32];
   uint32_t base = 0;
@@ -109,11 +114,17 @@ __device__ void build_prefix(const AttnArgs &p, uint32_t *prefix, int *lens) {
       if (w < (tid >> 5)) before += warp_sum[w];
       all += warp_sum[w];
     }
-    if (b < B) prefix[b] = before + x - n;
+    if (b < B) {
+      prefix[b] = before + x - n;
+      if (leave && blockIdx.x == 0) p.prefix[b] = before + x - n;
+    }
     base = all;
     __syncthreads();
   }
-  if (tid == 0) prefix[B] = base;
+  if (tid == 0) {
+    prefix[B] = base;
+    if (leave && blockIdx.x == 0) p.prefix[B] = base;
+  }
   __syncthreads();
 }
 
@@ -142,12 +153,6 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool l
                "r"(live ? 16 : 0)
                : "memory");
 }
-// Programmatic dependent launch: the join's blocks may be set up while the
-// attention's work ends; wait() returns when all of it is done and visible.
-__device__ __forceinline__ void let_dependents_launch() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
-__device__ __forceinline__ void wait_for_prior_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -524,7 +529,7 @@ __global__ void __launch_bounds__(MmaShape<T, DP>::THREADS)
       *reinterpret_cast<uint4 *>(sm.ring + i) = make_uint4(0u, 0u, 0u, 0u);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  build_prefix<TOK>(p, sm.prefix, sm.lens);  // (ends with a block barrier)
+  build_prefix<TOK>(p, sm.prefix, sm.lens, p.scores != nullptr);  // (ends with a block barrier)
   const int rows = c.kv_heads * p.chunks;
   const uint32_t total = sm.prefix[c.batch] * uint32_t(rows);
   const uint32_t workers = worker_count(p, total);
@@ -861,7 +866,7 @@ __global__ void __launch_bounds__(MmaShape<T, DP>::THREADS)
           p.stats[(int64_t(cur.b) * rows + cur.row) * PA_HEADS + g] = make_float2(m[x], sum);
       } else {
         const int64_t at = (int64_t(me) * 2 + (from_begin ? 1 : 0)) * p.heads + g;
-        float *po = p.part_o + at * D;
+        float *po = p.part_o + at * p.part_stride;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -928,7 +933,7 @@ __global__ void __launch_bounds__(SimtShape<DP, G>::THREADS)
       *reinterpret_cast<uint4 *>(sm.ring + i) = make_uint4(0u, 0u, 0u, 0u);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  build_prefix<TOK>(p, sm.prefix, sm.lens);  // (ends with a block barrier)
+  build_prefix<TOK>(p, sm.prefix, sm.lens, p.scores != nullptr);  // (ends with a block barrier)
   const int rows = c.kv_heads;  // (p.chunks is 1)
   const uint32_t total = sm.prefix[c.batch] * uint32_t(rows);
   const uint32_t workers = worker_count(p, total);
@@ -1118,7 +1123,7 @@ __global__ void __launch_bounds__(SimtShape<DP, G>::THREADS)
       const float inv = !whole ? 1.f : sum > 0.f || sum != sum ? 1.f / sum : 0.f;
       float *to = whole ? static_cast<float *>(p.a.out) + int64_t(cur.b) * p.a.out_batch_stride +
                               int64_t(h * nh + g) * p.a.out_head_stride
-                        : p.part_o + at * D;
+                        : p.part_o + at * p.part_stride;
       if (half == 0) {
 #pragma unroll
         for (int k = 0; k < OV; ++k) {
@@ -1139,167 +1144,167 @@ __global__ void __launch_bounds__(SimtShape<DP, G>::THREADS)
   if (!ok) drain<STAGES>(loader.live_ring, bars, stage, phase);
 }
 
-// Block reductions of the join: all threads get the result.
-__device__ __forceinline__ float join_max(float x, float *red) {
+__device__ __forceinline__ float warp_max(float x) {
 #pragma unroll
   for (int d = 16; d; d /= 2) x = fmaxf(x, __shfl_xor_sync(~0u, x, d));
-  __syncthreads();
-  if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = x;
-  __syncthreads();
-  x = red[0];
-#pragma unroll
-  for (int w = 1; w < PA_JOIN_THREADS / 32; ++w) x = fmaxf(x, red[w]);
   return x;
 }
-__device__ __forceinline__ float join_sum(float x, float *red) {
+__device__ __forceinline__ float warp_sum(float x) {
 #pragma unroll
   for (int d = 16; d; d /= 2) x += __shfl_xor_sync(~0u, x, d);
-  __syncthreads();
-  if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = x;
-  __syncthreads();
-  x = 0.f;
-#pragma unroll
-  for (int w = 0; w < PA_JOIN_THREADS / 32; ++w) x += red[w];
   return x;
 }
 
-// Rows cut between warps: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i.
-// Block (b * kv_heads + h, y): y < group joins that query head; with
-// accumulation every y also adds the probabilities of its slots. The partial
-// results (up to one per warp of the grid for a lone long row) are spread over
-// the block's warps, whose lanes take neighbouring channels.
-template <typename T, int TOK>
+// Rows cut between workers: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i.
+// Blocks below o_blocks join query heads, join_warps warps each (one where a
+// row has few partial results, the whole block for a lone long row that most
+// of the grid worked on); the others add the probabilities of PA_JOIN_SLOTS
+// slots of a K/V head to its weights. Where the rows lie in the line of work
+// was left in scratch by the attention.
+// KQ: groups of 128 channels.
+template <typename T, int TOK, int KQ>
 __global__ void __launch_bounds__(PA_JOIN_THREADS) join_kernel(const __grid_constant__ AttnArgs p) {
+  constexpr int WARPS = PA_JOIN_THREADS / 32, FLIGHT = 8;
   extern __shared__ __align__(16) uint8_t jn_smem[];
-  constexpr int WARPS = PA_JOIN_THREADS / 32;
   __shared__ float head_m[PA_MAX_GROUP], head_inv[PA_MAX_GROUP];
-  __shared__ float red[WARPS], factor[PA_JOIN_THREADS];
-  __shared__ __align__(16) float sums[WARPS][256];
+  __shared__ __align__(16) float sums[WARPS][128 * KQ];
   const wgx_kv_cache &c = p.a.cache;
-  uint32_t *prefix = reinterpret_cast<uint32_t *>(jn_smem);
-  int *lens = reinterpret_cast<int *>(prefix + c.batch + 1);
-  build_prefix<TOK>(p, prefix, lens);  // (of the call's inputs)
-  wait_for_prior_kernel();
-  const int b = blockIdx.x / c.kv_heads, h = blockIdx.x % c.kv_heads, y = blockIdx.y;
-  const int rows = c.kv_heads * p.chunks, D = c.head_dim, tid = threadIdx.x;
-  const uint32_t total = prefix[c.batch] * uint32_t(rows);
-  const Shares shares(total, worker_count(p, total));
-  const Span s = span_of<TOK>(p, lens[b]);
-  const int warp = tid / 32, lane = tid % 32;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int rows = c.kv_heads * p.chunks, D = c.head_dim;
 
-  // the workers that worked on the row of chunk
-  auto locate = [&](int chunk, int &w0, int &w1) {
+  // the workers that worked on row (h, chunk) of b
+  auto locate = [&](const uint32_t *prefix, int b, int h, int chunk, const Span &s, int &w0, int &w1) {
+    const uint32_t total = prefix[c.batch] * uint32_t(rows);
+    const Shares shares(total, worker_count(p, total));
     const uint32_t r0 = prefix[b] * uint32_t(rows) + uint32_t(h * p.chunks + chunk) * uint32_t(s.steps);
     w0 = int(shares.of(r0));
     w1 = int(shares.of(r0 + uint32_t(s.steps) - 1));
   };
-  // row `g` of worker w's partial result of the row: the first worker began the
-  // row, the others were in it when their shares began
-  auto part_of = [&](int w, bool begins, int g) {
-    return (int64_t(w) * 2 + (begins ? 1 : 0)) * p.heads + g;
+  // row `g` of worker w0 + i's partial result of a row: the first worker began
+  // the row, the others were in it when their shares began
+  auto part_of = [&](int w0, int i, int g) { return (int64_t(w0 + i) * 2 + (i == 0 ? 1 : 0)) * p.heads + g; };
+  // (maximum, sum) of head g's n partial results; all lanes get them
+  auto stats_of = [&](int w0, int n, int g) {
+    float M = -INFINITY, sum = 0.f;
+    for (int i = lane; i < n; i += 32) M = fmaxf(M, p.part_ml[part_of(w0, i, g)].x);
+    M = warp_max(M);
+    const float mu = M == -INFINITY ? 0.f : M;
+    for (int i = lane; i < n; i += 32) {
+      const float2 ml = p.part_ml[part_of(w0, i, g)];
+      sum += ml.y * exp2_approx(ml.x - mu);
+    }
+    return make_float2(mu, warp_sum(sum));
   };
 
-  if (y < p.group) {
-    const int chunk = y / PA_HEADS, g = y % PA_HEADS;
-    T *out = static_cast<T *>(p.a.out) + int64_t(b) * p.a.out_batch_stride +
-             int64_t(h * p.group + y) * p.a.out_head_stride;
-    if (s.steps <= 0) {
-      for (int d = tid; d < D; d += PA_JOIN_THREADS) out[d] = T(0.f);
-    } else {
-      int w0, w1;
-      locate(chunk, w0, w1);
-      if (w0 != w1) {
-        float M = -INFINITY, sum = 0.f;
-        for (int w = w0 + tid; w <= w1; w += PA_JOIN_THREADS)
-          M = fmaxf(M, p.part_ml[part_of(w, w == w0, g)].x);
-        M = join_max(M, red);
-        const float mu = M == -INFINITY ? 0.f : M;
-        float4 acc[2] = {};
-        const int quads = (D + 3) / 4;
-        for (int base = w0; base <= w1; base += PA_JOIN_THREADS) {
-          __syncthreads();
-          float f = 0.f;
-          if (base + tid <= w1) {
-            const float2 ml = p.part_ml[part_of(base + tid, base + tid == w0, g)];
-            f = exp2_approx(ml.x - mu);
-            sum += f * ml.y;
-          }
-          factor[tid] = f;
-          __syncthreads();
-          const int n = min(PA_JOIN_THREADS, w1 - base + 1);
-#pragma unroll 4
-          for (int i = warp; i < n; i += WARPS) {
-            const float fi = factor[i];
-            const float *po = p.part_o + part_of(base + i, base + i == w0, g) * D;
+  if (int(blockIdx.x) < p.o_blocks) {
+    // (all of this from the call's inputs, while the attention ends)
+    uint32_t *prefix = reinterpret_cast<uint32_t *>(jn_smem);
+    int *lens = reinterpret_cast<int *>(prefix + c.batch + 1);
+    build_prefix<TOK>(p, prefix, lens, false);
+    const int per = p.join_warps, sub = warp % per;
+    const int unit = blockIdx.x * (WARPS / per) + warp / per;
+    const bool real = unit < c.batch * p.a.q_heads;
+    const int b = real ? unit / p.a.q_heads : 0, i = unit - b * p.a.q_heads;
+    const int h = i / p.group, gi = i - h * p.group, chunk = gi / PA_HEADS, g = gi % PA_HEADS;
+    const Span s = span_of<TOK>(p, lens[b]);
+    T *out = static_cast<T *>(p.a.out) + int64_t(b) * p.a.out_batch_stride + int64_t(i) * p.a.out_head_stride;
+    int w0 = 0, w1 = 0;
+    if (real && s.steps > 0) locate(prefix, b, h, chunk, s, w0, w1);
+    const bool split = w0 != w1;
+    float4 acc[KQ] = {};
+    float inv = 0.f;
+    const int quads = (D + 3) / 4;
+    int at_quad[KQ];  // (lanes behind the row's end repeat its last four channels)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const int q = lane + 32 * k;
-              if (q >= quads) break;
-              float4 v;
-              if (D % 4 == 0) {
-                v = *reinterpret_cast<const float4 *>(po + 4 * q);
-              } else {
-                v.x = po[4 * q];
-                v.y = 4 * q + 1 < D ? po[4 * q + 1] : 0.f;
-                v.z = 4 * q + 2 < D ? po[4 * q + 2] : 0.f;
-                v.w = 4 * q + 3 < D ? po[4 * q + 3] : 0.f;
+    for (int k = 0; k < KQ; ++k) at_quad[k] = min(lane + 32 * k, quads - 1);
+    wait_for_prior_kernel();
+    if (split) {
+      const int n = w1 - w0 + 1;
+      const float2 st = stats_of(w0, n, g);
+      inv = st.y > 0.f || st.y != st.y ? 1.f / st.y : 0.f;
+      for (int base = sub; base < n; base += 32 * per) {
+        const int mine = base + lane * per;
+        const float f = mine < n ? exp2_approx(p.part_ml[part_of(w0, mine, g)].x - st.x) : 0.f;
+        const int cnt = min(32, (n - base + per - 1) / per);
+        for (int j0 = 0; j0 < cnt; j0 += FLIGHT) {
+          float4 v[FLIGHT][KQ];
+#pragma unroll
+          for (int j = 0; j < FLIGHT; ++j) {
+            const float4 *po = reinterpret_cast<const float4 *>(
+                p.part_o + part_of(w0, base + min(j0 + j, cnt - 1) * per, g) * p.part_stride);
+#pragma unroll
+            for (int k = 0; k < KQ; ++k) v[j][k] = po[at_quad[k]];
+          }
+#pragma unroll
+          for (int j = 0; j < FLIGHT; ++j) {
+            const float fj = __shfl_sync(~0u, f, j0 + j);  // (zero behind the last)
+            if (j0 + j < cnt) {
+#pragma unroll
+              for (int k = 0; k < KQ; ++k) {
+                acc[k].x += fj * v[j][k].x;
+                acc[k].y += fj * v[j][k].y;
+                acc[k].z += fj * v[j][k].z;
+                acc[k].w += fj * v[j][k].w;
               }
-              acc[k].x += fi * v.x;
-              acc[k].y += fi * v.y;
-              acc[k].z += fi * v.z;
-              acc[k].w += fi * v.w;
             }
           }
         }
-        sum = join_sum(sum, red);
-        const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-          if (lane + 32 * k < quads) *reinterpret_cast<float4 *>(&sums[warp][4 * (lane + 32 * k)]) = acc[k];
-        __syncthreads();
-        for (int d = tid; d < D; d += PA_JOIN_THREADS) {
-          float v = 0.f;
-#pragma unroll
-          for (int w = 0; w < WARPS; ++w) v += sums[w][d];
-          out[d] = T(v * inv);
-        }
       }
     }
+    if (per > 1) {
+#pragma unroll
+      for (int k = 0; k < KQ; ++k)
+        if (lane + 32 * k < quads) *reinterpret_cast<float4 *>(&sums[warp][4 * (lane + 32 * k)]) = acc[k];
+      __syncthreads();
+      if (sub) return;
+      for (int w = 1; w < per; ++w)
+#pragma unroll
+        for (int k = 0; k < KQ; ++k)
+          if (lane + 32 * k < quads) {
+            const float4 v = *reinterpret_cast<const float4 *>(&sums[warp + w][4 * (lane + 32 * k)]);
+            acc[k].x += v.x;
+            acc[k].y += v.y;
+            acc[k].z += v.z;
+            acc[k].w += v.w;
+          }
+    }
+    if (!real || (s.steps > 0 && !split)) return;
+#pragma unroll
+    for (int k = 0; k < KQ; ++k) {
+      const int d = 4 * (lane + 32 * k);
+      if (d < D) out[d] = T(acc[k].x * inv);
+      if (d + 1 < D) out[d + 1] = T(acc[k].y * inv);
+      if (d + 2 < D) out[d + 2] = T(acc[k].z * inv);
+      if (d + 3 < D) out[d + 3] = T(acc[k].w * inv);
+    }
+    return;
   }
-  if (!p.a.weights_out) return;
-  const int t0 = y * PA_JOIN_SLOTS;
+
+  const int at_row = (int(blockIdx.x) - p.o_blocks) % (c.batch * c.kv_heads);
+  const int t0 = (int(blockIdx.x) - p.o_blocks) / (c.batch * c.kv_heads) * PA_JOIN_SLOTS;
+  const int b = at_row / c.kv_heads, h = at_row % c.kv_heads;
+  const Span s = span_of<TOK>(p, slots_in_use(p.a.lengths, b, p.capacity, p.err));
   const int t1 = min(t0 + PA_JOIN_SLOTS, int(min(int64_t(s.len), p.a.slots)));
   if (t0 >= t1) return;
+  wait_for_prior_kernel();
   for (int g = warp; g < p.group; g += WARPS) {
     const int chunk = g / PA_HEADS, gr = g % PA_HEADS;
     int w0, w1;
-    locate(chunk, w0, w1);
-    float M, sum;
+    locate(p.prefix, b, h, chunk, s, w0, w1);
+    float2 st;
     if (w0 == w1) {
-      const float2 ml = p.stats[(int64_t(b) * rows + h * p.chunks + chunk) * PA_HEADS + gr];
-      M = ml.x;
-      sum = ml.y;
+      st = p.stats[(int64_t(b) * rows + h * p.chunks + chunk) * PA_HEADS + gr];
+      if (st.x == -INFINITY) st.x = 0.f;
     } else {
-      M = -INFINITY;
-      for (int w = w0 + lane; w <= w1; w += 32) M = fmaxf(M, p.part_ml[part_of(w, w == w0, gr)].x);
-#pragma unroll
-      for (int d = 16; d; d /= 2) M = fmaxf(M, __shfl_xor_sync(~0u, M, d));
-      const float mu = M == -INFINITY ? 0.f : M;
-      sum = 0.f;
-      for (int w = w0 + lane; w <= w1; w += 32) {
-        const float2 ml = p.part_ml[part_of(w, w == w0, gr)];
-        sum += ml.y * exp2_approx(ml.x - mu);
-      }
-#pragma unroll
-      for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(~0u, sum, d);
+      st = stats_of(w0, w1 - w0 + 1, gr);
     }
     if (lane == 0) {
-      head_m[g] = M == -INFINITY ? 0.f : M;
-      head_inv[g] = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+      head_m[g] = st.x;
+      head_inv[g] = st.y > 0.f || st.y != st.y ? 1.f / st.y : 0.f;
     }
   }
   __syncthreads();
-  const int64_t at = (int64_t(b) * c.kv_heads + h) * p.a.slots;
+  const int64_t at = int64_t(at_row) * p.a.slots;
   const float *sc = p.scores + (int64_t(b) * p.a.q_heads + h * p.group) * p.score_stride;
   auto one = [&](int t) {
     float w = p.a.weights[at + t];
@@ -1443,8 +1448,16 @@ Layout layout_of(const wgx_paged_attention_args &a, bool for_launch) {
     off += align256(bytes);
     return static_cast<uint8_t *>(a.scratch) + at;
   };
-  p.part_o = reinterpret_cast<float *>(take(parts * c.head_dim * 4));
+  p.part_stride = (c.head_dim + 3) / 4 * 4;
+  p.part_o = reinterpret_cast<float *>(take(parts * p.part_stride * 4));
   p.part_ml = reinterpret_cast<float2 *>(take(parts * 8));
+  p.prefix = reinterpret_cast<uint32_t *>(take((uint64_t(c.batch) + 1) * 4));
+  // warps per head of the join, by the partial results a row can have when the
+  // rows are alike
+  const int64_t expect = p.max_workers / (int64_t(c.batch) * c.kv_heads * p.chunks);
+  p.join_warps = expect > 64 ? 8 : expect > 32 ? 4 : expect > 16 ? 2 : 1;
+  const int per_block = PA_JOIN_THREADS / 32 / p.join_warps;
+  p.o_blocks = int((int64_t(c.batch) * a.q_heads + per_block - 1) / per_block);
   if (a.weights_out) {
     p.stats = reinterpret_cast<float2 *>(take(uint64_t(c.batch) * c.kv_heads * p.chunks * PA_HEADS * 8));
     p.score_stride = (p.capacity + 15) / 16 * 16;
@@ -1473,12 +1486,13 @@ void launch_paged_attention(const wgx_paged_attention_args &a, cudaStream_t stre
                               size_t(l.cfg->ring + pre), stream),
              "paged_attention launch");
   timer_end(th, stream);
-  int pieces = l.p.group;
+  int64_t blocks = l.p.o_blocks;
   if (a.weights_out)
-    pieces = std::max<int>(pieces, int((l.p.capacity + PA_JOIN_SLOTS - 1) / PA_JOIN_SLOTS));
-  const dim3 grid(unsigned(c.batch) * unsigned(c.kv_heads), unsigned(pieces));
-  launch_dependent(c.dtype == WGX_FLOAT16 ? join_kernel<__half, 16> : join_kernel<float, 8>, grid,
-                   PA_JOIN_THREADS, size_t(pre), stream, "paged_attention join launch", l.p);
+    blocks += int64_t(c.batch) * c.kv_heads * ((l.p.capacity + PA_JOIN_SLOTS - 1) / PA_JOIN_SLOTS);
+  const bool wide = c.head_dim > 128, half = c.dtype == WGX_FLOAT16;
+  launch_dependent(half ? (wide ? join_kernel<__half, 16, 2> : join_kernel<__half, 16, 1>)
+                        : (wide ? join_kernel<float, 8, 2> : join_kernel<float, 8, 1>),
+                   dim3(unsigned(blocks)), PA_JOIN_THREADS, size_t(pre), stream, "paged_attention join launch", l.p);
 }
 
 }  // namespace wgx

@@ -30,6 +30,7 @@ constexpr int BM_LIST = 1024;                   // logits of a segment ranked by
 constexpr int BM_CAND = 1024;                   // proposals ranked by counting
 constexpr int BM_BLOCKS_PER_SM = 4;             // of scan_kernel: 40 KB of shared memory each
 constexpr int BM_SEL_THREADS = 256;
+constexpr int BM_HELD = 4;                      // entries a thread of select_kernel holds
 constexpr int BM_COPY_THREADS = 256;
 constexpr int BM_UNITS = 4;  // units of K and of V a thread has in flight
 
@@ -106,6 +107,7 @@ __global__ void __launch_bounds__(BM_THREADS, BM_BLOCKS_PER_SM) scan_kernel(cons
   __shared__ uint64_t bound, best[BM_WARPS];
   __shared__ uint64_t list[BM_LIST];
   __shared__ uint32_t n_list;
+  let_dependents_launch();
   const wgx_beam_search_args &a = p.a;
   const int row = blockIdx.y, seg = blockIdx.x, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   if (a.finished[row]) return;  // proposes eos: its logits are not needed
@@ -297,16 +299,29 @@ __global__ void __launch_bounds__(BM_SEL_THREADS) select_kernel(const __grid_con
   __shared__ uint32_t n_cand;
   const int b = blockIdx.x, W = a.beams, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int list = p.segments * W, all = W * list;
+  let_dependents_launch();
+  wait_for_prior_kernel();
   if (tid == 0) n_cand = 0;
+  // entry i % list of beam i / list, i = tid + j * threads: the first BM_HELD of
+  // a thread are loaded now, beside the segments' sums
+  float held_x[BM_HELD];
+  int held_t[BM_HELD];
+  const int64_t first = int64_t(b) * all;
+#pragma unroll
+  for (int j = 0; j < BM_HELD; ++j) {
+    const int i = tid + j * BM_SEL_THREADS;
+    held_t[j] = i < all ? p.top_t[first + i] : -1;
+    held_x[j] = i < all ? p.top_x[first + i] : 0.f;
+  }
   for (int w = warp; w < W; w += BM_SEL_THREADS / 32) {
     const int row = b * W + w;
     const bool done = a.finished[row] != 0;
     const float score = a.scores[row];
-    float m = -INFINITY, s = 0.f;
+    const float2 *ms = p.seg_ms + int64_t(row) * p.segments;
+    // (a finished beam's sums were not written: they are read, not used)
+    const float2 mine = lane < p.segments ? ms[lane] : make_float2(-INFINITY, 0.f);
+    float m = mine.x, s = 0.f;
     if (!done) {
-      const float2 *ms = p.seg_ms + int64_t(row) * p.segments;
-      const float2 mine = lane < p.segments ? ms[lane] : make_float2(-INFINITY, 0.f);
-      m = mine.x;
       for (int c = lane + 32; c < p.segments; c += 32) m = fmaxf(m, ms[c].x);
       m = warp_max(m);
       const float mu = m == -INFINITY ? 0.f : m;
@@ -322,44 +337,54 @@ __global__ void __launch_bounds__(BM_SEL_THREADS) select_kernel(const __grid_con
     }
   }
   __syncthreads();
-  // candidate i: entry i % list of beam i / list; false: none
-  auto get = [&](int i, Proposal &q) {
-    const int w = i / list, e = i - w * list;
+  // proposal of entry i; false: none
+  auto propose = [&](int i, float x, int t, Proposal &q) {
+    const int w = i / list;
     q.beam = w;
     if (row_done[w]) {
       q.token = a.eos;
       q.logit = 0.f;
       q.total = row_score[w];
-      if (e) return false;
+      if (i != w * list) return false;
     } else {
-      const int64_t at = int64_t(b * W + w) * list + e;
-      q.token = p.top_t[at];
-      if (q.token < 0) return false;
-      q.logit = p.top_x[at];
-      q.total = row_score[w] + ((q.logit - row_max[w]) - row_log[w]);
+      q.token = t;
+      if (t < 0) return false;
+      q.logit = x;
+      q.total = row_score[w] + ((x - row_max[w]) - row_log[w]);
     }
     if (q.total != q.total) q.total = -INFINITY;
     return true;
   };
+  // f(entry's place in its list, proposal) for this thread's proposals
+  auto each = [&](auto &&f) {
+#pragma unroll
+    for (int j = 0; j < BM_HELD; ++j) {
+      const int i = tid + j * BM_SEL_THREADS;
+      Proposal q;
+      if (i < all && propose(i, held_x[j], held_t[j], q)) f(i % W, q);
+    }
+    for (int i = tid + BM_HELD * BM_SEL_THREADS; i < all; i += BM_SEL_THREADS) {
+      Proposal q;
+      if (propose(i, p.top_x[first + i], p.top_t[first + i], q)) f(i % W, q);
+    }
+  };
   // ---- threshold: at least W proposals are not below the W-th entry of any
   // one segment's list
   float tau = -INFINITY;
-  for (int i = W - 1 + tid * W; i < all; i += BM_SEL_THREADS * W) {
-    Proposal q;
-    if (get(i, q)) tau = fmaxf(tau, q.total);
-  }
+  each([&](int place, const Proposal &q) {
+    if (place == W - 1 && !row_done[q.beam]) tau = fmaxf(tau, q.total);
+  });
   tau = warp_max(tau);
   if (lane == 0) red[warp] = tau;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < BM_SEL_THREADS / 32; ++w) tau = fmaxf(tau, red[w]);
-  for (int i = tid; i < all; i += BM_SEL_THREADS) {
-    Proposal q;
-    if (get(i, q) && q.total >= tau) {
+  each([&](int, const Proposal &q) {
+    if (q.total >= tau) {
       const uint32_t at = atomicAdd(&n_cand, 1u);
       if (at < BM_CAND) cand[at] = q;
     }
-  }
+  });
   __syncthreads();
   auto emit = [&](int r, const Proposal &q) {
     const int64_t at = int64_t(b) * W + r;
@@ -382,10 +407,9 @@ __global__ void __launch_bounds__(BM_SEL_THREADS) select_kernel(const __grid_con
     Proposal last{INFINITY, 0.f, -1, -1};
     for (int r = 0; r < W; ++r) {
       Proposal k{-INFINITY, -INFINITY, 0x7fffffff, 0x7fffffff};
-      for (int i = tid; i < all; i += BM_SEL_THREADS) {
-        Proposal q;
-        if (get(i, q) && (r == 0 || before(last, q)) && before(q, k)) k = q;
-      }
+      each([&](int, const Proposal &q) {
+        if ((r == 0 || before(last, q)) && before(q, k)) k = q;
+      });
 #pragma unroll
       for (int d = 16; d; d /= 2) {
         Proposal y;
@@ -416,8 +440,9 @@ __global__ void __launch_bounds__(BM_COPY_THREADS) reorder_kernel(const __grid_c
   const wgx_beam_search_args &a = p.a;
   const wgx_kv_cache &c = a.cache;
   const int child = blockIdx.y, tid = threadIdx.x;
-  const int from = child / a.beams * a.beams + a.parents[child];
   const int spare = a.spare[child];
+  wait_for_prior_kernel();
+  const int from = child / a.beams * a.beams + a.parents[child];
   const int len = slots_in_use(a.lengths, from, p.capacity, p.err);
   const int full = len / c.page_size, tail = len - full * c.page_size;
   const int32_t *src_table = c.page_table + int64_t(from) * c.table_stride;
@@ -525,8 +550,8 @@ void launch_beam_search_step(const wgx_beam_search_args &a, cudaStream_t stream)
   }
   check_cuda(cudaGetLastError(), "beam_search_step launch");
   timer_end(th, stream);
-  select_kernel<<<unsigned(a.batch), BM_SEL_THREADS, 0, stream>>>(p);
-  check_cuda(cudaGetLastError(), "beam_search_step selection launch");
+  launch_dependent(select_kernel, dim3(unsigned(a.batch)), BM_SEL_THREADS, 0, stream,
+                   "beam_search_step selection launch", p);
   if (!c.k) return;
   const int es = dtype_size(c.dtype);
   const uint64_t units = uint64_t(c.layers) * c.kv_heads * c.page_size *
@@ -535,15 +560,9 @@ void launch_beam_search_step(const wgx_beam_search_args &a, cudaStream_t stream)
   const uint64_t want = (units + BM_COPY_THREADS * BM_UNITS - 1) / (BM_COPY_THREADS * BM_UNITS);
   const uint64_t most = std::max<uint64_t>(1, uint64_t(device_sm_count()) * 16 / rows);
   const dim3 cgrid(unsigned(std::min(want, most)), rows);
-  if (p.vec && es == 2)
-    reorder_kernel<uint4, 8><<<cgrid, BM_COPY_THREADS, 0, stream>>>(p);
-  else if (p.vec)
-    reorder_kernel<uint4, 4><<<cgrid, BM_COPY_THREADS, 0, stream>>>(p);
-  else if (es == 2)
-    reorder_kernel<uint16_t, 1><<<cgrid, BM_COPY_THREADS, 0, stream>>>(p);
-  else
-    reorder_kernel<uint32_t, 1><<<cgrid, BM_COPY_THREADS, 0, stream>>>(p);
-  check_cuda(cudaGetLastError(), "beam_search_step reorder launch");
+  launch_dependent(p.vec ? (es == 2 ? reorder_kernel<uint4, 8> : reorder_kernel<uint4, 4>)
+                         : (es == 2 ? reorder_kernel<uint16_t, 1> : reorder_kernel<uint32_t, 1>),
+                   cgrid, BM_COPY_THREADS, 0, stream, "beam_search_step reorder launch", p);
 }
 
 }  // namespace wgx

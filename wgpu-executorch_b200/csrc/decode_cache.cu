@@ -106,7 +106,7 @@ __global__ void advance_kernel(const __grid_constant__ AppendArgs p) {
 // numbers (weight key << 32 | complement of the slot), all distinct; the
 // budget-th largest is found by radix selection, 11 bits a pass (histograms in
 // shared memory, summed over the cluster through distributed shared memory),
-// until the class it lies in is wholly taken or small enough (256) to be
+// until the class it lies in is wholly taken or small enough (128) to be
 // ranked by counting: one or two passes unless weights tie. Keys are held in
 // shared memory, weights and positions are read once. Survivors behind the
 // budget then move into the holes before it, both listed in slot order.
@@ -114,7 +114,7 @@ constexpr int EV_THREADS = 512;
 constexpr int EV_MAX_CLUSTER = 8;
 constexpr int EV_MAX_CHUNK = 32768;  // slots per CTA: 6 bytes of shared memory each
 constexpr int EV_BINS = 2048, EV_BITS = 11;
-constexpr int EV_CLASS = 256;        // slots of a class that are ranked by counting
+constexpr int EV_CLASS = 128;        // slots of a class that are ranked by counting
 static_assert(EV_CLASS <= EV_THREADS, "one thread ranks one member");
 constexpr int EV_FLIGHT = 4;         // rows a warp has in flight
 constexpr uint32_t kProtected = 0xffffffffu;
@@ -124,6 +124,7 @@ struct EvictArgs {
   int64_t capacity;
   int chunk;     // slots per CTA
   int vec;       // rows move in 16-byte units
+  int quads;     // weights and positions move four slots at a time
   int counters;  // this kernel writes lengths_out (it is not lengths)
   uint32_t *err;
 };
@@ -190,17 +191,44 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const __grid_const
     }
     return;
   }
-  const int per = (n + S - 1) / S, s0 = min(rank * per, n), s1 = min(s0 + per, n), cnt = s1 - s0;
+  const int per = ((n + S - 1) / S + 3) & ~3, s0 = min(rank * per, n), s1 = min(s0 + per, n), cnt = s1 - s0;
+  // one CTA alone needs no cluster barrier and reads its own shared memory
+  auto sync_all = [&]() {
+    if (S == 1) __syncthreads();
+    else cluster.sync();
+  };
+  auto of = [&](auto *mine, int r) { return S == 1 ? mine : cluster.map_shared_rank(mine, r); };
 
   for (int i = tid; i < 3 * EV_BINS; i += EV_THREADS) (&hist[0][0])[i] = 0;
   if (tid == 0) counts[0] = 0;
   const bool w_apart = a.weights_out != a.weights, p_apart = a.positions_out != a.positions;
+  int done = 0;
+  if (p.quads) {
+    done = cnt & ~3;
+#pragma unroll 2
+    for (int i = 4 * tid; i < done; i += 4 * EV_THREADS) {
+      const float4 w = *reinterpret_cast<const float4 *>(a.weights + at + s0 + i);
+      const int4 pos = *reinterpret_cast<const int4 *>(a.positions + at + s0 + i);
+      *reinterpret_cast<uint4 *>(keys + i) =
+          make_uint4(evict_key(w.x, pos.x, recent_from, a.sinks), evict_key(w.y, pos.y, recent_from, a.sinks),
+                     evict_key(w.z, pos.z, recent_from, a.sinks), evict_key(w.w, pos.w, recent_from, a.sinks));
+      if (s0 + i + 4 <= C) {  // holes among these are overwritten below
+        if (w_apart) *reinterpret_cast<float4 *>(a.weights_out + at + s0 + i) = w;
+        if (p_apart) *reinterpret_cast<int4 *>(a.positions_out + at + s0 + i) = pos;
+      } else {
+        for (int e = 0; e < 4 && s0 + i + e < C; ++e) {
+          a.weights_out[at + s0 + i + e] = e == 0 ? w.x : e == 1 ? w.y : w.z;
+          a.positions_out[at + s0 + i + e] = e == 0 ? pos.x : e == 1 ? pos.y : pos.z;
+        }
+      }
+    }
+  }
 #pragma unroll 4
-  for (int i = tid; i < cnt; i += EV_THREADS) {
+  for (int i = done + tid; i < cnt; i += EV_THREADS) {
     const float w = a.weights[at + s0 + i];
     const int pos = a.positions[at + s0 + i];
     keys[i] = evict_key(w, pos, recent_from, a.sinks);
-    if (s0 + i < C) {  // holes among these are overwritten below
+    if (s0 + i < C) {
       if (w_apart) a.weights_out[at + s0 + i] = w;
       if (p_apart) a.positions_out[at + s0 + i] = pos;
     }
@@ -226,12 +254,12 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const __grid_const
       uint32_t *next = hist[(pass + 1) % 3];
       for (int i = tid; i < EV_BINS; i += EV_THREADS) next[i] = 0;
     }
-    cluster.sync();
+    sync_all();
     // thread t: the four bins from 4 * (511 - t), largest first
     uint4 q = make_uint4(0, 0, 0, 0);
     const int bin = EV_BINS - 4 * (tid + 1);
     for (int r = 0; r < S; ++r) {
-      const uint4 y = *reinterpret_cast<const uint4 *>(cluster.map_shared_rank(mine, r) + bin);
+      const uint4 y = *reinterpret_cast<const uint4 *>(of(mine, r) + bin);
       q.x += y.x;
       q.y += y.y;
       q.z += y.z;
@@ -260,12 +288,12 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const __grid_const
         const uint64_t x = number(i);
         if ((x >> shift) == (found >> shift)) members[atomicAdd(&counts[0], 1u)] = x;
       }
-      cluster.sync();
+      sync_all();
       // every CTA ranks them all: thread i counts the members larger than i
       uint32_t base = 0;
       for (int r = 0; r < S; ++r) {
-        const uint32_t m = *cluster.map_shared_rank(&counts[0], r);
-        if (uint32_t(tid) < m) all_members[base + tid] = cluster.map_shared_rank(members, r)[tid];
+        const uint32_t m = *of(&counts[0], r);
+        if (uint32_t(tid) < m) all_members[base + tid] = of(members, r)[tid];
         base += m;
       }
       __syncthreads();
@@ -306,34 +334,36 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const __grid_const
       at_list += 0x10000u;
     }
   }
-  cluster.sync();
+  sync_all();
   if (tid == 0) {
     uint32_t hs = 0, ms = 0;
     for (int r = 0; r < S; ++r) {
-      const uint32_t *o = cluster.map_shared_rank(&counts[0], r);
+      const uint32_t *o = of(&counts[0], r);
       hole_end[r] = hs += o[1];
       mover_end[r] = ms += o[2];
     }
   }
   __syncthreads();
 
-  // ---- moves: pair j = (j-th hole, j-th mover); a warp resolves 32 pairs,
-  // one per lane, and copies them with all lanes
+  // ---- moves: pair j = (j-th hole, j-th mover). A warp resolves up to 32
+  // pairs, one per lane, and copies them with all lanes; few pairs are spread
+  // over all warps
   const int lane = tid & 31, warps = S * (EV_THREADS / 32);
   const int moves = int(min(hole_end[S - 1], mover_end[S - 1]));
+  const int batch = min(32, (moves + warps - 1) / warps);
   const int es = c.dtype == WGX_FLOAT16 ? 2 : 4;
-  for (int j0 = (rank * (EV_THREADS / 32) + (tid >> 5)) * 32; j0 < moves; j0 += warps * 32) {
+  for (int j0 = (rank * (EV_THREADS / 32) + (tid >> 5)) * batch; j0 < moves; j0 += warps * batch) {
     const int j = j0 + lane;
-    int64_t kd = -1, ks = 0, vd = 0, vs = 0;  // byte offsets
-    if (j < moves) {
+    int64_t kd = -1, ks = -1, vd = 0, vs = 0;  // byte offsets; -1: no pair
+    if (lane < batch && j < moves) {
       int r = 0;
       while (uint32_t(j) >= hole_end[r]) ++r;
-      const int dst = r * per + cluster.map_shared_rank(list, r)[j - (r ? hole_end[r - 1] : 0)];
+      const int dst = r * per + of(list, r)[j - (r ? hole_end[r - 1] : 0)];
       r = 0;
       while (uint32_t(j) >= mover_end[r]) ++r;
       const int rsplit = max(0, min(C - r * per, min(per, n - r * per)));
       const int src =
-          r * per + cluster.map_shared_rank(list, r)[rsplit + (j - (r ? mover_end[r - 1] : 0))];
+          r * per + of(list, r)[rsplit + (j - (r ? mover_end[r - 1] : 0))];
       a.weights_out[at + dst] = a.weights[at + src];
       a.positions_out[at + dst] = a.positions[at + src];
       const int dp = dst / c.page_size, sp = src / c.page_size;
@@ -353,7 +383,7 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const __grid_const
       }
     }
     uint8_t *kb = static_cast<uint8_t *>(c.k), *vb = static_cast<uint8_t *>(c.v);
-    const int pairs = min(32, moves - j0);
+    const int pairs = min(batch, moves - j0);
     if (p.vec) {
       // a unit of EV_FLIGHT rows at a time: loads first, then stores
       const int units = c.head_dim * es / 16;
@@ -364,20 +394,16 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const __grid_const
           const int o = (isv ? i - units : i) * 16;
           uint8_t *base = (isv ? vb : kb) + o;
           uint4 v[EV_FLIGHT];
-          uint8_t *to[EV_FLIGHT];
 #pragma unroll
           for (int e = 0; e < EV_FLIGHT; ++e) {
-            const int64_t xkd = __shfl_sync(~0u, kd, x0 + e), xks = __shfl_sync(~0u, ks, x0 + e);
-            const int64_t xvd = __shfl_sync(~0u, vd, x0 + e), xvs = __shfl_sync(~0u, vs, x0 + e);
-            to[e] = nullptr;
-            if (on && xkd >= 0) {  // (lanes without a pair hold -1)
-              v[e] = *reinterpret_cast<const uint4 *>(base + (isv ? xvs : xks));
-              to[e] = base + (isv ? xvd : xkd);
-            }
+            const int64_t xks = __shfl_sync(~0u, ks, x0 + e), xvs = __shfl_sync(~0u, vs, x0 + e);
+            if (on && xks >= 0) v[e] = *reinterpret_cast<const uint4 *>(base + (isv ? xvs : xks));
           }
 #pragma unroll
-          for (int e = 0; e < EV_FLIGHT; ++e)
-            if (to[e]) *reinterpret_cast<uint4 *>(to[e]) = v[e];
+          for (int e = 0; e < EV_FLIGHT; ++e) {
+            const int64_t xkd = __shfl_sync(~0u, kd, x0 + e), xvd = __shfl_sync(~0u, vd, x0 + e);
+            if (on && xkd >= 0) *reinterpret_cast<uint4 *>(base + (isv ? xvd : xkd)) = v[e];
+          }
         }
       }
     } else {
@@ -397,7 +423,7 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const __grid_const
       }
     }
   }
-  cluster.sync();  // a CTA's lists are read by the others until here
+  if (S > 1) cluster.sync();  // a CTA's lists are read by the others until here
 }
 
 __global__ void evict_lengths_kernel(const __grid_constant__ EvictArgs p) {
@@ -463,6 +489,9 @@ void launch_cache_evict(const wgx_cache_evict_args &a, cudaStream_t stream) {
          " slots per sequence are not supported");
   p.chunk = int(((slots + S - 1) / S + 7) / 8 * 8);
   p.vec = cache_rows_16b(c);
+  p.quads = a.slots % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.weights) | reinterpret_cast<uintptr_t>(a.weights_out) |
+                                  reinterpret_cast<uintptr_t>(a.positions) |
+                                  reinterpret_cast<uintptr_t>(a.positions_out)) & 15) == 0;
   p.counters = a.lengths_out != a.lengths;
   const int dev = current_device();
   p.err = device_error_word(dev);
