@@ -49,7 +49,10 @@ inline int current_device() {
 #ifdef __CUDACC__
 // Programmatic dependent launch: the next kernel's blocks may be set up while
 // this one's work ends (every block of this kernel has started); wait returns
-// when all of the prior kernel's work is done and visible.
+// when all of the prior kernel's work is done and visible. Every kernel here
+// lets its dependents launch after its own wait: what a kernel reads before its
+// wait may then come from anything but its direct predecessor, which is what
+// the join and reorder_kernel rely on for the call's inputs.
 __device__ __forceinline__ void let_dependents_launch() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }

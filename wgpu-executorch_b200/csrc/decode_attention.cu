@@ -497,7 +497,6 @@ __global__ void __launch_bounds__(MmaShape<T, DP>::THREADS)
   const wgx_kv_cache &c = p.a.cache;
   const int lane = threadIdx.x % 32, worker = threadIdx.x / (32 * M::WARPS);
   const int part = threadIdx.x / 32 % M::WARPS;  // of the worker
-  let_dependents_launch();
   const BlockSmem sm = block_smem(pa_smem_raw, worker, M::RING, PA_BLOCK_WORKERS, c.batch);
   uint64_t *bars = all_bars[worker];
   const int D = c.head_dim;
@@ -529,6 +528,8 @@ __global__ void __launch_bounds__(MmaShape<T, DP>::THREADS)
       *reinterpret_cast<uint4 *>(sm.ring + i) = make_uint4(0u, 0u, 0u, 0u);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
+  wait_for_prior_kernel();
+  let_dependents_launch();
   build_prefix<TOK>(p, sm.prefix, sm.lens, p.scores != nullptr);  // (ends with a block barrier)
   const int rows = c.kv_heads * p.chunks;
   const uint32_t total = sm.prefix[c.batch] * uint32_t(rows);
@@ -919,7 +920,6 @@ __global__ void __launch_bounds__(SimtShape<DP, G>::THREADS)
   __shared__ __align__(8) uint64_t all_bars[PA_BLOCK_WORKERS][STAGES];
   const wgx_kv_cache &c = p.a.cache;
   const int lane = threadIdx.x % 32, worker = threadIdx.x / 32;
-  let_dependents_launch();
   const BlockSmem sm = block_smem(pa_smem_raw, worker, M::RING, PA_BLOCK_WORKERS, c.batch);
   uint64_t *bars = all_bars[worker];
   const int D = c.head_dim;
@@ -933,6 +933,8 @@ __global__ void __launch_bounds__(SimtShape<DP, G>::THREADS)
       *reinterpret_cast<uint4 *>(sm.ring + i) = make_uint4(0u, 0u, 0u, 0u);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
+  wait_for_prior_kernel();
+  let_dependents_launch();
   build_prefix<TOK>(p, sm.prefix, sm.lens, p.scores != nullptr);  // (ends with a block barrier)
   const int rows = c.kv_heads;  // (p.chunks is 1)
   const uint32_t total = sm.prefix[c.batch] * uint32_t(rows);
@@ -1218,6 +1220,7 @@ __global__ void __launch_bounds__(PA_JOIN_THREADS) join_kernel(const __grid_cons
 #pragma unroll
     for (int k = 0; k < KQ; ++k) at_quad[k] = min(lane + 32 * k, quads - 1);
     wait_for_prior_kernel();
+    let_dependents_launch();
     if (split) {
       const int n = w1 - w0 + 1;
       const float2 st = stats_of(w0, n, g);
@@ -1287,6 +1290,7 @@ __global__ void __launch_bounds__(PA_JOIN_THREADS) join_kernel(const __grid_cons
   const int t1 = min(t0 + PA_JOIN_SLOTS, int(min(int64_t(s.len), p.a.slots)));
   if (t0 >= t1) return;
   wait_for_prior_kernel();
+  let_dependents_launch();
   for (int g = warp; g < p.group; g += WARPS) {
     const int chunk = g / PA_HEADS, gr = g % PA_HEADS;
     int w0, w1;
@@ -1339,14 +1343,14 @@ __global__ void __launch_bounds__(PA_JOIN_THREADS) join_kernel(const __grid_cons
 }
 
 struct Config {
-  const void *kernel;
+  void (*kernel)(AttnArgs);
   int ring, tok, threads, ctas_per_sm;
 };
 
 template <typename T, int DP, bool HALF_ROWS>
 Config mma_config() {
   Config c{};
-  c.kernel = reinterpret_cast<const void *>(paged_attention_kernel<T, DP, HALF_ROWS>);
+  c.kernel = paged_attention_kernel<T, DP, HALF_ROWS>;
   c.ring = PA_BLOCK_WORKERS * MmaShape<T, DP>::RING + 1024;  // + alignment
   c.tok = Tile<T, DP>::TOK;
   c.threads = MmaShape<T, DP>::THREADS;
@@ -1355,7 +1359,7 @@ Config mma_config() {
 template <int DP, int G>
 Config simt_config() {
   Config c{};
-  c.kernel = reinterpret_cast<const void *>(paged_attention_simt_kernel<DP, G>);
+  c.kernel = paged_attention_simt_kernel<DP, G>;
   c.ring = PA_BLOCK_WORKERS * SimtShape<DP, G>::RING + 1024;
   c.tok = 8;
   c.threads = SimtShape<DP, G>::THREADS;
@@ -1479,12 +1483,10 @@ void launch_paged_attention(const wgx_paged_attention_args &a, cudaStream_t stre
     fail("paged_attention: scratch of " + std::to_string(l.bytes) + " bytes, 256-byte aligned, needed");
   l.p.err = device_error_word(current_device());
   const wgx_kv_cache &c = a.cache;
-  void *args[] = {&l.p};
   const int pre = prefix_bytes(c.batch);
   const int th = timer_begin("paged_attention_kernel", stream);
-  check_cuda(cudaLaunchKernel(l.cfg->kernel, dim3(unsigned(l.grid)), dim3(unsigned(l.cfg->threads)), args,
-                              size_t(l.cfg->ring + pre), stream),
-             "paged_attention launch");
+  launch_dependent(l.cfg->kernel, dim3(unsigned(l.grid)), l.cfg->threads, size_t(l.cfg->ring + pre), stream,
+                   "paged_attention launch", l.p);
   timer_end(th, stream);
   int64_t blocks = l.p.o_blocks;
   if (a.weights_out)

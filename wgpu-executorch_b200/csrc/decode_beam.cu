@@ -107,9 +107,10 @@ __global__ void __launch_bounds__(BM_THREADS, BM_BLOCKS_PER_SM) scan_kernel(cons
   __shared__ uint64_t bound, best[BM_WARPS];
   __shared__ uint64_t list[BM_LIST];
   __shared__ uint32_t n_list;
-  let_dependents_launch();
   const wgx_beam_search_args &a = p.a;
   const int row = blockIdx.y, seg = blockIdx.x, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  wait_for_prior_kernel();
+  let_dependents_launch();
   if (a.finished[row]) return;  // proposes eos: its logits are not needed
   const int K = a.beams;
   const T *x = static_cast<const T *>(a.logits) + int64_t(row / K) * a.logits_batch_stride +
@@ -299,8 +300,8 @@ __global__ void __launch_bounds__(BM_SEL_THREADS) select_kernel(const __grid_con
   __shared__ uint32_t n_cand;
   const int b = blockIdx.x, W = a.beams, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int list = p.segments * W, all = W * list;
-  let_dependents_launch();
   wait_for_prior_kernel();
+  let_dependents_launch();
   if (tid == 0) n_cand = 0;
   // entry i % list of beam i / list, i = tid + j * threads: the first BM_HELD of
   // a thread are loaded now, beside the segments' sums
@@ -442,6 +443,7 @@ __global__ void __launch_bounds__(BM_COPY_THREADS) reorder_kernel(const __grid_c
   const int child = blockIdx.y, tid = threadIdx.x;
   const int spare = a.spare[child];
   wait_for_prior_kernel();
+  let_dependents_launch();
   const int from = child / a.beams * a.beams + a.parents[child];
   const int len = slots_in_use(a.lengths, from, p.capacity, p.err);
   const int full = len / c.page_size, tail = len - full * c.page_size;
@@ -541,14 +543,9 @@ void launch_beam_search_step(const wgx_beam_search_args &a, cudaStream_t stream)
   const int ls = dtype_size(a.dtype);
   const bool vec = ((a.logits_batch_stride * ls) | (a.logits_beam_stride * ls) |
                     int64_t(reinterpret_cast<uintptr_t>(a.logits))) % 16 == 0;
-  if (a.dtype == WGX_FLOAT16) {
-    if (vec) scan_kernel<__half, true><<<grid, BM_THREADS, 0, stream>>>(p);
-    else scan_kernel<__half, false><<<grid, BM_THREADS, 0, stream>>>(p);
-  } else {
-    if (vec) scan_kernel<float, true><<<grid, BM_THREADS, 0, stream>>>(p);
-    else scan_kernel<float, false><<<grid, BM_THREADS, 0, stream>>>(p);
-  }
-  check_cuda(cudaGetLastError(), "beam_search_step launch");
+  launch_dependent(a.dtype == WGX_FLOAT16 ? (vec ? scan_kernel<__half, true> : scan_kernel<__half, false>)
+                                          : (vec ? scan_kernel<float, true> : scan_kernel<float, false>),
+                   grid, BM_THREADS, 0, stream, "beam_search_step launch", p);
   timer_end(th, stream);
   launch_dependent(select_kernel, dim3(unsigned(a.batch)), BM_SEL_THREADS, 0, stream,
                    "beam_search_step selection launch", p);

@@ -40,6 +40,8 @@ __global__ void __launch_bounds__(AP_THREADS) append_kernel(const __grid_constan
   const wgx_kv_append_args &a = p.a;
   const wgx_kv_cache &c = a.cache;
   const int b = blockIdx.y;
+  wait_for_prior_kernel();
+  let_dependents_launch();
   const int len = slots_in_use(a.lengths, b, p.capacity, p.err);
   const int seen = a.seen ? a.seen[b] : 0;
   const bool fits = int64_t(len) + a.tokens <= p.capacity;
@@ -179,6 +181,10 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const __grid_const
   const wgx_kv_cache &c = a.cache;
   const int tid = threadIdx.x, row = int(blockIdx.x) / S;
   const int b = row / c.kv_heads, h = row % c.kv_heads, C = a.budget;
+  for (int i = tid; i < 3 * EV_BINS; i += EV_THREADS) (&hist[0][0])[i] = 0;
+  if (tid == 0) counts[0] = 0;
+  wait_for_prior_kernel();
+  let_dependents_launch();
   const int len = slots_in_use(a.lengths, b, p.capacity, p.err);
   const int recent_from = a.seen[b] - a.recent;
   const int n = int(min(int64_t(len), a.slots));
@@ -199,8 +205,6 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const __grid_const
   };
   auto of = [&](auto *mine, int r) { return S == 1 ? mine : cluster.map_shared_rank(mine, r); };
 
-  for (int i = tid; i < 3 * EV_BINS; i += EV_THREADS) (&hist[0][0])[i] = 0;
-  if (tid == 0) counts[0] = 0;
   const bool w_apart = a.weights_out != a.weights, p_apart = a.positions_out != a.positions;
   int done = 0;
   if (p.quads) {
@@ -457,15 +461,15 @@ void launch_kv_append(const wgx_kv_append_args &a, cudaStream_t stream) {
   const int th = timer_begin("append_kernel", stream);
 #define WGX_APPEND(U, STEP)                                                          \
   do {                                                                               \
-    if (wide) append_kernel<U, STEP, uint64_t><<<grid, AP_THREADS, 0, stream>>>(p);  \
-    else append_kernel<U, STEP, uint32_t><<<grid, AP_THREADS, 0, stream>>>(p);       \
+    launch_dependent(wide ? append_kernel<U, STEP, uint64_t>                         \
+                          : append_kernel<U, STEP, uint32_t>,                        \
+                     grid, AP_THREADS, 0, stream, "kv_append launch", p);            \
   } while (0)
   if (vec && es == 2) WGX_APPEND(uint4, 8);
   else if (vec) WGX_APPEND(uint4, 4);
   else if (es == 2) WGX_APPEND(uint16_t, 1);
   else WGX_APPEND(uint32_t, 1);
 #undef WGX_APPEND
-  check_cuda(cudaGetLastError(), "kv_append launch");
   timer_end(th, stream);
   if (!p.counters) {
     advance_kernel<<<unsigned(c.batch + 127) / 128, 128, 0, stream>>>(p);
@@ -511,12 +515,14 @@ void launch_cache_evict(const wgx_cache_evict_args &a, cudaStream_t stream) {
   cfg.blockDim = dim3(EV_THREADS);
   cfg.dynamicSmemBytes = size_t(p.chunk) * 6;
   cfg.stream = stream;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = unsigned(S);
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   const int th = timer_begin("evict_kernel", stream);
   check_cuda(cudaLaunchKernelEx(&cfg, evict_kernel, p), "cache_evict launch");
   timer_end(th, stream);
