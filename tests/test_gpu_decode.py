@@ -154,6 +154,17 @@ def test_attention_lengths(dec, dtype, n):
 
 
 @pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("width", [4, 14, 30, 60, 400])
+@pytest.mark.parametrize("D,G", [(64, 2), (128, 4), (256, 3), (128, 12), (64, 20)])
+def test_attention_table_widths(dec, dtype, width, D, G):
+    """The same sequences under tables of more and more pages: how a row's work
+    is divided (a block, a cluster of blocks, shares of the whole grid) goes by
+    what the table can name, the result does not."""
+    check_attention(dec, Cache([64, 0, 1, 33, 50], 2, D, 16, dtype, width=width), 2 * G, weights=True)
+    check_attention(dec, Cache([64, 7], 2, D, 16, dtype, width=width), 2 * G, window=20)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
 def test_attention_ragged_batch(dec, dtype):
     rng = np.random.default_rng(3)
     lengths = rng.integers(0, 700, 150)

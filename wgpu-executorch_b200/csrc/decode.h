@@ -59,20 +59,24 @@ __device__ __forceinline__ void let_dependents_launch() {
 __device__ __forceinline__ void wait_for_prior_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // Launches a kernel that may be set up while the stream's previous kernel ends
 // (it calls griddepcontrol.wait before it touches what that one writes).
-template <typename... P, typename... A>
-void launch_dependent(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t stream,
-                      const char *what, const A &...args) {
+// cluster > 1: in clusters of so many blocks.
+template <typename P>
+void launch_dependent(void (*kernel)(P), dim3 grid, int threads, size_t smem, cudaStream_t stream,
+                      const char *what, const P &arg, int cluster = 0) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(unsigned(threads));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = unsigned(cluster);
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
-  check_cuda(cudaLaunchKernelEx(&cfg, kernel, args...), what);
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  check_cuda(cudaLaunchKernelEx(&cfg, kernel, arg), what);
 }
 
 // Slots in use of sequence b, held within [0, capacity].

@@ -24,6 +24,8 @@
 // by a share's end leave (max, sum, unnormalised result) in scratch, at most
 // two per warp, and join_kernel combines them; it also accumulates the
 // probabilities per slot from the scores, kept in scratch for it.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <mutex>
 
@@ -31,12 +33,27 @@
 #include "tcgen05.h"
 #include "tma.h"
 
+namespace cg = cooperative_groups;
+
 namespace wgx {
 
 namespace {
 
 constexpr int PA_HEADS = 16;        // rows of an mma tile
 constexpr int PA_MAX_GROUP = 128;   // query heads per K/V head
+// Row mode, a block (or a cluster of 2 or 4) per row instead of equal shares of
+// the line and a second kernel: no scratch, no join, but rows must be alike and
+// short. Steps a block's part of a row may have: 16; 8 with fp32, 4 above 128
+// channels (their steps take longer). Measured, us a call, 8 K/V heads x 4 heads
+// of 128, fp16, batch 1 / 8: 128 slots 6.1 / 6.5 in row mode, 11.4 / 11.4
+// split; 256: 8.3 / 8.7, 10.8 / 11.6; 512, clusters of 4: 9.6 / 10.6, 10.2 /
+// 12.6; 1024: 11.9 / 13.6, 13.2 / 16.3; 2048: 16.5 / 19.5, 12.2 / 24.2. fp32:
+// 64 slots 8.1 / 8.2, 9.9 / 10.7; 256, clusters of 4: 11.4 / 12.6, 11.6 / 13.6.
+// A lone row is better split from the start of clusters on (one head of 256
+// channels x 16, 256 slots: 12.6 in a cluster, 10.2 split).
+constexpr int PA_ROW_STEPS = 16;
+constexpr int PA_ROW_CLUSTER = 4;
+constexpr int PA_ROW_MIN = 8;  // rows from which clusters are used
 constexpr int PA_JOIN_THREADS = 256;
 constexpr int PA_JOIN_SLOTS = 4096;  // slots per join block of the accumulation
 
@@ -47,7 +64,8 @@ struct AttnArgs {
   int group;          // query heads per K/V head
   int chunks;         // ceil(group / PA_HEADS)
   int max_workers;    // warps the scratch has room for
-  int min_steps;      // steps a warp takes at least
+  int min_steps;      // steps a worker takes at least
+  int row_blocks;     // row mode: a cluster of so many blocks per row of work; 0: off
   int vec;            // rows move in 16-byte units
   int tma;            // a step's rows lie in one page and move by TMA
   int boxes;          // TMA copies per operand and step
@@ -448,29 +466,97 @@ __device__ void drain(uint64_t live_ring, uint64_t *bars, int stage, uint32_t ph
   }
 }
 
-// Shared memory of a block: the workers' rings (1024-byte aligned), then the
-// sequences' prefix and lengths.
+// Shared memory of a block: the workers' rings (1024-byte aligned), what else
+// each worker needs, then the sequences' prefix and lengths.
 struct BlockSmem {
-  uint8_t *ring;
+  uint8_t *ring, *extra;
   uint32_t *prefix;
   int *lens;
 };
-__device__ __forceinline__ BlockSmem block_smem(uint8_t *raw, int worker, int ring_bytes, int workers, int batch) {
+__device__ __forceinline__ BlockSmem block_smem(uint8_t *raw, int worker, int ring_bytes, int extra_bytes,
+                                                int workers, int batch) {
   uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   BlockSmem m;
   m.ring = base + size_t(worker) * ring_bytes;
-  m.prefix = reinterpret_cast<uint32_t *>(base + size_t(workers) * ring_bytes);
+  m.extra = base + size_t(workers) * ring_bytes + size_t(worker) * extra_bytes;
+  m.prefix = reinterpret_cast<uint32_t *>(base + size_t(workers) * (ring_bytes + extra_bytes));
   m.lens = reinterpret_cast<int *>(m.prefix + batch + 1);
   return m;
 }
 
 constexpr int PA_BLOCK_WORKERS = 4;
 
+// Row mode: joins the results of the row's workers, four per block of the
+// cluster (o: [head][stride] floats at the front of each worker's ring; ml:
+// their maxima and sums), and accumulates the row's probabilities: each block
+// takes a share of the output and the slots whose scores it wrote. Every thread
+// of the block.
+// CLUSTER: more blocks than one.
+template <typename T, int TOK, bool CLUSTER>
+__device__ void finish_row(const AttnArgs &p, int b, int row, const Span &s, float2 (*ml)[PA_HEADS],
+                           uint8_t *rings, int ring_bytes, int stride) {
+  constexpr int MOST = PA_BLOCK_WORKERS * PA_ROW_CLUSTER;
+  __shared__ float factor[MOST][PA_HEADS], head_m[PA_HEADS], head_inv[PA_HEADS];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int S = CLUSTER ? p.row_blocks : 1, rank = CLUSTER ? int(cluster.block_rank()) : 0;
+  auto of = [&](auto *mine, int r) {
+    if constexpr (CLUSTER) return cluster.map_shared_rank(mine, r);
+    else return mine;
+  };
+  const int tid = threadIdx.x, D = p.a.cache.head_dim, parts = S * PA_BLOCK_WORKERS;
+  const int h = row / p.chunks, chunk = row - h * p.chunks, nh = min(p.heads, p.group - chunk * PA_HEADS);
+  if constexpr (CLUSTER) cluster.sync();
+  else __syncthreads();
+  if (tid < nh) {
+    float M = -INFINITY, sum = 0.f;
+    for (int w = 0; w < parts; ++w)
+      M = fmaxf(M, of(&ml[0][0], w / PA_BLOCK_WORKERS)[w % PA_BLOCK_WORKERS * PA_HEADS + tid].x);
+    const float mu = M == -INFINITY ? 0.f : M;
+    for (int w = 0; w < parts; ++w) {
+      const float2 x = of(&ml[0][0], w / PA_BLOCK_WORKERS)[w % PA_BLOCK_WORKERS * PA_HEADS + tid];
+      const float f = exp2_approx(x.x - mu);
+      factor[w][tid] = f;
+      sum += f * x.y;
+    }
+    head_m[tid] = mu;
+    head_inv[tid] = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+  }
+  __syncthreads();
+  T *out = static_cast<T *>(p.a.out) + int64_t(b) * p.a.out_batch_stride +
+           int64_t(h * p.group + chunk * PA_HEADS) * p.a.out_head_stride;
+  for (int i = rank * int(blockDim.x) + tid; i < nh * D; i += S * int(blockDim.x)) {
+    const int g = i / D, d = i - g * D;
+    float v = 0.f;
+#pragma unroll 4
+    for (int w = 0; w < parts; ++w) {
+      const float f = factor[w][g];  // (zero: the worker may not have written its result)
+      const float *o = reinterpret_cast<const float *>(of(rings, w / PA_BLOCK_WORKERS) +
+                                                       size_t(w % PA_BLOCK_WORKERS) * ring_bytes);
+      if (f != 0.f) v += f * o[g * stride + d];
+    }
+    out[int64_t(g) * p.a.out_head_stride + d] = T(v * head_inv[g]);
+  }
+  if (p.scores) {
+    const int64_t at = (int64_t(b) * p.a.cache.kv_heads + h) * p.a.slots;
+    const float *sc = p.scores + (int64_t(b) * p.a.q_heads + h * p.group) * p.score_stride;
+    const int t0 = rank ? (s.first + s.steps * rank / S) * TOK : 0;
+    const int t1 = min((s.first + s.steps * (rank + 1) / S) * TOK, int(min(int64_t(s.len), p.a.slots)));
+    for (int t = t0 + tid; t < t1; t += int(blockDim.x)) {
+      float w = p.a.weights[at + t];
+      if (t >= s.first * TOK)
+        for (int g = 0; g < nh; ++g) w += exp2_approx(sc[int64_t(g) * p.score_stride + t] - head_m[g]) * head_inv[g];
+      p.a.weights_out[at + t] = w;
+    }
+  }
+  if constexpr (CLUSTER) cluster.sync();  // a block's results are read by the others until here
+}
+
 // Tensor-core form: the worker's heads are the 16 rows of an mma tile.
 // HALF_ROWS: at most 8 heads (rows 8-15 are padding and their softmax is left
-// out). Heads of 256 channels: two warps share a worker; both form the scores,
-// each the result of its half of the channels (one warp's 128 result registers
-// beside 64 of the query left room for one warp per scheduler).
+// out). Heads of 256 channels: two warps share a worker, each with half of the
+// channels: the halves of the scores are added through shared memory (one
+// warp's 128 result registers beside 64 of the query left room for one warp per
+// scheduler).
 template <typename T, int DP>
 struct MmaShape {
   static constexpr int WARPS = DP > 128 ? 2 : 1;  // per worker
@@ -479,9 +565,9 @@ struct MmaShape {
   static constexpr bool kQShared = sizeof(T) == 4 && DP > 128;
   static constexpr int STAGES = kQShared ? 2 : Tile<T, DP>::STAGE > 4096 ? 3 : 4;
   static constexpr int QBYTES = kQShared ? PA_HEADS * Tile<T, DP>::ROW : 0;
-  static constexpr int RING = STAGES * Tile<T, DP>::STAGE + QBYTES;
+  static constexpr int RING = STAGES * Tile<T, DP>::STAGE, EXTRA = QBYTES;
   static constexpr int THREADS = PA_BLOCK_WORKERS * WARPS * 32;
-  static_assert(PA_BLOCK_WORKERS * RING + 1024 + (2 * 2048 + 1) * 4 <= 227 * 1024, "shared memory of a block");
+  static_assert(PA_BLOCK_WORKERS * (RING + EXTRA) + 1024 + (2 * 2048 + 1) * 4 + 10 * 1024 <= 227 * 1024, "shared memory of a block");
 };
 
 template <typename T, int DP, bool HALF_ROWS>
@@ -494,10 +580,12 @@ __global__ void __launch_bounds__(MmaShape<T, DP>::THREADS)
   constexpr int HALVES = HALF_ROWS ? 1 : 2, ST = TOK / 8;
   extern __shared__ uint8_t pa_smem_raw[];
   __shared__ __align__(8) uint64_t all_bars[PA_BLOCK_WORKERS][STAGES];
+  __shared__ float2 row_ml[PA_BLOCK_WORKERS][PA_HEADS];
+  __shared__ __align__(16) float4 halves[M::WARPS == 2 ? PA_BLOCK_WORKERS : 1][2][M::WARPS == 2 ? ST : 1][32];
   const wgx_kv_cache &c = p.a.cache;
   const int lane = threadIdx.x % 32, worker = threadIdx.x / (32 * M::WARPS);
   const int part = threadIdx.x / 32 % M::WARPS;  // of the worker
-  const BlockSmem sm = block_smem(pa_smem_raw, worker, M::RING, PA_BLOCK_WORKERS, c.batch);
+  const BlockSmem sm = block_smem(pa_smem_raw, worker, M::RING, M::EXTRA, PA_BLOCK_WORKERS, c.batch);
   uint64_t *bars = all_bars[worker];
   const int D = c.head_dim;
   // barrier among the worker's warps; true when all of their threads say so
@@ -521,33 +609,104 @@ __global__ void __launch_bounds__(MmaShape<T, DP>::THREADS)
     for (int s = 0; s < STAGES; ++s) mbar_init(smem_u32(&bars[s]), p.tma ? 1 : 32);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (D < DP && part == 0) {
+  if (D < DP && !p.tma && part == 0) {
     // chunks behind the rows' ends: read by the products (with zero queries),
     // never loaded
     for (int i = lane * 16; i < M::RING; i += 512)
       *reinterpret_cast<uint4 *>(sm.ring + i) = make_uint4(0u, 0u, 0u, 0u);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
+  if (p.tma && threadIdx.x == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&p.k_map) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&p.v_map) : "memory");
+  }
   wait_for_prior_kernel();
   let_dependents_launch();
-  build_prefix<TOK>(p, sm.prefix, sm.lens, p.scores != nullptr);  // (ends with a block barrier)
   const int rows = c.kv_heads * p.chunks;
-  const uint32_t total = sm.prefix[c.batch] * uint32_t(rows);
-  const uint32_t workers = worker_count(p, total);
-  const uint32_t me = uint32_t(worker) * gridDim.x + blockIdx.x;
-  if (total == 0 || me >= workers) return;
-  const Shares shares(total, workers);
-  const uint32_t begin = shares.begin(me), end = shares.begin(me + 1);
-
   Walk<TOK> cur;
-  cur.start(p, sm.prefix, sm.lens, rows, begin);
-  uint32_t to_do = end - begin;
+  uint32_t to_do, me = 0;
+  if (p.row_blocks) {
+    // this cluster's row, this block's part of it, a quarter of that per worker
+    const int unit = int(blockIdx.x) / p.row_blocks, rank = int(blockIdx.x) - unit * p.row_blocks;
+    cur.b = unit / rows;
+    cur.row = unit - cur.b * rows;
+    cur.s = span_of<TOK>(p, slots_in_use(p.a.lengths, cur.b, p.capacity, p.err));
+    // (steps * blocks * workers is small: row mode is for short tables)
+    const int lo = cur.s.steps * rank / p.row_blocks, hi = cur.s.steps * (rank + 1) / p.row_blocks;
+    cur.step = lo + (hi - lo) * worker / PA_BLOCK_WORKERS;
+    to_do = uint32_t(lo + (hi - lo) * (worker + 1) / PA_BLOCK_WORKERS - cur.step);
+    if (part == 0 && lane < PA_HEADS) row_ml[worker][lane] = make_float2(-INFINITY, 0.f);
+    __syncthreads();
+  } else {
+    build_prefix<TOK>(p, sm.prefix, sm.lens, p.scores != nullptr);  // (ends with a block barrier)
+    const uint32_t total = sm.prefix[c.batch] * uint32_t(rows);
+    const uint32_t workers = worker_count(p, total);
+    me = uint32_t(worker) * gridDim.x + blockIdx.x;
+    if (total == 0 || me >= workers) return;
+    const Shares shares(total, workers);
+    const uint32_t begin = shares.begin(me);
+    cur.start(p, sm.prefix, sm.lens, rows, begin);
+    to_do = shares.begin(me + 1) - begin;
+  }
   Loader<T, DP, STAGES> loader;
-  loader.start(p, cur, to_do, lane);
+  loader.to_load = 0;
+  // the queries of the row at hand
+  constexpr int QK = DP / M::WARPS / (L::kHalf ? 16 : 8);  // this warp's operand columns
+  const int d0 = part * WP * PANEL;                        // and first channel
+  uint32_t qf[M::kQShared ? 1 : QK][4];
+  auto load_q = [&]() {
+    const int h = cur.row / p.chunks, chunk = cur.row - h * p.chunks;
+    const int nh = min(p.heads, p.group - chunk * PA_HEADS);
+    const T *q = static_cast<const T *>(p.a.q) + int64_t(cur.b) * p.a.q_batch_stride +
+                 int64_t(h * p.group + chunk * PA_HEADS) * p.a.q_head_stride;
+    auto qv = [&](int g, int d) -> T {
+      return (g < nh && d < D) ? q[int64_t(g) * p.a.q_head_stride + d] : T(0.f);
+    };
+    const int r0 = lane >> 2, kq = lane & 3;
+    if constexpr (L::kHalf) {
+#pragma unroll
+      for (int kk = 0; kk < QK; ++kk)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int g = r0 + (j & 1) * 8, d = d0 + kk * 16 + 2 * kq + (j >> 1) * 8;
+          if ((j & 1) && HALF_ROWS) {
+            qf[kk][j] = 0u;
+          } else if (p.q_pairs) {
+            qf[kk][j] = g < nh && d < D ? *reinterpret_cast<const uint32_t *>(
+                                              q + int64_t(g) * p.a.q_head_stride + d)
+                                        : 0u;
+          } else {
+            const __half2 v = __half2(qv(g, d), qv(g, d + 1));
+            qf[kk][j] = *reinterpret_cast<const uint32_t *>(&v);
+          }
+        }
+    } else if constexpr (!M::kQShared) {
+#pragma unroll
+      for (int kk = 0; kk < QK; ++kk)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          qf[kk][j] = __float_as_uint(qv(r0 + (j & 1) * 8, d0 + kk * 8 + kq + (j >> 1) * 4));
+    } else {
+      // (this warp's channels; it alone reads them)
+      __syncwarp();
+      const uint32_t q_a = smem_u32(sm.extra);
+      for (int g = 0; g < PA_HEADS; ++g)
+        for (int d = d0 + lane; d < d0 + WP * PANEL; d += 32) {
+          const bool in = g < nh && d < D;
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(
+                           q_a + uint32_t(g * L::ROW + (((d / 4) ^ (g & 7)) << 4) + (d % 4) * 4)),
+                       "l"(in ? q + int64_t(g) * p.a.q_head_stride + d : q), "r"(in ? 4 : 0)
+                       : "memory");
+        }
+    }
+  };
+  if (to_do) {
+    load_q();  // (in flight beside the first steps' page table entries)
+    loader.start(p, cur, to_do, lane);
+  }
 #pragma unroll 1
   for (int s = 0; s < STAGES - 1; ++s) loader.next(p, sm.lens, rows, sm.ring, bars, s, lane, part == 0);
 
-  uint32_t qf[M::kQShared ? 1 : (L::kHalf ? DP / 16 : DP / 8)][4];
   float o[NT][4];
   const uint32_t ring_a = smem_u32(sm.ring);
   // Bytes of this lane's chunks within a panel of K and of V (L::at): the
@@ -566,15 +725,14 @@ __global__ void __launch_bounds__(MmaShape<T, DP>::THREADS)
       v0 = uint32_t(vt * 128 + (((lane >> 4) ^ vt) << 4) + in);
       v1 = uint32_t((vt + 1) * 128 + (((lane >> 4) ^ (vt + 1)) << 4) + in);
     }
-    const uint32_t mine = uint32_t(part * WP * TOK * 128);  // this warp's panels of V
+    const uint32_t mine = uint32_t(part * WP * TOK * 128);  // this warp's panels
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      kx[i] = k0 ^ uint32_t(32 * i);
+      kx[i] = (k0 ^ uint32_t(32 * i)) + mine;
       vx[i] = (v0 ^ uint32_t(32 * i)) + mine;
       if constexpr (!L::kHalf) vx[4 + i] = (v1 ^ uint32_t(32 * i)) + mine;
     }
   }
-  const int d0 = part * WP * PANEL;  // this warp's first channel of the result
   int stage = 0;
   uint32_t phase = 0;  // bit s: parity of stage s's next wait
   bool ok = true;
@@ -584,48 +742,13 @@ __global__ void __launch_bounds__(MmaShape<T, DP>::THREADS)
     const bool from_begin = cur.step == 0;  // this share holds the row's first step
     const int nh = min(p.heads, p.group - chunk * PA_HEADS);
     float m[HALVES], l[HALVES];
-    {
-      const T *q = static_cast<const T *>(p.a.q) + int64_t(cur.b) * p.a.q_batch_stride +
-                   int64_t(h * p.group + chunk * PA_HEADS) * p.a.q_head_stride;
-      auto qv = [&](int g, int d) -> T {
-        return (g < nh && d < D) ? q[int64_t(g) * p.a.q_head_stride + d] : T(0.f);
-      };
-      const int r0 = lane >> 2, kq = lane & 3;
-      if constexpr (L::kHalf) {
 #pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk)
+    for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int g = r0 + (j & 1) * 8, d = kk * 16 + 2 * kq + (j >> 1) * 8;
-            if ((j & 1) && HALF_ROWS) {
-              qf[kk][j] = 0u;
-            } else if (p.q_pairs) {
-              qf[kk][j] = g < nh && d < D ? *reinterpret_cast<const uint32_t *>(
-                                                q + int64_t(g) * p.a.q_head_stride + d)
-                                          : 0u;
-            } else {
-              const __half2 v = __half2(qv(g, d), qv(g, d + 1));
-              qf[kk][j] = *reinterpret_cast<const uint32_t *>(&v);
-            }
-          }
-      } else if constexpr (!M::kQShared) {
-#pragma unroll
-        for (int kk = 0; kk < DP / 8; ++kk)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            qf[kk][j] = __float_as_uint(qv(r0 + (j & 1) * 8, kk * 8 + kq + (j >> 1) * 4));
-      } else {
-        worker_all(true);
-        for (int g = part; g < PA_HEADS; g += M::WARPS)
-          for (int d = lane; d < DP; d += 32)
-            *reinterpret_cast<T *>(sm.ring + STAGES * L::STAGE + g * L::ROW +
-                                   (((d / 4) ^ (g & 7)) << 4) + (d % 4) * 4) = qv(g, d);
-        worker_all(true);
-      }
-#pragma unroll
-      for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-#pragma unroll
-      for (int x = 0; x < HALVES; ++x) m[x] = -INFINITY, l[x] = 0.f;
+    for (int x = 0; x < HALVES; ++x) m[x] = -INFINITY, l[x] = 0.f;
+    if constexpr (M::kQShared) {
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      __syncwarp();
     }
     const uint32_t here = min(uint32_t(cur.s.steps - cur.step), to_do);
 #pragma unroll 1
@@ -654,8 +777,8 @@ __global__ void __launch_bounds__(MmaShape<T, DP>::THREADS)
       if constexpr (L::kHalf) {
         float s2[2][4] = {};  // odd columns: sums of their own, for the pipeline
 #pragma unroll
-        for (int pn = 0; pn < L::PANELS; ++pn) {
-          if (pn * PANEL < D) {
+        for (int pn = 0; pn < WP; ++pn) {
+          if (d0 + pn * PANEL < D) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               uint32_t b[4];
@@ -675,8 +798,8 @@ __global__ void __launch_bounds__(MmaShape<T, DP>::THREADS)
         // small products have sums of their own, and the large ones two
         float lo[4] = {}, lo2[4] = {}, odd[4] = {};
 #pragma unroll
-        for (int pn = 0; pn < L::PANELS; ++pn) {
-          if (pn * PANEL < D) {
+        for (int pn = 0; pn < WP; ++pn) {
+          if (d0 + pn * PANEL < D) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const int kk = pn * 4 + i;
@@ -685,8 +808,8 @@ __global__ void __launch_bounds__(MmaShape<T, DP>::THREADS)
               for (int j = 0; j < 4; ++j) {
                 if constexpr (M::kQShared) {
                   const int g = r + (j & 1) * 8;
-                  const uint32_t qa = ring_a + uint32_t(STAGES * L::STAGE + g * L::ROW + ((g & 7) << 4) + (lane & 3) * 4);
-                  split_tf32(lds32(qa ^ uint32_t((2 * kk + (j >> 1)) << 4)), ah[j], al[j]);
+                  const uint32_t qa = smem_u32(sm.extra) + uint32_t(g * L::ROW + ((g & 7) << 4) + (lane & 3) * 4);
+                  split_tf32(lds32(qa ^ uint32_t((d0 / 4 + 2 * kk + (j >> 1)) << 4)), ah[j], al[j]);
                 } else {
                   split_tf32(__uint_as_float(qf[kk][j]), ah[j], al[j]);
                 }
@@ -702,6 +825,21 @@ __global__ void __launch_bounds__(MmaShape<T, DP>::THREADS)
         }
 #pragma unroll
         for (int j = 0; j < 2 * HALVES; ++j) s[0][j] += odd[j] + (lo[j] + lo2[j]);
+      }
+      if constexpr (M::WARPS == 2) {
+        // the other warp's half of the channels
+#pragma unroll
+        for (int t = 0; t < ST; ++t)
+          halves[worker][part][t][lane] = make_float4(s[t][0], s[t][1], s[t][2], s[t][3]);
+        worker_all(true);
+#pragma unroll
+        for (int t = 0; t < ST; ++t) {
+          const float4 y = halves[worker][part ^ 1][t][lane];
+          s[t][0] += y.x;
+          s[t][1] += y.y;
+          s[t][2] += y.z;
+          s[t][3] += y.w;
+        }
       }
       // ---- running softmax, base 2. The reference value m follows the
       // maximum only when that has grown by more than 2^8: the probabilities
@@ -845,6 +983,7 @@ __global__ void __launch_bounds__(MmaShape<T, DP>::THREADS)
     }
     to_do -= here;
     const bool whole = from_begin && cur.step + int(here) == cur.s.steps;
+    if (p.row_blocks) worker_all(true);  // (the ring becomes the result's place)
 #pragma unroll
     for (int x = 0; x < HALVES; ++x) {
       float sum = l[x];
@@ -852,7 +991,13 @@ __global__ void __launch_bounds__(MmaShape<T, DP>::THREADS)
       sum += __shfl_xor_sync(~0u, sum, 2);
       const int g = (lane >> 2) + 8 * x;
       if (g >= nh || !ok) continue;
-      if (whole) {
+      if (p.row_blocks) {
+        float *ro = reinterpret_cast<float *>(sm.ring) + g * DP;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          *reinterpret_cast<float2 *>(ro + d0 + n * 8 + 2 * (lane & 3)) = make_float2(o[n][2 * x], o[n][2 * x + 1]);
+        if (part == 0 && (lane & 3) == 0) row_ml[worker][g] = make_float2(m[x], sum);
+      } else if (whole) {
         const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
         T *out = static_cast<T *>(p.a.out) + int64_t(cur.b) * p.a.out_batch_stride +
                  int64_t(h * p.group + chunk * PA_HEADS + g) * p.a.out_head_stride;
@@ -878,9 +1023,16 @@ __global__ void __launch_bounds__(MmaShape<T, DP>::THREADS)
         if (part == 0 && (lane & 3) == 0) p.part_ml[at] = make_float2(m[x], sum);
       }
     }
+    if (p.row_blocks || !to_do) break;
     cur.next_row(p, sm.lens, rows);
+    load_q();
   }
   if (!ok) drain<STAGES>(loader.live_ring, bars, stage, phase);
+  uint8_t *rings = sm.ring - size_t(worker) * M::RING;
+  if (p.row_blocks == 1)
+    finish_row<T, TOK, false>(p, cur.b, cur.row, cur.s, row_ml, rings, M::RING, DP);
+  else if (p.row_blocks > 1)
+    finish_row<T, TOK, true>(p, cur.b, cur.row, cur.s, row_ml, rings, M::RING, DP);
 }
 
 // CUDA-core form for fp32 caches and groups of at most 8 heads (G: the group
@@ -893,9 +1045,9 @@ struct SimtShape {
   static constexpr int STAGES = DP > 128 && G > 2 ? 2 : Tile<float, DP>::STAGE > 4096 ? 3 : 4;
   static constexpr int QBYTES = G * DP * 4;
   static constexpr int PBYTES = 8 * G * 4;
-  static constexpr int RING = (STAGES * Tile<float, DP>::STAGE + QBYTES + PBYTES + 1023) / 1024 * 1024;
+  static constexpr int RING = STAGES * Tile<float, DP>::STAGE, EXTRA = QBYTES + PBYTES;
   static constexpr int THREADS = PA_BLOCK_WORKERS * 32;
-  static_assert(PA_BLOCK_WORKERS * RING + 1024 + (2 * 2048 + 1) * 4 <= 227 * 1024, "shared memory of a block");
+  static_assert(PA_BLOCK_WORKERS * (RING + EXTRA) + 1024 + (2 * 2048 + 1) * 4 + 2 * 1024 <= 227 * 1024, "shared memory of a block");
 };
 
 __device__ __forceinline__ float4 lds128(uint32_t addr) {
@@ -918,44 +1070,81 @@ __global__ void __launch_bounds__(SimtShape<DP, G>::THREADS)
   constexpr int OV = CHUNKS / LANES;                // chunks of the result per lane
   extern __shared__ uint8_t pa_smem_raw[];
   __shared__ __align__(8) uint64_t all_bars[PA_BLOCK_WORKERS][STAGES];
+  __shared__ float2 row_ml[PA_BLOCK_WORKERS][PA_HEADS];
   const wgx_kv_cache &c = p.a.cache;
   const int lane = threadIdx.x % 32, worker = threadIdx.x / 32;
-  const BlockSmem sm = block_smem(pa_smem_raw, worker, M::RING, PA_BLOCK_WORKERS, c.batch);
+  const BlockSmem sm = block_smem(pa_smem_raw, worker, M::RING, M::EXTRA, PA_BLOCK_WORKERS, c.batch);
   uint64_t *bars = all_bars[worker];
   const int D = c.head_dim;
   if (lane == 0) {
     for (int s = 0; s < STAGES; ++s) mbar_init(smem_u32(&bars[s]), p.tma ? 1 : 32);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (D < DP) {
+  if (D < DP && !p.tma) {
     // chunks behind the rows' ends are read but never loaded
     for (int i = lane * 16; i < M::RING; i += 512)
       *reinterpret_cast<uint4 *>(sm.ring + i) = make_uint4(0u, 0u, 0u, 0u);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
+  if (p.tma && threadIdx.x == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&p.k_map) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&p.v_map) : "memory");
+  }
   wait_for_prior_kernel();
   let_dependents_launch();
-  build_prefix<TOK>(p, sm.prefix, sm.lens, p.scores != nullptr);  // (ends with a block barrier)
   const int rows = c.kv_heads;  // (p.chunks is 1)
-  const uint32_t total = sm.prefix[c.batch] * uint32_t(rows);
-  const uint32_t workers = worker_count(p, total);
-  const uint32_t me = uint32_t(worker) * gridDim.x + blockIdx.x;
-  if (total == 0 || me >= workers) return;
-  const Shares shares(total, workers);
-  const uint32_t begin = shares.begin(me), end = shares.begin(me + 1);
-
   Walk<TOK> cur;
-  cur.start(p, sm.prefix, sm.lens, rows, begin);
-  uint32_t to_do = end - begin;
+  uint32_t to_do, me = 0;
+  if (p.row_blocks) {
+    // this cluster's row, this block's part of it, a quarter of that per worker
+    const int unit = int(blockIdx.x) / p.row_blocks, rank = int(blockIdx.x) - unit * p.row_blocks;
+    cur.b = unit / rows;
+    cur.row = unit - cur.b * rows;
+    cur.s = span_of<TOK>(p, slots_in_use(p.a.lengths, cur.b, p.capacity, p.err));
+    // (steps * blocks * workers is small: row mode is for short tables)
+    const int lo = cur.s.steps * rank / p.row_blocks, hi = cur.s.steps * (rank + 1) / p.row_blocks;
+    cur.step = lo + (hi - lo) * worker / PA_BLOCK_WORKERS;
+    to_do = uint32_t(lo + (hi - lo) * (worker + 1) / PA_BLOCK_WORKERS - cur.step);
+    if (lane < PA_HEADS) row_ml[worker][lane] = make_float2(-INFINITY, 0.f);
+    __syncthreads();
+  } else {
+    build_prefix<TOK>(p, sm.prefix, sm.lens, p.scores != nullptr);  // (ends with a block barrier)
+    const uint32_t total = sm.prefix[c.batch] * uint32_t(rows);
+    const uint32_t workers = worker_count(p, total);
+    me = uint32_t(worker) * gridDim.x + blockIdx.x;
+    if (total == 0 || me >= workers) return;
+    const Shares shares(total, workers);
+    const uint32_t begin = shares.begin(me);
+    cur.start(p, sm.prefix, sm.lens, rows, begin);
+    to_do = shares.begin(me + 1) - begin;
+  }
   Loader<float, DP, STAGES> loader;
-  loader.start(p, cur, to_do, lane);
+  loader.to_load = 0;
+  const uint32_t ring_a = smem_u32(sm.ring);
+  const uint32_t q_a = smem_u32(sm.extra);              // [head][channel]
+  const uint32_t p_a = q_a + uint32_t(M::QBYTES);             // [slot][head]
+  float *p_s = reinterpret_cast<float *>(sm.extra + M::QBYTES);
+  // the queries of the row at hand, zeros behind the group and the channels
+  auto load_q = [&]() {
+    const float *q = static_cast<const float *>(p.a.q) + int64_t(cur.b) * p.a.q_batch_stride +
+                     int64_t(cur.row) * p.group * p.a.q_head_stride;
+    __syncwarp();
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+      for (int d = lane; d < DP; d += 32) {
+        const bool in = g < p.group && d < D;
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(q_a + uint32_t((g * DP + d) * 4)),
+                     "l"(in ? q + int64_t(g) * p.a.q_head_stride + d : q), "r"(in ? 4 : 0)
+                     : "memory");
+      }
+  };
+  if (to_do) {
+    load_q();  // (in flight beside the first steps' page table entries)
+    loader.start(p, cur, to_do, lane);
+  }
 #pragma unroll 1
   for (int s = 0; s < STAGES - 1; ++s) loader.next(p, sm.lens, rows, sm.ring, bars, s, lane, true);
 
-  const uint32_t ring_a = smem_u32(sm.ring);
-  const uint32_t q_a = ring_a + uint32_t(STAGES * L::STAGE), p_a = q_a + uint32_t(M::QBYTES);
-  float *q_s = reinterpret_cast<float *>(sm.ring + STAGES * L::STAGE);  // [head][channel]
-  float *p_s = q_s + G * DP;                                            // [slot][head]
   // scores: lane = quarter * 8 + slot, chunks 4 * i + quarter of the slot's row
   const int ks = lane & 7, quarter = lane >> 3;
   const uint32_t k0 = uint32_t(ks * 128 + ((quarter ^ ks) << 4));
@@ -971,21 +1160,15 @@ __global__ void __launch_bounds__(SimtShape<DP, G>::THREADS)
     const int nh = p.group;
     float m[G], l[G];
     float4 o[OV][G];
-    {
-      const float *q = static_cast<const float *>(p.a.q) + int64_t(cur.b) * p.a.q_batch_stride +
-                       int64_t(h) * nh * p.a.q_head_stride;
-      __syncwarp();
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        for (int d = lane; d < DP; d += 32)
-          q_s[g * DP + d] = g < nh && d < D ? q[int64_t(g) * p.a.q_head_stride + d] * p.scale2 : 0.f;
-        m[g] = -INFINITY;
-        l[g] = 0.f;
+    for (int g = 0; g < G; ++g) {
+      m[g] = -INFINITY;
+      l[g] = 0.f;
 #pragma unroll
-        for (int k = 0; k < OV; ++k) o[k][g] = make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-      __syncwarp();
+      for (int k = 0; k < OV; ++k) o[k][g] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncwarp();
     const uint32_t here = min(uint32_t(cur.s.steps - cur.step), to_do);
 #pragma unroll 1
     for (uint32_t i = 0; i < here; ++i) {
@@ -1034,7 +1217,7 @@ __global__ void __launch_bounds__(SimtShape<DP, G>::THREADS)
       for (int g = 0; g < G; ++g) {
         s[g] += __shfl_xor_sync(~0u, s[g], 8);
         s[g] += __shfl_xor_sync(~0u, s[g], 16);
-        s[g] = on ? s[g] : -INFINITY;
+        s[g] = on ? s[g] * p.scale2 : -INFINITY;
         mx[g] = fmaxf(s[g], __shfl_xor_sync(~0u, s[g], 1));
         mx[g] = fmaxf(mx[g], __shfl_xor_sync(~0u, mx[g], 2));
         mx[g] = fmaxf(mx[g], __shfl_xor_sync(~0u, mx[g], 4));
@@ -1108,6 +1291,7 @@ __global__ void __launch_bounds__(SimtShape<DP, G>::THREADS)
     }
     to_do -= here;
     const bool whole = from_begin && cur.step + int(here) == cur.s.steps;
+    if (p.row_blocks) __syncwarp();  // (the ring becomes the result's place)
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       float sum = l[g];
@@ -1122,8 +1306,9 @@ __global__ void __launch_bounds__(SimtShape<DP, G>::THREADS)
       }
       if (g >= nh || !ok) continue;
       const int64_t at = (int64_t(me) * 2 + (from_begin ? 1 : 0)) * p.heads + g;
-      const float inv = !whole ? 1.f : sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-      float *to = whole ? static_cast<float *>(p.a.out) + int64_t(cur.b) * p.a.out_batch_stride +
+      const float inv = p.row_blocks || !whole ? 1.f : sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+      float *to = p.row_blocks ? reinterpret_cast<float *>(sm.ring) + g * DP
+                  : whole ? static_cast<float *>(p.a.out) + int64_t(cur.b) * p.a.out_batch_stride +
                               int64_t(h * nh + g) * p.a.out_head_stride
                         : p.part_o + at * p.part_stride;
       if (half == 0) {
@@ -1137,13 +1322,21 @@ __global__ void __launch_bounds__(SimtShape<DP, G>::THREADS)
         }
       }
       if (lane == 0) {
-        if (!whole) p.part_ml[at] = make_float2(m[g], sum);
+        if (p.row_blocks) row_ml[worker][g] = make_float2(m[g], sum);
+        else if (!whole) p.part_ml[at] = make_float2(m[g], sum);
         else if (p.stats) p.stats[(int64_t(cur.b) * rows + cur.row) * PA_HEADS + g] = make_float2(m[g], sum);
       }
     }
+    if (p.row_blocks || !to_do) break;
     cur.next_row(p, sm.lens, rows);
+    load_q();
   }
   if (!ok) drain<STAGES>(loader.live_ring, bars, stage, phase);
+  uint8_t *rings = sm.ring - size_t(worker) * M::RING;
+  if (p.row_blocks == 1)
+    finish_row<float, TOK, false>(p, cur.b, cur.row, cur.s, row_ml, rings, M::RING, DP);
+  else if (p.row_blocks > 1)
+    finish_row<float, TOK, true>(p, cur.b, cur.row, cur.s, row_ml, rings, M::RING, DP);
 }
 
 __device__ __forceinline__ float warp_max(float x) {
@@ -1351,7 +1544,7 @@ template <typename T, int DP, bool HALF_ROWS>
 Config mma_config() {
   Config c{};
   c.kernel = paged_attention_kernel<T, DP, HALF_ROWS>;
-  c.ring = PA_BLOCK_WORKERS * MmaShape<T, DP>::RING + 1024;  // + alignment
+  c.ring = PA_BLOCK_WORKERS * (MmaShape<T, DP>::RING + MmaShape<T, DP>::EXTRA) + 1024;  // + alignment
   c.tok = Tile<T, DP>::TOK;
   c.threads = MmaShape<T, DP>::THREADS;
   return c;
@@ -1360,7 +1553,7 @@ template <int DP, int G>
 Config simt_config() {
   Config c{};
   c.kernel = paged_attention_simt_kernel<DP, G>;
-  c.ring = PA_BLOCK_WORKERS * SimtShape<DP, G>::RING + 1024;
+  c.ring = PA_BLOCK_WORKERS * (SimtShape<DP, G>::RING + SimtShape<DP, G>::EXTRA) + 1024;
   c.tok = 8;
   c.threads = SimtShape<DP, G>::THREADS;
   return c;
@@ -1437,16 +1630,25 @@ Layout layout_of(const wgx_paged_attention_args &a, bool for_launch) {
     p.tma = encode_rows_tmap(&p.k_map, c.k, c, c.k_page_stride, c.k_head_stride, c.k_slot_stride, panels, l.cfg->tok) &&
             encode_rows_tmap(&p.v_map, c.v, c, c.v_page_stride, c.v_head_stride, c.v_slot_stride, panels, l.cfg->tok);
   }
+  const int64_t rows = int64_t(c.batch) * c.kv_heads * p.chunks;
+  const int64_t row_steps = (p.capacity + l.cfg->tok - 1) / l.cfg->tok;
+  // Row mode where a row's table is short (see the constants). Blocks that share
+  // a K/V head's weights cannot accumulate them (chunks > 1).
+  const int per = c.head_dim > 128 ? PA_ROW_STEPS / 4 : l.cfg->tok == 16 ? PA_ROW_STEPS : PA_ROW_STEPS / 2;
+  if (p.chunks == 1 || !a.weights_out) {
+    const int64_t room = int64_t(device_sm_count()) * l.cfg->ctas_per_sm;
+    if (row_steps <= per) p.row_blocks = 1;
+    else if (rows >= PA_ROW_MIN && rows * 4 <= room && row_steps <= 4 * per) p.row_blocks = 4;
+    else if (rows >= PA_ROW_MIN && rows * 2 <= room && row_steps <= 2 * per) p.row_blocks = 2;
+  }
   p.min_steps = 1;
-  const uint64_t steps = uint64_t((p.capacity + l.cfg->tok - 1) / l.cfg->tok) * c.batch *
-                         uint64_t(c.kv_heads) * p.chunks;
+  const uint64_t steps = uint64_t(row_steps) * uint64_t(rows);
   if (steps >= uint64_t(1) << 31) fail("paged_attention: too many slots");
-  const uint64_t want = (steps + p.min_steps - 1) / p.min_steps;
   const int resident = device_sm_count() * l.cfg->ctas_per_sm;
-  p.max_workers = int(std::min<uint64_t>(std::max<uint64_t>(want, 1), uint64_t(resident) * PA_BLOCK_WORKERS));
-  l.grid = std::min(resident, p.max_workers);
+  p.max_workers = int(std::min<uint64_t>(std::max<uint64_t>(steps, 1), uint64_t(resident) * PA_BLOCK_WORKERS));
+  l.grid = p.row_blocks ? int(rows) * p.row_blocks : std::min(resident, p.max_workers);
   uint64_t off = 0;
-  const uint64_t parts = uint64_t(p.max_workers) * 2 * p.heads;
+  const uint64_t parts = p.row_blocks ? 0 : uint64_t(p.max_workers) * 2 * p.heads;
   auto take = [&](uint64_t bytes) {
     const uint64_t at = off;
     off += align256(bytes);
@@ -1486,8 +1688,9 @@ void launch_paged_attention(const wgx_paged_attention_args &a, cudaStream_t stre
   const int pre = prefix_bytes(c.batch);
   const int th = timer_begin("paged_attention_kernel", stream);
   launch_dependent(l.cfg->kernel, dim3(unsigned(l.grid)), l.cfg->threads, size_t(l.cfg->ring + pre), stream,
-                   "paged_attention launch", l.p);
+                   "paged_attention launch", l.p, l.p.row_blocks);
   timer_end(th, stream);
+  if (l.p.row_blocks) return;
   int64_t blocks = l.p.o_blocks;
   if (a.weights_out)
     blocks += int64_t(c.batch) * c.kv_heads * ((l.p.capacity + PA_JOIN_SLOTS - 1) / PA_JOIN_SLOTS);

@@ -510,21 +510,9 @@ void launch_cache_evict(const wgx_cache_evict_args &a, cudaStream_t stream) {
       if (dev < 64) set[dev] = true;
     }
   }
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(rows * S));
-  cfg.blockDim = dim3(EV_THREADS);
-  cfg.dynamicSmemBytes = size_t(p.chunk) * 6;
-  cfg.stream = stream;
-  cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = unsigned(S);
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 2;
   const int th = timer_begin("evict_kernel", stream);
-  check_cuda(cudaLaunchKernelEx(&cfg, evict_kernel, p), "cache_evict launch");
+  launch_dependent(evict_kernel, dim3(unsigned(rows * S)), EV_THREADS, size_t(p.chunk) * 6, stream,
+                   "cache_evict launch", p, S);
   timer_end(th, stream);
   if (!p.counters) {
     evict_lengths_kernel<<<unsigned(c.batch + 127) / 128, 128, 0, stream>>>(p);
