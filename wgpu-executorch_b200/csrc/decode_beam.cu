@@ -83,6 +83,17 @@ __device__ __forceinline__ void warp_sort(uint64_t &x, int &tag) {
       }
     }
 }
+__device__ __forceinline__ float warp_sort(float x) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int k = 2; k <= 32; k *= 2)
+#pragma unroll
+    for (int j = k / 2; j; j /= 2) {
+      const float y = __shfl_xor_sync(~0u, x, j);
+      x = ((lane & k) == 0) == ((lane & j) == 0) ? fmaxf(x, y) : fminf(x, y);
+    }
+  return x;
+}
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -294,7 +305,7 @@ __global__ void __launch_bounds__(BM_SEL_THREADS) select_kernel(const __grid_con
   const wgx_beam_search_args &a = p.a;
   __shared__ float row_max[WGX_MAX_BEAMS], row_log[WGX_MAX_BEAMS], row_score[WGX_MAX_BEAMS];
   __shared__ uint8_t row_done[WGX_MAX_BEAMS];
-  __shared__ float red[BM_SEL_THREADS / 32];
+  __shared__ float tops[BM_SEL_THREADS], bound;
   __shared__ Proposal cand[BM_CAND];
   __shared__ Proposal best[BM_SEL_THREADS / 32];
   __shared__ uint32_t n_cand;
@@ -356,31 +367,39 @@ __global__ void __launch_bounds__(BM_SEL_THREADS) select_kernel(const __grid_con
     if (q.total != q.total) q.total = -INFINITY;
     return true;
   };
-  // f(entry's place in its list, proposal) for this thread's proposals
+  // f(proposal) for this thread's proposals
   auto each = [&](auto &&f) {
 #pragma unroll
     for (int j = 0; j < BM_HELD; ++j) {
       const int i = tid + j * BM_SEL_THREADS;
       Proposal q;
-      if (i < all && propose(i, held_x[j], held_t[j], q)) f(i % W, q);
+      if (i < all && propose(i, held_x[j], held_t[j], q)) f(q);
     }
     for (int i = tid + BM_HELD * BM_SEL_THREADS; i < all; i += BM_SEL_THREADS) {
       Proposal q;
-      if (propose(i, p.top_x[first + i], p.top_t[first + i], q)) f(i % W, q);
+      if (propose(i, p.top_x[first + i], p.top_t[first + i], q)) f(q);
     }
   };
-  // ---- threshold: at least W proposals are not below the W-th entry of any
-  // one segment's list
-  float tau = -INFINITY;
-  each([&](int place, const Proposal &q) {
-    if (place == W - 1 && !row_done[q.beam]) tau = fmaxf(tau, q.total);
-  });
-  tau = warp_max(tau);
-  if (lane == 0) red[warp] = tau;
+  // ---- threshold: at least W proposals are not below the W-th largest of the
+  // threads' maxima, which are among the W first of their warps
+  float most = -INFINITY;
+  each([&](const Proposal &q) { most = fmaxf(most, q.total); });
+  most = warp_sort(most);
+  tops[tid] = most;
+  if (tid == 0) bound = -INFINITY;
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < BM_SEL_THREADS / 32; ++w) tau = fmaxf(tau, red[w]);
-  each([&](int, const Proposal &q) {
+  if (lane < W) {
+    int r = 0;
+    for (int o = 0; o < BM_SEL_THREADS / 32; ++o)
+      for (int j = 0; j < W; ++j) {
+        const float y = tops[o * 32 + j];
+        r += y > most || (y == most && o * 32 + j < tid);
+      }
+    if (r == W - 1) bound = most;
+  }
+  __syncthreads();
+  const float tau = bound;
+  each([&](const Proposal &q) {
     if (q.total >= tau) {
       const uint32_t at = atomicAdd(&n_cand, 1u);
       if (at < BM_CAND) cand[at] = q;
@@ -408,7 +427,7 @@ __global__ void __launch_bounds__(BM_SEL_THREADS) select_kernel(const __grid_con
     Proposal last{INFINITY, 0.f, -1, -1};
     for (int r = 0; r < W; ++r) {
       Proposal k{-INFINITY, -INFINITY, 0x7fffffff, 0x7fffffff};
-      each([&](int, const Proposal &q) {
+      each([&](const Proposal &q) {
         if ((r == 0 || before(last, q)) && before(q, k)) k = q;
       });
 #pragma unroll
