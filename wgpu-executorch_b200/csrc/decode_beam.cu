@@ -367,45 +367,51 @@ __global__ void __launch_bounds__(BM_SEL_THREADS) select_kernel(const __grid_con
     if (q.total != q.total) q.total = -INFINITY;
     return true;
   };
+  Proposal held[BM_HELD];  // beam -1: none
+#pragma unroll
+  for (int j = 0; j < BM_HELD; ++j) {
+    const int i = tid + j * BM_SEL_THREADS;
+    if (i >= all || !propose(i, held_x[j], held_t[j], held[j])) held[j].beam = -1;
+  }
   // f(proposal) for this thread's proposals
   auto each = [&](auto &&f) {
 #pragma unroll
-    for (int j = 0; j < BM_HELD; ++j) {
-      const int i = tid + j * BM_SEL_THREADS;
-      Proposal q;
-      if (i < all && propose(i, held_x[j], held_t[j], q)) f(q);
-    }
+    for (int j = 0; j < BM_HELD; ++j)
+      if (held[j].beam >= 0) f(held[j]);
     for (int i = tid + BM_HELD * BM_SEL_THREADS; i < all; i += BM_SEL_THREADS) {
       Proposal q;
       if (propose(i, p.top_x[first + i], p.top_t[first + i], q)) f(q);
     }
   };
   // ---- threshold: at least W proposals are not below the W-th largest of the
-  // threads' maxima, which are among the W first of their warps
-  float most = -INFINITY;
-  each([&](const Proposal &q) { most = fmaxf(most, q.total); });
-  most = warp_sort(most);
-  tops[tid] = most;
-  if (tid == 0) bound = -INFINITY;
-  __syncthreads();
-  if (lane < W) {
-    int r = 0;
-    for (int o = 0; o < BM_SEL_THREADS / 32; ++o)
-      for (int j = 0; j < W; ++j) {
-        const float y = tops[o * 32 + j];
-        r += y > most || (y == most && o * 32 + j < tid);
-      }
-    if (r == W - 1) bound = most;
-  }
-  __syncthreads();
-  const float tau = bound;
-  each([&](const Proposal &q) {
-    if (q.total >= tau) {
-      const uint32_t at = atomicAdd(&n_cand, 1u);
-      if (at < BM_CAND) cand[at] = q;
+  // threads' maxima, which are among the W first of their warps; those that
+  // pass are ranked by counting. (One beam: one maximum, below.)
+  if (W > 1) {
+    float most = -INFINITY;
+    each([&](const Proposal &q) { most = fmaxf(most, q.total); });
+    most = warp_sort(most);
+    tops[tid] = most;
+    if (tid == 0) bound = -INFINITY;
+    __syncthreads();
+    if (lane < W) {
+      int r = 0;
+      for (int o = 0; o < BM_SEL_THREADS / 32; ++o)
+        for (int j = 0; j < W; ++j) {
+          const float y = tops[o * 32 + j];
+          r += y > most || (y == most && o * 32 + j < tid);
+        }
+      if (r == W - 1) bound = most;
     }
-  });
-  __syncthreads();
+    __syncthreads();
+    const float tau = bound;
+    each([&](const Proposal &q) {
+      if (q.total >= tau) {
+        const uint32_t at = atomicAdd(&n_cand, 1u);
+        if (at < BM_CAND) cand[at] = q;
+      }
+    });
+    __syncthreads();
+  }
   auto emit = [&](int r, const Proposal &q) {
     const int64_t at = int64_t(b) * W + r;
     a.scores_out[at] = q.total;
@@ -414,7 +420,7 @@ __global__ void __launch_bounds__(BM_SEL_THREADS) select_kernel(const __grid_con
     a.finished_out[at] = row_done[q.beam] || q.token == a.eos;
   };
   const int n = int(n_cand);
-  if (n <= BM_CAND) {
+  if (W > 1 && n <= BM_CAND) {
     for (int i = tid; i < n; i += BM_SEL_THREADS) {
       const Proposal q = cand[i];
       int rank = 0;
@@ -422,8 +428,7 @@ __global__ void __launch_bounds__(BM_SEL_THREADS) select_kernel(const __grid_con
       if (rank < W) emit(rank, q);
     }
   } else {
-    // many equal totals (a single list's threshold can leave more): one
-    // maximum after another
+    // one beam, or many equal totals: one maximum after another
     Proposal last{INFINITY, 0.f, -1, -1};
     for (int r = 0; r < W; ++r) {
       Proposal k{-INFINITY, -INFINITY, 0x7fffffff, 0x7fffffff};
