@@ -203,6 +203,29 @@ def test_attention_mask(dec, dtype, kind):
     check_attention(dec, c, 6, mask=mask.astype(np.uint8) * 3, window=30)
 
 
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("window", [1, 8, 17, 64, 200])
+@pytest.mark.parametrize("lengths", [[40, 700, 16], [3000]])
+def test_attention_window_over_a_long_cache(dec, dtype, window, lengths):
+    """The window's slots only, whatever the table can name; weights in place:
+    the slots in front of the window stay as they are."""
+    c = Cache(lengths, 2, 64, 16, dtype)
+    check_attention(dec, c, 4, window=window)
+    check_attention(dec, c, 4, window=window, weights=True)
+    rng = np.random.default_rng(1)
+    q = rng.standard_normal((len(lengths), 4, 64)).astype(np.float16 if dtype == F16 else np.float32)
+    w = rng.random((len(lengths), 2, c.width * 16)).astype(np.float32)
+    dw = dev(w)
+    dec.paged_attention(dev(q), c.dk, c.dv, c.dtable, c.dlengths, window=window, weights=dw, weights_out=dw)
+    _, want = ref.paged_attention(q, c.k, c.v, c.table, c.lengths, 0.125, window, None, w)
+    got = host(dw)
+    for b, n in enumerate(lengths):
+        first = max(0, n - window)
+        np.testing.assert_array_equal(got[b, :, :first], w[b, :, :first])
+        np.testing.assert_allclose(got[b, :, first:n], want[b, :, first:n], rtol=1e-6, atol=8e-5)
+        np.testing.assert_array_equal(got[b, :, n:], w[b, :, n:])
+
+
 def test_attention_extreme_scores(dec):
     """Scores far apart (one slot takes all) and a scale of zero (all equal)."""
     for dtype in (F16, F32):

@@ -539,7 +539,8 @@ __device__ void finish_row(const AttnArgs &p, int b, int row, const Span &s, flo
   if (p.scores) {
     const int64_t at = (int64_t(b) * p.a.cache.kv_heads + h) * p.a.slots;
     const float *sc = p.scores + (int64_t(b) * p.a.q_heads + h * p.group) * p.score_stride;
-    const int t0 = rank ? (s.first + s.steps * rank / S) * TOK : 0;
+    const bool in_place = p.a.weights == p.a.weights_out;  // (slots in front of the window stay)
+    const int t0 = rank || in_place ? (s.first + s.steps * rank / S) * TOK : 0;
     const int t1 = min((s.first + s.steps * (rank + 1) / S) * TOK, int(min(int64_t(s.len), p.a.slots)));
     for (int t = t0 + tid; t < t1; t += int(blockDim.x)) {
       float w = p.a.weights[at + t];
@@ -1477,10 +1478,12 @@ __global__ void __launch_bounds__(PA_JOIN_THREADS) join_kernel(const __grid_cons
   }
 
   const int at_row = (int(blockIdx.x) - p.o_blocks) % (c.batch * c.kv_heads);
-  const int t0 = (int(blockIdx.x) - p.o_blocks) / (c.batch * c.kv_heads) * PA_JOIN_SLOTS;
+  const int slice = (int(blockIdx.x) - p.o_blocks) / (c.batch * c.kv_heads) * PA_JOIN_SLOTS;
   const int b = at_row / c.kv_heads, h = at_row % c.kv_heads;
   const Span s = span_of<TOK>(p, slots_in_use(p.a.lengths, b, p.capacity, p.err));
-  const int t1 = min(t0 + PA_JOIN_SLOTS, int(min(int64_t(s.len), p.a.slots)));
+  // (in place, slots in front of the window stay; first * TOK keeps quads aligned)
+  const int t0 = p.a.weights == p.a.weights_out ? max(slice, s.first * TOK) : slice;
+  const int t1 = min(slice + PA_JOIN_SLOTS, int(min(int64_t(s.len), p.a.slots)));
   if (t0 >= t1) return;
   wait_for_prior_kernel();
   let_dependents_launch();
@@ -1631,11 +1634,15 @@ Layout layout_of(const wgx_paged_attention_args &a, bool for_launch) {
             encode_rows_tmap(&p.v_map, c.v, c, c.v_page_stride, c.v_head_stride, c.v_slot_stride, panels, l.cfg->tok);
   }
   const int64_t rows = int64_t(c.batch) * c.kv_heads * p.chunks;
-  const int64_t row_steps = (p.capacity + l.cfg->tok - 1) / l.cfg->tok;
+  // steps a row can have: of the table's slots, or of the window (which may
+  // begin inside a step)
+  int64_t row_steps = (p.capacity + l.cfg->tok - 1) / l.cfg->tok;
+  if (a.window > 0) row_steps = std::min<int64_t>(row_steps, (int64_t(a.window) + l.cfg->tok - 1) / l.cfg->tok + 1);
   // Row mode where a row's table is short (see the constants). Blocks that share
-  // a K/V head's weights cannot accumulate them (chunks > 1).
+  // a K/V head's weights cannot accumulate them (chunks > 1), and one block would
+  // be long copying the weights in front of a window.
   const int per = c.head_dim > 128 ? PA_ROW_STEPS / 4 : l.cfg->tok == 16 ? PA_ROW_STEPS : PA_ROW_STEPS / 2;
-  if (p.chunks == 1 || !a.weights_out) {
+  if (!a.weights_out || (p.chunks == 1 && (a.weights == a.weights_out || p.capacity <= 4 * per * l.cfg->tok))) {
     const int64_t room = int64_t(device_sm_count()) * l.cfg->ctas_per_sm;
     if (row_steps <= per) p.row_blocks = 1;
     else if (rows >= PA_ROW_MIN && rows * 4 <= room && row_steps <= 4 * per) p.row_blocks = 4;
