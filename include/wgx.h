@@ -282,7 +282,9 @@ WGX_API int wgx_conv2d_noalloc(const wgx_conv2d_params *p, const void *in, const
  * Page ids and lengths are device data: a page id outside [0, pages), or a
  * length outside [0, table_width * page_size], is never followed; what it
  * names is left out and the device error word gets a bit, which the next
- * wgx_sync reports as WGX_ERR_DEVICE. */
+ * wgx_sync reports as WGX_ERR_DEVICE. Limits: head_dim <= 256, batch <= 65535,
+ * 2^30 slots per sequence. All calls enqueue on `stream` of the current device
+ * and return; scratch memory is in use until the enqueued work is done. */
 typedef struct wgx_kv_cache {
   void *k, *v;
   const int32_t *page_table; /* [batch][table_width] */
@@ -325,8 +327,10 @@ WGX_API int wgx_kv_append(const wgx_kv_append_args *a, void *stream);
  * [batch][kv_heads][slots], the probabilities are accumulated per slot:
  *   weights_out[b][h][j] = weights[b][h][j] + sum of the group's p_j
  * for j < lengths[b] (other slots are not written; may be the same array).
- * Scores, softmax and sums are fp32, one rounding at the end. scratch:
- * wgx_paged_attention_scratch_bytes() (its contents need no preparation). */
+ * Scores, softmax and sums are fp32, one rounding at the end; the same inputs
+ * give the same bits. scratch: wgx_paged_attention_scratch_bytes(), 256-byte
+ * aligned (its contents need no preparation). Limits: batch <= 2048, 128 query
+ * heads per K/V head, weights over 2^25 slots. */
 typedef struct wgx_paged_attention_args {
   wgx_kv_cache cache;
   const void *q; /* [batch][q_heads][head_dim] */
@@ -355,7 +359,8 @@ WGX_API int wgx_paged_attention(const wgx_paged_attention_args *a, void *stream)
  * moves, so slot order is not token order: positions say which token a slot
  * holds. weights_out / positions_out (may be the inputs) are written for the
  * slots that remain; lengths_out[b] = min(lengths[b], budget) (may be
- * lengths). Sequences must not share the pages that are written. */
+ * lengths). Sequences must not share the pages that are written. Limit: 262144
+ * slots per sequence. */
 typedef struct wgx_cache_evict_args {
   wgx_kv_cache cache;
   const int32_t *lengths;
@@ -383,7 +388,9 @@ WGX_API int wgx_cache_evict(const wgx_cache_evict_args *a, void *stream);
  * takes its parent's page table (full pages are shared) and length, and the
  * used slots of a partly filled last page are copied, in every layer, into
  * the child's page spare[sequence], which takes that page's place. Spare
- * pages must be in no table; outputs must not overlap inputs. */
+ * pages must be in no table; outputs must not overlap inputs. scratch:
+ * wgx_beam_search_scratch_bytes(), 256-byte aligned. Limits: 32 beams, batch *
+ * beams <= 65535, vocab <= 2^24. */
 typedef struct wgx_beam_search_args {
   wgx_kv_cache cache;
   const void *logits; /* [batch][beams][vocab] */

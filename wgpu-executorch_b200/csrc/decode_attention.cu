@@ -6,24 +6,36 @@
 // Every cached byte is read once and used for 2 * group multiply-adds per
 // element, so the cache's bytes over the HBM rate are the floor. The work is
 // split over the cache's length: a step is TOK slots of one (sequence, K/V
-// head), all steps of the batch stand in one line, and every warp of the grid
-// takes an equal, contiguous share of it, whatever the lengths are. A warp
-// streams its steps through a ring of its own in shared memory (cp.async,
-// rows of slots that are not live are zero-filled instead of read: stale
-// infinities and NaN of a page cannot reach a product), so no block barrier
-// stands between loads and products. The softmax is the running one: maximum
-// and sum in fp32 per head, the result rescaled when the maximum grows.
+// head), all steps of the batch stand in one line, and every worker (a warp; two
+// above 128 channels) of the grid takes an equal, contiguous share of it,
+// whatever the lengths are. A worker streams its steps through a ring of its own
+// in shared memory, so no block barrier stands between loads and products:
+// where a step's rows lie in one page they come by TMA (one copy per operand
+// and step, any strides), elsewhere by 16-byte cp.async or element by element.
+// The V rows of slots that are not live are cleared in shared memory: stale
+// infinities and NaN of a page must not reach a product. The softmax is the
+// running one: a reference value and the sum in fp32 per head, the result
+// rescaled when the maximum has grown by more than 2^8.
 //
 // The group's heads are the 16 rows of an mma.sync tile (M = heads, N = slots
 // for the scores, N = channels for the result). tcgen05 would need 64 or 128
-// rows; a decode step has at most a group of them, and its time is the
-// loads'. fp16: m16n8k16, exact products, fp32 sums. fp32: m16n8k8 tf32 with
-// every operand split into a tf32 head and the fp32 tail (3 products).
+// rows; a decode step has at most a group of them, and its time is the loads'.
+// fp16: m16n8k16, exact products, fp32 sums. fp32: CUDA cores for groups of at
+// most 8 heads, above that m16n8k8 tf32 with every operand split in two.
 //
-// A row of work that lies within one warp's share is finished by it. Rows cut
-// by a share's end leave (max, sum, unnormalised result) in scratch, at most
-// two per warp, and join_kernel combines them; it also accumulates the
-// probabilities per slot from the scores, kept in scratch for it.
+// A row of work that lies within one worker's share is finished by it. Rows cut
+// by a share's end leave (reference, sum, unnormalised result) in scratch, at
+// most two per worker, and join_kernel combines them; it also accumulates the
+// probabilities per slot from the scores, kept in scratch for it. Short rows
+// are not cut: row mode (below) joins them in shared memory.
+//
+// Measured (fp16, K and V bytes over the time of the kernel, then the whole
+// call): 8 K/V heads x 128 channels, 131071 slots: 84.5 us, 6.35 TB/s, call 97
+// us; 64 sequences of 17-8192 slots with weights: 190 us, 5.7 TB/s, call 207;
+// 48 sequences of one head of 256 channels x 16, 4096 slots each: steps run at
+// 6.4 TB/s, but start, cut rows and join are 20 us of the call's 52. What is
+// left is the chain lengths -> page table -> rows at the start (about 4 us)
+// and the join (5 us).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -552,7 +564,10 @@ __device__ void finish_row(const AttnArgs &p, int b, int row, const Span &s, flo
   if constexpr (CLUSTER) cluster.sync();  // a block's results are read by the others until here
 }
 
-// Tensor-core form: the worker's heads are the 16 rows of an mma tile.
+// Tensor-core form: the worker's heads are the 16 rows of an mma tile. A step of
+// 16 slots costs a warp about 48 mma of 128 channels and as many other
+// instructions; with operand addresses computed in full it was 450 instructions
+// and the kernel issue-bound (101 instead of 84.5 us at 131071 slots).
 // HALF_ROWS: at most 8 heads (rows 8-15 are padding and their softmax is left
 // out). Heads of 256 channels: two warps share a worker, each with half of the
 // channels: the halves of the scores are added through shared memory (one
@@ -1039,8 +1054,11 @@ __global__ void __launch_bounds__(MmaShape<T, DP>::THREADS)
 // CUDA-core form for fp32 caches and groups of at most 8 heads (G: the group
 // rounded up to 1, 2, 4, 8): 2 * G multiply-adds per cached element, exact
 // products. On the tensor cores a step of 8 slots costs the same whatever the
-// group (about 450 instructions and the operands' splitting); here 80 * G and
-// about 100 more.
+// group (about 450 instructions, most of them the operands' splitting); here
+// about 100 and 64 * G more at 128 channels. 12 sequences of 129-2001 slots x 5
+// heads x 80 channels, 2 query heads each: 23.5 us on the tensor cores, 19 here
+// (34 MB; the rest is latency: six steps per worker). 116 sequences x 2 heads x
+// 128 channels, 762-1525 slots: 52 us a call, 5.2 TB/s.
 template <int DP, int G>
 struct SimtShape {
   static constexpr int STAGES = DP > 128 && G > 2 ? 2 : Tile<float, DP>::STAGE > 4096 ? 3 : 4;

