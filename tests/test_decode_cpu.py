@@ -66,6 +66,9 @@ def test_cache_checks(op):
     refuse(op, "head size", head_dim=0)
     refuse(op, "head size", head_dim=257)
     refuse(op, "2\\^30 slots", page_size=1 << 20, table_width=1 << 20)
+    refuse(op, "2\\^27 sequences", batch=60000, kv_heads=60000)
+    refuse(op, "extents too large", page_size=1 << 29, table_width=1)
+    refuse(op, "extents too large", layers=1 << 30)
 
 
 def test_append_checks():
@@ -89,6 +92,7 @@ def test_attention_checks():
     refuse("attention", "come together", weights=4, slots=64)
     refuse("attention", "cover every slot", weights=4, weights_out=4, slots=63)
     refuse("attention", "mask width", mask=4, mask_width=-1)
+    refuse("attention", "2\\^30 sequences", batch=2048, kv_heads=5000, q_heads=128 * 5000)
     refuse("attention", "2\\^33 slots", batch=2048, page_size=1 << 20, table_width=8)
     refuse("attention", "2\\^25 slots", weights=4, weights_out=4, slots=1 << 40, page_size=1 << 20, table_width=64)
 

@@ -47,8 +47,7 @@ __global__ void __launch_bounds__(AP_THREADS, 3) append_kernel(const __grid_cons
   const int b = blockIdx.y;
   const int units = c.head_dim / STEP, all = c.kv_heads * units;  // of a row, of a token
   const int per = max(1, AP_THREADS / all);                       // tokens side by side
-  const int sub = int(threadIdx.x) / all < per ? int(threadIdx.x) / all : a.tokens;  // (or idle)
-  const int first = per > 1 ? int(threadIdx.x) - sub * all : int(threadIdx.x);
+  const int sub = int(threadIdx.x) / all, first = sub < per ? int(threadIdx.x) - sub * all : all;  // (or idle)
   wait_for_prior_kernel();
   let_dependents_launch();
   const int len = slots_in_use(a.lengths, b, p.capacity, p.err);

@@ -41,6 +41,11 @@ void check_cache(const wgx_kv_cache &c, const char *op) {
   need(c.kv_heads <= 65535, op, "at most 65535 K/V heads");
   need(c.head_dim >= 1 && c.head_dim <= 256, op, "head size must be in [1, 256]");
   need(cache_capacity(c) <= kMaxSlots, op, "page table names more than 2^30 slots");
+  // kernels count rows, and elements of a page's row of heads, in 32 bits
+  need(int64_t(c.batch) * c.kv_heads <= int64_t(1) << 27, op, "more than 2^27 sequences x K/V heads");
+  need(int64_t(c.page_size) * c.head_dim <= int64_t(1) << 30 &&
+           int64_t(c.layers) * c.kv_heads <= int64_t(1) << 30,
+       op, "cache extents too large");
 }
 
 void check_append(const wgx_kv_append_args *a) {
@@ -70,6 +75,7 @@ void check_attention(const wgx_paged_attention_args *a) {
        "query heads must be a multiple of the K/V heads");
   need(a->q_heads / c.kv_heads <= 128, op, "at most 128 query heads per K/V head");
   need(cache_capacity(c) * c.batch <= int64_t(1) << 33, op, "page tables name more than 2^33 slots");
+  need(int64_t(c.batch) * a->q_heads <= int64_t(1) << 30, op, "more than 2^30 sequences x query heads");
   need(a->window >= 0, op, "window must not be negative");
   need(a->scale == a->scale, op, "scale is NaN");
   need(!a->mask || a->mask_width >= 0, op, "mask width must not be negative");
