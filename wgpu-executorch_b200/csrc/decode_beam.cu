@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(BM_THREADS, BM_BLOCKS_PER_SM) scan_kernel(cons
   const int row = blockIdx.y, seg = blockIdx.x, tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   wait_for_prior_kernel();
   let_dependents_launch();
-  if (a.finished[row]) return;  // proposes eos: its logits are not needed
+  const bool done = a.finished[row];
   const int K = a.beams;
   const T *x = static_cast<const T *>(a.logits) + int64_t(row / K) * a.logits_batch_stride +
                int64_t(row % K) * a.logits_beam_stride;
@@ -161,7 +161,8 @@ __global__ void __launch_bounds__(BM_THREADS, BM_BLOCKS_PER_SM) scan_kernel(cons
   float m = -INFINITY, sum = 0.f;  // of this thread
   int top_tile = tile0;            // the first tile with its maximum
   Raw next;
-  load(tile0, next);
+  load(tile0, next);   // (beside the load of `done`)
+  if (done) return;    // proposes eos: its logits are not needed
 #pragma unroll 1
   for (int tile = tile0; tile < tile1; ++tile) {
     float v[BM_ITEMS];
@@ -189,7 +190,7 @@ __global__ void __launch_bounds__(BM_THREADS, BM_BLOCKS_PER_SM) scan_kernel(cons
   // ---- this thread's largest key: the first token with its maximum
   uint64_t top = 0;
   {
-    load(top_tile, next);
+    if (top_tile != tile1 - 1) load(top_tile, next);  // (the last one is still here)
     const int t0 = top_tile * BM_TILE;
 #pragma unroll
     for (int i = BM_ITEMS - 1; i >= 0; --i) {
