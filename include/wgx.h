@@ -282,7 +282,9 @@ WGX_API int wgx_conv2d_noalloc(const wgx_conv2d_params *p, const void *in, const
  * Page ids and lengths are device data: a page id outside [0, pages), or a
  * length outside [0, table_width * page_size], is never followed; what it
  * names is left out and the device error word gets a bit, which the next
- * wgx_sync reports as WGX_ERR_DEVICE. Limits: head_dim <= 256, batch <= 65535,
+ * wgx_sync reports as WGX_ERR_DEVICE. Of such a length wgx_paged_attention
+ * reads the slots that the table has; the calls that write leave the sequence
+ * as it is and hand its length on unchanged. Limits: head_dim <= 256, batch <= 65535,
  * 2^30 slots per sequence. All calls enqueue on `stream` of the current device
  * and return; scratch memory is in use until the enqueued work is done. */
 typedef struct wgx_kv_cache {
@@ -300,7 +302,8 @@ typedef struct wgx_kv_cache {
  * same array). Optional (NULL): weights, positions [batch][kv_heads][slots]
  * dense: 0 and seen[b] + t are written at the new slots, and seen_out[b] =
  * seen[b] + tokens (may be the same array). A sequence whose table has no
- * room for all of the tokens gets none and keeps its length (error word). */
+ * room for all of the tokens gets none and keeps its length (error word), and
+ * so does one whose length is negative. */
 typedef struct wgx_kv_append_args {
   wgx_kv_cache cache;
   const void *k, *v; /* [batch][tokens][kv_heads][head_dim] */

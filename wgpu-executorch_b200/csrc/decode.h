@@ -79,12 +79,19 @@ void launch_dependent(void (*kernel)(P), dim3 grid, int threads, size_t smem, cu
   check_cuda(cudaLaunchKernelEx(&cfg, kernel, arg), what);
 }
 
-// Slots in use of sequence b, held within [0, capacity].
+// Whether n is a length that a table of so many slots can have; noted where not.
+// The operators that write leave a sequence of another length as it is: what
+// its table names may be other sequences' rows.
+__device__ __forceinline__ bool valid_length(int n, int64_t capacity, uint32_t *err) {
+  if (n >= 0 && n <= capacity) return true;
+  atomicOr(err, kErrCache);
+  return false;
+}
+// Slots in use of sequence b, held within [0, capacity] (for reading).
 __device__ __forceinline__ int slots_in_use(const int32_t *lengths, int b, int64_t capacity,
                                             uint32_t *err) {
   const int n = lengths[b];
-  if (n >= 0 && n <= capacity) return n;
-  atomicOr(err, kErrCache);
+  if (valid_length(n, capacity, err)) return n;
   return n < 0 ? 0 : int(capacity);
 }
 #endif

@@ -475,8 +475,10 @@ __global__ void __launch_bounds__(BM_COPY_THREADS) reorder_kernel(const __grid_c
   wait_for_prior_kernel();
   let_dependents_launch();
   const int from = child / a.beams * a.beams + a.parents[child];
-  const int len = slots_in_use(a.lengths, from, p.capacity, p.err);
-  const int full = len / c.page_size, tail = len - full * c.page_size;
+  const int len = a.lengths[from];
+  // (a length the table cannot have is handed on as it is, with nothing copied)
+  const int used = valid_length(len, p.capacity, p.err) ? len : 0;
+  const int full = used / c.page_size, tail = used - full * c.page_size;
   const int32_t *src_table = c.page_table + int64_t(from) * c.table_stride;
   if (blockIdx.x == 0) {
     int32_t *dst = a.page_table_out + int64_t(child) * c.table_width;

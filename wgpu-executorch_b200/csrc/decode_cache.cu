@@ -27,6 +27,11 @@ struct AppendArgs {
   uint32_t *err;
 };
 
+// Whether the new tokens of a sequence of `len` slots are written. A length that
+// the table cannot have (a negative one too) is no place to write behind.
+__device__ __forceinline__ bool fits_behind(const wgx_kv_append_args &a, int len, int64_t capacity) {
+  return len >= 0 && int64_t(len) + a.tokens <= capacity;
+}
 // The counters of sequence b (lengths_out may be lengths).
 __device__ __forceinline__ void advance(const wgx_kv_append_args &a, int b, int len, int seen, bool fits) {
   a.lengths_out[b] = len + (fits ? a.tokens : 0);
@@ -50,9 +55,9 @@ __global__ void __launch_bounds__(AP_THREADS, 3) append_kernel(const __grid_cons
   const int sub = int(threadIdx.x) / all, first = sub < per ? int(threadIdx.x) - sub * all : all;  // (or idle)
   wait_for_prior_kernel();
   let_dependents_launch();
-  const int len = slots_in_use(a.lengths, b, p.capacity, p.err);
+  const int len = a.lengths[b];
   const int seen = a.seen ? a.seen[b] : 0;
-  const bool fits = int64_t(len) + a.tokens <= p.capacity;
+  const bool fits = fits_behind(a, len, p.capacity);
   if (!fits && threadIdx.x == 0 && blockIdx.x == 0) atomicOr(p.err, kErrCache);
   const int t0 = int(blockIdx.x) * p.block_tokens, t1 = min(t0 + p.block_tokens, a.tokens);
   if (fits) {
@@ -108,8 +113,8 @@ __global__ void __launch_bounds__(AP_THREADS, 3) append_kernel(const __grid_cons
 __global__ void advance_kernel(const __grid_constant__ AppendArgs p) {
   const int b = blockIdx.x * blockDim.x + threadIdx.x;
   if (b >= p.a.cache.batch) return;
-  const int len = slots_in_use(p.a.lengths, b, p.capacity, p.err);
-  advance(p.a, b, len, p.a.seen ? p.a.seen[b] : 0, int64_t(len) + p.a.tokens <= p.capacity);
+  const int len = p.a.lengths[b];
+  advance(p.a, b, len, p.a.seen ? p.a.seen[b] : 0, fits_behind(p.a, len, p.capacity));
 }
 
 // ------------------------------------------------------------------- evict
@@ -199,11 +204,12 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const __grid_const
   if (tid == 0) counts[0] = 0;
   wait_for_prior_kernel();
   let_dependents_launch();
-  const int len = slots_in_use(a.lengths, b, p.capacity, p.err);
+  const int len = a.lengths[b];
+  const bool valid = valid_length(len, p.capacity, p.err);
   const int recent_from = a.seen[b] - a.recent;
-  const int n = int(min(int64_t(len), a.slots));
+  const int n = valid ? len : 0;  // (a.slots >= capacity)
   const int64_t at = int64_t(row) * a.slots;
-  if (p.counters && h == 0 && rank == 0 && tid == 0) a.lengths_out[b] = min(len, C);
+  if (p.counters && h == 0 && rank == 0 && tid == 0) a.lengths_out[b] = valid ? min(len, C) : len;
   if (n <= C) {  // the same for the whole cluster
     for (int i = rank * EV_THREADS + tid; i < n; i += S * EV_THREADS) {
       if (a.weights_out != a.weights) a.weights_out[at + i] = a.weights[at + i];
@@ -447,7 +453,8 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const __grid_const
 __global__ void evict_lengths_kernel(const __grid_constant__ EvictArgs p) {
   const int b = blockIdx.x * blockDim.x + threadIdx.x;
   if (b >= p.a.cache.batch) return;
-  p.a.lengths_out[b] = min(slots_in_use(p.a.lengths, b, p.capacity, p.err), p.a.budget);
+  const int len = p.a.lengths[b];
+  if (valid_length(len, p.capacity, p.err)) p.a.lengths_out[b] = min(len, p.a.budget);
 }
 
 }  // namespace
