@@ -362,8 +362,9 @@ WGX_API int wgx_paged_attention(const wgx_paged_attention_args *a, void *stream)
  * moves, so slot order is not token order: positions say which token a slot
  * holds. weights_out / positions_out (may be the inputs) are written for the
  * slots that remain; lengths_out[b] = min(lengths[b], budget) (may be
- * lengths). Sequences must not share the pages that are written. Limit: 262144
- * slots per sequence. */
+ * lengths). Where a row cannot move (a page id outside the pool), its weight and
+ * position do not either: the free slot keeps its own. Sequences must not share
+ * the pages that are written. Limit: 262144 slots per sequence. */
 typedef struct wgx_cache_evict_args {
   wgx_kv_cache cache;
   const int32_t *lengths;

@@ -97,3 +97,35 @@ def test_beams_of_invalid_length_copy_nothing_and_keep_it(dec, bad):  # noqa: F8
     np.testing.assert_array_equal(host(c.dk), k0)
     np.testing.assert_array_equal(host(c.dv), v0)
     assert dec.device_error(0) == 32
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("bad", ["source", "destination"])
+def test_evict_moves_a_slots_label_only_with_its_row(dec, in_place, bad):  # noqa: F811
+    """A page id outside the pool: the rows of that page do not move, so
+    neither do their weights and positions; every other pair moves."""
+    H, D, page, n, budget = 1, 16, 16, 64, 32
+    c = Cache([n], H, D, page, F16, seed=5)
+    table = c.table.copy()
+    entry = 3 if bad == "source" else 0
+    table[0, entry] = c.k.shape[0]
+    rng = np.random.default_rng(2)
+    w = rng.random((1, H, c.width * page)).astype(np.float32)
+    pos = np.arange(c.width * page, dtype=np.int32)[None, None]
+    dw, dp, dl = dev(w), dev(pos), c.dlengths
+    wo, po, lo = (dw, dp, dl) if in_place else (torch.full_like(dw, -9.0), torch.full_like(dp, -9),
+                                                torch.full_like(dl, -9))
+    dec.cache_evict(c.dk, c.dv, dev(table), dl, lo, dw, wo, dp, po, dev(np.array([n], np.int32)), budget=budget)
+    _, moves = ref.evict_plan(w[0, 0], pos[0, 0], n, n, budget, 0, 0)
+    done = [(d, s) for d, s in moves if entry not in (d // page, s // page)]
+    assert 0 < len(done) < len(moves)
+    ww, pw = w[0, 0].copy(), pos[0, 0].copy()
+    for d, s in done:
+        for x in (c.k, c.v):
+            ref.slot_row(x, c.table, 0, 0, d)[:] = ref.slot_row(x, c.table, 0, 0, s)
+        ww[d], pw[d] = ww[s], pw[s]
+    np.testing.assert_array_equal(host(c.dk), c.k)
+    np.testing.assert_array_equal(host(c.dv), c.v)
+    np.testing.assert_array_equal(host(wo)[0, 0, :budget], ww[:budget])
+    np.testing.assert_array_equal(host(po)[0, 0, :budget], pw[:budget])
+    assert host(lo).tolist() == [budget] and dec.device_error(0) == 32

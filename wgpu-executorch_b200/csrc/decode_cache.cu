@@ -388,12 +388,13 @@ __global__ void __launch_bounds__(EV_THREADS, 2) evict_kernel(const __grid_const
       const int rsplit = max(0, min(C - r * per, min(per, n - r * per)));
       const int src =
           r * per + of(list, r)[rsplit + (j - (r ? mover_end[r - 1] : 0))];
-      a.weights_out[at + dst] = a.weights[at + src];
-      a.positions_out[at + dst] = a.positions[at + src];
       const int dp = dst / c.page_size, sp = src / c.page_size;
       const int dpage = c.page_table[int64_t(b) * c.table_stride + dp];
       const int spage = c.page_table[int64_t(b) * c.table_stride + sp];
       if (dpage >= 0 && dpage < c.pages && spage >= 0 && spage < c.pages) {
+        // (a slot's weight and position move with its row only)
+        a.weights_out[at + dst] = a.weights[at + src];
+        a.positions_out[at + dst] = a.positions[at + src];
         kd = (int64_t(dpage) * c.k_page_stride + int64_t(h) * c.k_head_stride +
               int64_t(dst - dp * c.page_size) * c.k_slot_stride) * es;
         ks = (int64_t(spage) * c.k_page_stride + int64_t(h) * c.k_head_stride +
