@@ -330,10 +330,15 @@ WGX_API int wgx_kv_append(const wgx_kv_append_args *a, void *stream);
  * [batch][kv_heads][slots], the probabilities are accumulated per slot:
  *   weights_out[b][h][j] = weights[b][h][j] + sum of the group's p_j
  * for j < lengths[b] (other slots are not written; may be the same array).
- * Scores, softmax and sums are fp32, one rounding at the end; the same inputs
- * give the same bits. scratch: wgx_paged_attention_scratch_bytes(), 256-byte
- * aligned (its contents need no preparation). Limits: batch <= 2048, 128 query
- * heads per K/V head, weights over 2^25 slots. */
+ * Scores, their maximum and all sums are fp32, with one rounding at the end.
+ * Fewer bits are in: the exponentials (2^-22 of themselves); fp16's probabilities
+ * in the product with V (2^-22 of themselves, or 2^-26 of the largest among 16
+ * neighbouring slots); fp32 products where a K/V head has more than 8 query heads
+ * (operands to 2^-22). A live slot's NaN makes the results that it enters NaN,
+ * and an infinite K or V may. The same inputs give the same bits. scratch:
+ * wgx_paged_attention_scratch_bytes(), 256-byte aligned (its contents need no
+ * preparation). Limits: batch <= 2048, 128 query heads per K/V head, weights
+ * over 2^25 slots. */
 typedef struct wgx_paged_attention_args {
   wgx_kv_cache cache;
   const void *q; /* [batch][q_heads][head_dim] */

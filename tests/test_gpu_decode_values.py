@@ -1,0 +1,78 @@
+"""What paged_attention's result and accumulated weights hold where scores are
+far apart or not finite.
+
+A row with one slot (a "sink", value zero) far above all others: its result is
+the others' small probabilities times their values. Tolerance, relative to
+that result, derived before the first run: probabilities of a step (16 slots)
+enter the product to 2^-21 of themselves, or of the step's largest by 2^-25
+where they are smaller; scores of up to 50 (base 2) are off by 2^-23 of
+themselves, exp2 by 2^-22: below 1e-5 in all. The sums are fp32, which a tensor
+core may cut instead of round: at most two additions per step of 16 slots, each
+by 2^-23, below 2^-12 for the 16384 slots here. The up to 15 slots that share a
+step with the sink are held to 2^-36 of the sink's probability. fp16's output
+adds half a unit: 2^-11, or 2^-25 absolutely below its normal range."""
+import numpy as np
+import pytest
+import torch
+
+import decode_reference as ref
+from test_gpu_decode import F16, F32, Cache, dec, dev, host  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def sink_rows(n, gap, D, H, G, dtype, at, rng):
+    """(q, k, v): scores are `gap` nats for slot `at` and 0 for the others,
+    with scale 1 (exact in fp16: the gap is a product of two numbers)."""
+    npdt = np.float16 if dtype == F16 else np.float32
+    k = np.zeros((n, D), npdt)
+    k[at, 0] = 1
+    q = np.zeros((H * G, D), npdt)
+    q[:, 0] = gap
+    v = (rng.random((n, D)) + 0.5).astype(npdt)
+    v[at] = 0
+    return q, k, v
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("n,rows", [(300, 8), (4096, 1300), (16384, 1300), (16384, 2)])
+@pytest.mark.parametrize("gap", [10, 14, 16, 17, 18, 20, 23])
+@pytest.mark.parametrize("D,G", [(64, 1), (128, 4), (128, 12), (256, 16)])
+def test_attention_keeps_the_tail_of_a_peaked_row(dec, dtype, n, rows, gap, D, G):  # noqa: F811
+    """All sequences read the same pages, so that thousands of slots of a row
+    lie in one warp's share without a large cache."""
+    page, B = 16, rows
+    rng = np.random.default_rng(gap)
+    at = {300: 0, 4096: 37, 16384: 16383 if rows > 2 else 8000}[n]
+    q, k, v = sink_rows(n, gap, D, 1, G, dtype, at, rng)
+    pages = -(-n // page)
+    pool = lambda x: dev(np.pad(x, ((0, pages * page - n), (0, 0))).reshape(pages, 1, page, D))  # noqa: E731
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None].expand(B, pages)
+    size = 1000.0  # values of this size: results stay far above fp16's smallest numbers
+    out = dec.paged_attention(dev(q)[None].expand(B, G, D), pool(k), pool((v * size).astype(v.dtype)), table,
+                              torch.full((B,), n, dtype=torch.int32, device="cuda"), scale=1.0)
+    p = np.where(np.arange(n) == at, 1.0, np.exp(-float(gap)))
+    vv = (v * size).astype(v.dtype).astype(np.float64)
+    want = (p / p.sum()) @ vv
+    got = out.double().cpu().numpy()
+    tol = want * (1e-5 + 2.0 ** -12 + (2.0 ** -11 if dtype == F16 else 0)) + 15 * 2.0 ** -36 * vv.max() + \
+        (2.0 ** -25 if dtype == F16 else 0)
+    assert (np.abs(got - want) <= tol).all(), np.abs(got / want - 1).max()
+    assert dec.device_error(0) == 0
+
+
+@pytest.mark.parametrize("n", [4096, 16384, 131072])
+@pytest.mark.parametrize("D,G", [(64, 1), (128, 4), (256, 16)])
+def test_attention_of_equal_values_is_that_value(dec, n, D, G):  # noqa: F811
+    """Every value 1: the result is 1 to within fp16's rounding, however many
+    slots one warp adds up (sums cut by the tensor core would fall short)."""
+    B, page = 1300, 64
+    pages = n // page
+    k = torch.randn(pages, 1, page, D, device="cuda").half()
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None].expand(B, pages)
+    q = torch.randn(B, G, D, device="cuda").half()
+    out = dec.paged_attention(q, k, torch.ones_like(k), table,
+                              torch.full((B,), n, dtype=torch.int32, device="cuda"))
+    assert float((out.float() - 1).abs().max()) <= 2.0 ** -11
+
+

@@ -15,12 +15,14 @@
 // The V rows of slots that are not live are cleared in shared memory: stale
 // infinities and NaN of a page must not reach a product. The softmax is the
 // running one: a reference value and the sum in fp32 per head, the result
-// rescaled when the maximum has grown by more than 2^8.
+// rescaled when a step's scores lie too far from the reference (a few powers of
+// two above it, and in fp16 also below it).
 //
 // The group's heads are the 16 rows of an mma.sync tile (M = heads, N = slots
 // for the scores, N = channels for the result). tcgen05 would need 64 or 128
 // rows; a decode step has at most a group of them, and its time is the loads'.
-// fp16: m16n8k16, exact products, fp32 sums. fp32: CUDA cores for groups of at
+// fp16: m16n8k16, exact products of scores, probabilities as a sum of two fp16
+// numbers, fp32 sums. fp32: CUDA cores for groups of at
 // most 8 heads, above that m16n8k8 tf32 with every operand split in two.
 //
 // A row of work that lies within one worker's share is finished by it. Rows cut
@@ -66,6 +68,11 @@ constexpr int PA_MAX_GROUP = 128;   // query heads per K/V head
 constexpr int PA_ROW_STEPS = 16;
 constexpr int PA_ROW_CLUSTER = 4;
 constexpr int PA_ROW_MIN = 8;  // rows from which clusters are used
+// fp16 probabilities (see the running softmax), in powers of two: the reference
+// value is set PA_ABOVE below a step's maximum, and again when a step's maximum
+// is not within PA_FAR of PA_MIDDLE above it; never PA_DEPTH below the highest
+// that it has been.
+constexpr float PA_ABOVE = 11.f, PA_MIDDLE = 8.f, PA_FAR = 7.f, PA_DEPTH = 60.f;
 constexpr int PA_JOIN_THREADS = 256;
 constexpr int PA_JOIN_SLOTS = 4096;  // slots per join block of the accumulation
 
@@ -757,11 +764,14 @@ __global__ void __launch_bounds__(MmaShape<T, DP>::THREADS)
     const int h = cur.row / p.chunks, chunk = cur.row - h * p.chunks;
     const bool from_begin = cur.step == 0;  // this share holds the row's first step
     const int nh = min(p.heads, p.group - chunk * PA_HEADS);
-    float m[HALVES], l[HALVES];
+    float m[HALVES], l[HALVES], high[L::kHalf ? HALVES : 1];
 #pragma unroll
     for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
 #pragma unroll
-    for (int x = 0; x < HALVES; ++x) m[x] = -INFINITY, l[x] = 0.f;
+    for (int x = 0; x < HALVES; ++x) {
+      m[x] = -INFINITY, l[x] = 0.f;
+      if constexpr (L::kHalf) high[x] = -INFINITY;
+    }
     if constexpr (M::kQShared) {
       asm volatile("cp.async.wait_all;" ::: "memory");
       __syncwarp();
@@ -858,9 +868,20 @@ __global__ void __launch_bounds__(MmaShape<T, DP>::THREADS)
         }
       }
       // ---- running softmax, base 2. The reference value m follows the
-      // maximum only when that has grown by more than 2^8: the probabilities
-      // stay below 256, and the result is rescaled a few times per row instead
-      // of at every new maximum of any head.
+      // maximum only when that has grown by a few powers of two, so that the
+      // result is rescaled a few times per row instead of at every new maximum
+      // of any head. fp32: by more than 2^8.
+      // fp16: the probabilities 2^(s - m) enter the product as fp16 numbers, with
+      // 22 bits down to 2^-14 and none below 2^-25, so a step's largest has to
+      // lie well inside fp16's range, also where it is far below the row's
+      // maximum: a row of one dominant slot, whose value is near zero, has the
+      // sum of all the small probabilities for a result. m is set 2^11 below a
+      // step's maximum, up again when a later one is over 2^15 above it, down
+      // when one is less than 2 above it: a step's probabilities are below 2^15
+      // and keep 22 bits, or 2^-26 of its largest. Sums and results grow by
+      // as much in fp32; 2^60 is the limit, beyond which a step no longer
+      // counts. (Probabilities held relative to the row's maximum alone, below
+      // 2^8, were off by 6 % at 2^-23 of it, and zero from 2^-26 on.)
 #pragma unroll
       for (int t = 0; t < ST; ++t)
 #pragma unroll
@@ -889,7 +910,9 @@ __global__ void __launch_bounds__(MmaShape<T, DP>::THREADS)
         }
         if (!live) continue;
       }
-      bool grew = false;
+      // (false where neither has a score yet: the difference is NaN)
+      auto out_of_range = [](float most, float ref) { return fabsf(most - ref - PA_MIDDLE) > PA_FAR; };
+      bool far = false;
       float mx[HALVES];
 #pragma unroll
       for (int x = 0; x < HALVES; ++x) {
@@ -897,13 +920,18 @@ __global__ void __launch_bounds__(MmaShape<T, DP>::THREADS)
         if constexpr (ST > 1) mx[x] = fmaxf(mx[x], fmaxf(s[1][2 * x], s[1][2 * x + 1]));
         mx[x] = fmaxf(mx[x], __shfl_xor_sync(~0u, mx[x], 1));
         mx[x] = fmaxf(mx[x], __shfl_xor_sync(~0u, mx[x], 2));
-        grew |= mx[x] > m[x] + 8.f;
+        if constexpr (L::kHalf) far |= out_of_range(mx[x], m[x]);
+        else far |= mx[x] > m[x] + 8.f;
       }
-      if (__any_sync(~0u, grew)) {
+      if (__any_sync(~0u, far)) {
 #pragma unroll
         for (int x = 0; x < HALVES; ++x) {
-          const float mn = fmaxf(m[x], mx[x]);
-          const float f = mn > m[x] ? exp2_approx(m[x] - mn) : 1.f;
+          float mn = fmaxf(m[x], mx[x]);
+          if constexpr (L::kHalf) {
+            mn = out_of_range(mx[x], m[x]) ? fmaxf(mx[x] - PA_ABOVE, high[x] - PA_DEPTH) : m[x];
+            high[x] = fmaxf(high[x], mn);
+          }
+          const float f = mn != m[x] ? exp2_approx(m[x] - mn) : 1.f;
           l[x] *= f;
           m[x] = mn;
 #pragma unroll
