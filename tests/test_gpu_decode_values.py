@@ -76,3 +76,29 @@ def test_attention_of_equal_values_is_that_value(dec, n, D, G):  # noqa: F811
     assert float((out.float() - 1).abs().max()) <= 2.0 ** -11
 
 
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("gap", [41, 80, 300])
+@pytest.mark.parametrize("at", [0, 2000, 4095])
+@pytest.mark.parametrize("G,rows", [(4, 700), (16, 700), (4, 2)])
+def test_attention_of_a_row_that_one_slot_takes(dec, dtype, gap, at, G, rows):  # noqa: F811
+    """Scores further apart than any reference follows, values near fp16's
+    largest: the slot's own value and weight, in whatever order it comes.
+    (exp(-41) * 4096 is below 2^-46.)"""
+    n, D, page = 4096, 64, 16
+    rng = np.random.default_rng(at)
+    q, k, v = sink_rows(n, gap, D, 1, G, dtype, at, rng)
+    v = ((rng.random((n, D)) - 0.5) * 1.2e5).astype(v.dtype)
+    pages = n // page
+    pool = lambda x: dev(x.reshape(pages, 1, page, D))  # noqa: E731
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None].expand(rows, pages)
+    w = torch.zeros(rows, 1, n, device="cuda")
+    out = dec.paged_attention(dev(q)[None].expand(rows, G, D), pool(k), pool(v), table,
+                              torch.full((rows,), n, dtype=torch.int32, device="cuda"), scale=1.0, weights=w,
+                              weights_out=w)
+    got = out.double().cpu().numpy()
+    want = v[at].astype(np.float64)
+    assert (np.abs(got - want) <= 2.0 ** -20 * np.abs(want) + 2.0 ** -20).all() if dtype == F32 else (got == want).all()
+    weight = host(w)
+    np.testing.assert_allclose(weight[:, 0, at], G, rtol=2e-6)
+    rest = np.delete(weight, at, axis=2)
+    np.testing.assert_allclose(rest, G * np.exp(-float(gap)), rtol=gap * 2e-6 + 1e-5, atol=1e-37)
