@@ -334,8 +334,9 @@ WGX_API int wgx_kv_append(const wgx_kv_append_args *a, void *stream);
  * Fewer bits are in: the exponentials (2^-22 of themselves); fp16's probabilities
  * in the product with V (2^-22 of themselves, or 2^-26 of the largest among 16
  * neighbouring slots); fp32 products where a K/V head has more than 8 query heads
- * (operands to 2^-22). A live slot's NaN makes the results that it enters NaN,
- * and an infinite K or V may. The same inputs give the same bits. scratch:
+ * (operands to 2^-21). A live slot's NaN makes the results that it enters NaN,
+ * and an infinite K or V may (with more than 8 query heads, fp32 numbers within
+ * 2^-12 of the largest too). The same inputs give the same bits. scratch:
  * wgx_paged_attention_scratch_bytes(), 256-byte aligned (its contents need no
  * preparation). Limits: batch <= 2048, 128 query heads per K/V head, weights
  * over 2^25 slots. */

@@ -102,3 +102,45 @@ def test_attention_of_a_row_that_one_slot_takes(dec, dtype, gap, at, G, rows):  
     np.testing.assert_allclose(weight[:, 0, at], G, rtol=2e-6)
     rest = np.delete(weight, at, axis=2)
     np.testing.assert_allclose(rest, G * np.exp(-float(gap)), rtol=gap * 2e-6 + 1e-5, atol=1e-37)
+
+
+NANS = {"quiet": 0x7fc00000, "canonical": 0x7fffffff, "negative": 0xffffffff}
+
+
+@pytest.mark.parametrize("G", [1, 4, 12, 20])
+@pytest.mark.parametrize("D,n", [(64, 20), (128, 300), (256, 700)])
+@pytest.mark.parametrize("kind", list(NANS))
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_attention_of_a_live_nan_is_nan(dec, dtype, kind, D, n, G):  # noqa: F811
+    """NaN of a live key or of a query reaches every result of its row, NaN of
+    a live value its channel's, whatever bits the NaN has; nothing else."""
+    if dtype == F32:
+        nan = np.array([NANS[kind]], np.uint32).view(np.float32)[0]
+    else:
+        nan = np.array([NANS[kind] >> 16 if kind != "quiet" else 0x7e00], np.uint16).view(np.float16)[0]
+    assert np.isnan(nan)
+    c = Cache([n, n], 2, D, 16, dtype, seed=D)
+    q = np.random.default_rng(0).standard_normal((2, 2 * G, D)).astype(c.k.dtype)
+    clean = host(dec.paged_attention(dev(q), c.dk, c.dv, c.dtable, c.dlengths))
+    assert np.isfinite(clean).all()
+
+    def run(q=q, k=c.k, v=c.v):
+        return host(dec.paged_attention(dev(q), dev(k), dev(v), c.dtable, c.dlengths))
+    k = c.k.copy()
+    ref.slot_row(k, c.table, 1, 0, n // 2)[D // 3] = nan
+    out = run(k=k)
+    assert np.isnan(out[1, :G]).all()
+    np.testing.assert_array_equal(out[0], clean[0])
+    np.testing.assert_array_equal(out[1, G:], clean[1, G:])
+    v = c.v.copy()
+    ref.slot_row(v, c.table, 1, 1, n // 2)[D // 3] = nan
+    out = run(v=v)
+    assert np.isnan(out[1, G:, D // 3]).all()
+    out[1, G:, D // 3] = clean[1, G:, D // 3]
+    np.testing.assert_array_equal(out, clean)
+    qn = q.copy()
+    qn[0, G, D - 1] = nan
+    out = run(q=qn)
+    assert np.isnan(out[0, G]).all()
+    out[0, G] = clean[0, G]
+    np.testing.assert_array_equal(out, clean)
