@@ -329,7 +329,8 @@ WGX_API int wgx_kv_append(const wgx_kv_append_args *a, void *stream);
  * (infinities and NaN too) has no effect. With weights_out, dense
  * [batch][kv_heads][slots], the probabilities are accumulated per slot:
  *   weights_out[b][h][j] = weights[b][h][j] + sum of the group's p_j
- * for j < lengths[b] (other slots are not written; may be the same array).
+ * for j < lengths[b], p_j zero where j is not live (slots at or behind lengths[b]
+ * are not written; may be the same array).
  * Scores, their maximum and all sums are fp32, with one rounding at the end.
  * Fewer bits are in: the exponentials (2^-22 of themselves); fp16's probabilities
  * in the product with V (2^-22 of themselves, or 2^-26 of the largest among 16

@@ -144,3 +144,34 @@ def test_attention_of_a_live_nan_is_nan(dec, dtype, kind, D, n, G):  # noqa: F81
     assert np.isnan(out[0, G]).all()
     out[0, G] = clean[0, G]
     np.testing.assert_array_equal(out, clean)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("G", [2, 12, 20])
+@pytest.mark.parametrize("width,n", [(8, 100), (40, 600), (400, 6000)])
+@pytest.mark.parametrize("in_place", [True, False])
+def test_weights_of_slots_that_are_not_live_stay(dec, dtype, G, width, n, in_place):  # noqa: F811
+    """A row whose probabilities are NaN adds them to its live slots alone: what
+    the mask or the window leaves out keeps its weight."""
+    c = Cache([n, n], 2, 64, 16, dtype, width=width)
+    slots, window = width * 16, n - 21
+    rng = np.random.default_rng(0)
+    mask = rng.random((2, slots)) < 0.6
+    mask[1, n - 5] = True
+    ref.slot_row(c.k, c.table, 1, 0, n - 5)[0] = np.nan
+    w = rng.random((2, 2, slots)).astype(np.float32)
+    q = rng.standard_normal((2, 2 * G, 64)).astype(c.k.dtype)
+    dw = dev(w)
+    wo = dw if in_place else torch.full_like(dw, -5.0)
+    dec.paged_attention(dev(q), dev(c.k), c.dv, c.dtable, c.dlengths, window=window, mask=dev(mask), weights=dw,
+                        weights_out=wo)
+    got = host(wo)
+    live = mask & (np.arange(slots) >= n - window) & (np.arange(slots) < n)
+    assert np.isnan(got[1, 0][live[1]]).all()
+    for b in range(2):
+        for h in range(2):
+            dead = ~live[b] & (np.arange(slots) < n)
+            np.testing.assert_array_equal(got[b, h][dead], w[b, h][dead])
+            if (b, h) != (1, 0):
+                assert np.isfinite(got[b, h][:n]).all() and (got[b, h][live[b]] >= w[b, h][live[b]]).all()
+    np.testing.assert_array_equal(got[:, :, n:], w[:, :, n:] if in_place else np.full_like(w[:, :, n:], -5))

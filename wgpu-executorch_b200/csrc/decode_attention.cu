@@ -165,6 +165,16 @@ __device__ void build_prefix(const AttnArgs &p, uint32_t *prefix, int *lens, boo
   __syncthreads();
 }
 
+// Whether slot t of sequence b is live. The accumulation of weights asks where a
+// head's sum is NaN: its probabilities are NaN then, those of slots that are
+// not live (kept as scores of -infinity) zero all the same.
+__device__ __forceinline__ bool slot_is_live(const AttnArgs &p, int b, const Span &s, int t) {
+  const wgx_kv_cache &c = p.a.cache;
+  if (t < s.lo || t >= s.len) return false;
+  if (p.a.mask && (t >= p.a.mask_width || !p.a.mask[int64_t(b) * p.a.mask_stride + t])) return false;
+  return uint32_t(c.page_table[int64_t(b) * c.table_stride + t / c.page_size]) < uint32_t(c.pages);
+}
+
 __device__ __forceinline__ uint32_t worker_count(const AttnArgs &p, uint32_t total) {
   const uint32_t want = (total + uint32_t(p.min_steps) - 1) / uint32_t(p.min_steps);
   return max(1u, min(want, uint32_t(p.max_workers)));
@@ -520,6 +530,7 @@ __device__ void finish_row(const AttnArgs &p, int b, int row, const Span &s, flo
                            uint8_t *rings, int ring_bytes, int stride) {
   constexpr int MOST = PA_BLOCK_WORKERS * PA_ROW_CLUSTER;
   __shared__ float factor[MOST][PA_HEADS], head_m[PA_HEADS], head_inv[PA_HEADS];
+  __shared__ bool odd;  // a head without probabilities that are numbers
   cg::cluster_group cluster = cg::this_cluster();
   const int S = CLUSTER ? p.row_blocks : 1, rank = CLUSTER ? int(cluster.block_rank()) : 0;
   auto of = [&](auto *mine, int r) {
@@ -528,6 +539,7 @@ __device__ void finish_row(const AttnArgs &p, int b, int row, const Span &s, flo
   };
   const int tid = threadIdx.x, D = p.a.cache.head_dim, parts = S * PA_BLOCK_WORKERS;
   const int h = row / p.chunks, chunk = row - h * p.chunks, nh = min(p.heads, p.group - chunk * PA_HEADS);
+  if (tid == 0) odd = false;
   if constexpr (CLUSTER) cluster.sync();
   else __syncthreads();
   if (tid < nh) {
@@ -541,6 +553,7 @@ __device__ void finish_row(const AttnArgs &p, int b, int row, const Span &s, flo
       factor[w][tid] = f;
       sum += f * x.y;
     }
+    if (sum != sum) odd = true;
     head_m[tid] = mu;
     head_inv[tid] = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
   }
@@ -567,7 +580,8 @@ __device__ void finish_row(const AttnArgs &p, int b, int row, const Span &s, flo
     const int t1 = min((s.first + s.steps * (rank + 1) / S) * TOK, int(min(int64_t(s.len), p.a.slots)));
     for (int t = t0 + tid; t < t1; t += int(blockDim.x)) {
       float w = p.a.weights[at + t];
-      if (t >= s.first * TOK)
+      if (t >= s.first * TOK && (!odd || slot_is_live(p, b, s, t)))
+#pragma unroll 4
         for (int g = 0; g < nh; ++g) w += exp2_approx(sc[int64_t(g) * p.score_stride + t] - head_m[g]) * head_inv[g];
       p.a.weights_out[at + t] = w;
     }
@@ -1537,6 +1551,7 @@ __global__ void __launch_bounds__(PA_JOIN_THREADS) join_kernel(const __grid_cons
   if (t0 >= t1) return;
   wait_for_prior_kernel();
   let_dependents_launch();
+  bool odd = false;  // a head without probabilities that are numbers
   for (int g = warp; g < p.group; g += WARPS) {
     const int chunk = g / PA_HEADS, gr = g % PA_HEADS;
     int w0, w1;
@@ -1548,24 +1563,26 @@ __global__ void __launch_bounds__(PA_JOIN_THREADS) join_kernel(const __grid_cons
     } else {
       st = stats_of(w0, w1 - w0 + 1, gr);
     }
+    odd |= st.y != st.y;
     if (lane == 0) {
       head_m[g] = st.x;
       head_inv[g] = st.y > 0.f || st.y != st.y ? 1.f / st.y : 0.f;
     }
   }
-  __syncthreads();
+  odd = __syncthreads_or(odd);
   const int64_t at = int64_t(at_row) * p.a.slots;
   const float *sc = p.scores + (int64_t(b) * p.a.q_heads + h * p.group) * p.score_stride;
   auto one = [&](int t) {
     float w = p.a.weights[at + t];
-    if (t >= s.first * TOK)  // (masked slots in front of the window have scores of -infinity)
+    // (slots in front of the window have scores of -infinity)
+    if (t >= s.first * TOK && (!odd || slot_is_live(p, b, s, t)))
       for (int g = 0; g < p.group; ++g)
         w += exp2_approx(sc[int64_t(g) * p.score_stride + t] - head_m[g]) * head_inv[g];
     p.a.weights_out[at + t] = w;
   };
   int t = t0 + 4 * tid;
-  if (p.weights_quads) {
-    // four slots of four heads at a time
+  if (p.weights_quads && !odd) {
+    // four slots of four heads at a time (2^(-infinity) times a number is zero)
     for (; t + 4 <= t1; t += 4 * PA_JOIN_THREADS) {
       float4 w = *reinterpret_cast<const float4 *>(p.a.weights + at + t);
       if (t >= s.first * TOK) {
