@@ -512,8 +512,13 @@ LinkPlan plan_links(wgx_context *ctx, const Program &P,
 // and the operator records nothing. The input's storage must then outlive
 // the output, so an input held in a memory-plan pool (reused once the input
 // dies) first gets a buffer of its own. Program inputs and outputs keep
-// their operators.
-std::set<size_t> plan_aliases(wgx_context *ctx, const Program &P,
+// their operators. An input value may still be bound to the caller's tensor;
+// its aliases then follow it (`of`).
+struct Aliases {
+  std::set<size_t> skip;           // the operators that record nothing
+  std::map<int64_t, int64_t> of;   // value -> the value whose storage it shares, itself no alias
+};
+Aliases plan_aliases(wgx_context *ctx, const Program &P,
                               const std::map<int64_t, wgx_tensor *> &tensors,
                               const std::set<const wgx_buffer *> &pools) {
   static const std::set<std::string> kViews = {
@@ -522,7 +527,7 @@ std::set<size_t> plan_aliases(wgx_context *ctx, const Program &P,
       "aten._unsafe_view.default",   "aten.alias_copy.default",   "et_vk.prepack.default"};
   std::set<int64_t> boundary(P.output_ids.begin(), P.output_ids.end());
   boundary.insert(P.input_ids.begin(), P.input_ids.end());
-  std::set<size_t> skip;
+  Aliases A;
   for (size_t i = 0; i < P.chain.size(); ++i) {
     const POp &op = P.chain[i];
     if (!kViews.count(op.name) || op.args.size() < 2) continue;
@@ -542,9 +547,11 @@ std::set<size_t> plan_aliases(wgx_context *ctx, const Program &P,
       tx->buffer = b;
     }
     to->buffer = tx->buffer;
-    skip.insert(i);
+    const auto root = A.of.find(x);
+    A.of[o] = root == A.of.end() ? x : root->second;
+    A.skip.insert(i);
   }
-  return skip;
+  return A;
 }
 
 // Max-pool cascades (the SPPF block): 2-3 consecutive
@@ -892,7 +899,7 @@ static void record_program_impl(wgx_context *ctx, const char *text, uint64_t len
   // value may move to a buffer of its own)
   std::set<const wgx_buffer *> pool_set;
   for (auto &kv : pool_buf) pool_set.insert(kv.second);
-  const std::set<size_t> alias_skip = plan_aliases(ctx, P, tensors, pool_set);
+  const Aliases aliases = plan_aliases(ctx, P, tensors, pool_set);
 
   // ---- input copies
   for (size_t i = 0; i < n_in; ++i) {
@@ -904,6 +911,8 @@ static void record_program_impl(wgx_context *ctx, const char *text, uint64_t len
     if (!written.count(v) && !out_bufs.count(args[i].v.tensor->buffer) &&
         same_layout(it->second, args[i].v.tensor)) {
       it->second->buffer = args[i].v.tensor->buffer;
+      for (const auto &alias : aliases.of)
+        if (alias.second == v) tensors.at(alias.first)->buffer = it->second->buffer;
       continue;
     }
     if (wgx_copy(ctx, args[i].v.tensor, it->second) != WGX_OK) fail(wgx_last_error());
@@ -933,7 +942,7 @@ static void record_program_impl(wgx_context *ctx, const char *text, uint64_t len
       ctx->commands.push_back(std::move(c));
       continue;
     }
-    if (fusion[oi] == 2 || links.skip.count(oi) || attn.skip.count(oi) || alias_skip.count(oi) ||
+    if (fusion[oi] == 2 || links.skip.count(oi) || attn.skip.count(oi) || aliases.skip.count(oi) ||
         pool_skip.count(oi))
       continue;
     if (auto pc = pools.at.find(oi); pc != pools.at.end()) {
