@@ -191,6 +191,9 @@ namespace wgx {
 // reference operator's recordIn and appends one or more Commands.
 using OpRecorder = std::function<void(wgx_context *, const std::vector<wgx_arg> &)>;
 const std::unordered_map<std::string, OpRecorder> &op_registry();
+// The arguments that an operator of text decoding writes (empty: another
+// operator, which writes its last argument).
+const std::vector<size_t> &decode_written_args(const std::string &op);
 
 // ------------------------------------------------------ kernel front-ends
 // All of these enqueue work on `stream` and throw Error on bad input.

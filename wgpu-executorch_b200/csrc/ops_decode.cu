@@ -437,6 +437,21 @@ void record_beam_search_step(wgx_context *ctx, const std::vector<wgx_arg> &args)
 
 }  // namespace
 
+// The arguments that an operator writes, by position in the lists above: more
+// than the last one, and most of them are read too (caches, and what an
+// operator may update in place).
+const std::vector<size_t> &decode_written_args(const std::string &op) {
+  static const std::unordered_map<std::string, std::vector<size_t>> table = {
+      {"wgx.kv_append.default", {4, 6, 7, 8, 9, 10}},
+      {"wgx.paged_attention.default", {9, 10}},
+      {"wgx.cache_evict.default", {8, 9, 10, 11, 12}},
+      {"wgx.beam_search_step.default", {7, 8, 9, 10, 11, 12, 13, 14}},
+  };
+  static const std::vector<size_t> none;
+  const auto it = table.find(op);
+  return it == table.end() ? none : it->second;
+}
+
 void register_decode_ops(std::unordered_map<std::string, OpRecorder> &r) {
   r["wgx.kv_append.default"] = record_kv_append;
   r["wgx.paged_attention.default"] = record_paged_attention;

@@ -507,12 +507,30 @@ LinkPlan plan_links(wgx_context *ctx, const Program &P,
   return L;
 }
 
+// The values that an operator writes: the decoding operators' arguments by their
+// list, of others the last one (or its items).
+std::vector<int64_t> values_written(const Program &P, const POp &op) {
+  std::vector<int64_t> out;
+  auto add = [&](int64_t v) {
+    if (v < 0 || size_t(v) >= P.values.size()) return;
+    if (P.values[v].kind == PValue::Tensor) out.push_back(v);
+    if (P.values[v].kind == PValue::TensorList) out.insert(out.end(), P.values[v].items.begin(), P.values[v].items.end());
+  };
+  const std::vector<size_t> &args = decode_written_args(op.name);
+  for (size_t k : args)
+    if (k < op.args.size()) add(op.args[k]);
+  if (args.empty() && !op.args.empty()) add(op.args.back());
+  return out;
+}
+
 // View-like copies (reshape, squeeze, unsqueeze, contiguous clone, and
 // et_vk.prepack, a copy of a constant) of a dense tensor move no bytes: the output value aliases the input's storage
 // and the operator records nothing. The input's storage must then outlive
 // the output, so an input held in a memory-plan pool (reused once the input
 // dies) first gets a buffer of its own. Program inputs and outputs keep
-// their operators. An input value may still be bound to the caller's tensor;
+// their operators, and so does a copy of which either side is written again: a
+// value that a decoding operator updates in place after it was copied, or an
+// output that another operator writes too. An input value may still be bound to the caller's tensor;
 // its aliases then follow it (`of`).
 struct Aliases {
   std::set<size_t> skip;           // the operators that record nothing
@@ -527,7 +545,25 @@ Aliases plan_aliases(wgx_context *ctx, const Program &P,
       "aten._unsafe_view.default",   "aten.alias_copy.default",   "et_vk.prepack.default"};
   std::set<int64_t> boundary(P.output_ids.begin(), P.output_ids.end());
   boundary.insert(P.input_ids.begin(), P.input_ids.end());
+  std::map<int64_t, std::vector<size_t>> writers;  // value -> the operators that write it
+  for (size_t i = 0; i < P.chain.size(); ++i)
+    for (int64_t v : values_written(P, P.chain[i])) writers[v].push_back(i);
   Aliases A;
+  auto root_of = [&](int64_t v) {
+    const auto it = A.of.find(v);
+    return it == A.of.end() ? v : it->second;
+  };
+  // whether any value that shares v's storage is written behind operator i
+  auto written_after = [&](int64_t v, size_t i) {
+    const auto it = writers.find(v);
+    return it != writers.end() && it->second.back() > i;
+  };
+  auto storage_written_after = [&](int64_t v, size_t i) {
+    const int64_t root = root_of(v);
+    bool hit = written_after(root, i);
+    for (const auto &alias : A.of) hit = hit || (alias.second == root && written_after(alias.first, i));
+    return hit;
+  };
   for (size_t i = 0; i < P.chain.size(); ++i) {
     const POp &op = P.chain[i];
     if (!kViews.count(op.name) || op.args.size() < 2) continue;
@@ -536,6 +572,7 @@ Aliases plan_aliases(wgx_context *ctx, const Program &P,
     if (x == o || xt == tensors.end() || ot == tensors.end() || boundary.count(o)) continue;
     wgx_tensor *tx = xt->second, *to = ot->second;
     if (tx->dtype != to->dtype || tx->numel != to->numel) continue;
+    if (writers[o].size() != 1 || storage_written_after(x, i)) continue;
     if (pools.count(tx->buffer)) {
       auto *b = new wgx_buffer();
       b->ctx = ctx;
@@ -547,8 +584,7 @@ Aliases plan_aliases(wgx_context *ctx, const Program &P,
       tx->buffer = b;
     }
     to->buffer = tx->buffer;
-    const auto root = A.of.find(x);
-    A.of[o] = root == A.of.end() ? x : root->second;
+    A.of[o] = root_of(x);
     A.skip.insert(i);
   }
   return A;
@@ -723,10 +759,7 @@ AttnPlan plan_attention(wgx_context *ctx, const Program &P,
     bool safe = true;
     for (size_t k = i + 1; k < r5 && safe; ++k) {
       if (absorbed.count(k) || fusion[k] == 2 || already_skipped.count(k)) continue;
-      const int64_t o = fusion[k] == 1 ? P.chain[k + 2].args[2] : P.chain[k].args.back();
-      std::vector<int64_t> outs{o};
-      if (P.values[o].kind == PValue::TensorList) outs = P.values[o].items;
-      for (auto t : outs) {
+      for (auto t : values_written(P, P.chain[fusion[k] == 1 ? k + 2 : k])) {
         const wgx_tensor *w = T(t);
         if (w && (w->buffer == q->buffer || w->buffer == kt->buffer)) safe = false;
       }
