@@ -132,3 +132,135 @@ def test_a_copy_taken_before_an_append_keeps_the_old_values(ctx, name, what, cha
                                   c.lengths if what == "lengths" else c.lengths + 1, D ** -0.5)
     attention_close(ot.numpy(), want, 6.0, True)
     np.testing.assert_array_equal(kt.numpy(), c.k)  # the caller's cache itself
+
+
+@pytest.mark.parametrize("later", [False, True])
+def test_a_copy_of_weights_next_to_their_update_in_place(ctx, later):
+    """Taken before the attention adds to them, it holds the old weights; taken
+    after it, the new ones."""
+    B, H, D, page = 1, 2, 64, 16
+    c = Cache([30], H, D, page, F16)
+    slots = c.width * page
+    rng = np.random.default_rng(1)
+    hq = rng.standard_normal((B, H, D)).astype(np.float16)
+    hw = rng.random((B, H, slots)).astype(np.float32)
+    table = np.where(c.table < 0, 0, c.table)
+    p = Builder()
+    q, kc, vc, t, ln, w = (p.like(a) for a in (hq, c.k, c.v, table, c.lengths, hw))
+    kept, out, out2, w2 = p.like(hw), p.like(hq), p.like(hq), p.like(hw)
+    if not later:
+        p.op("aten.clone.default", w, None, kept)
+    p.op("wgx.paged_attention.default", q, kc, vc, t, ln, None, None, None, w, w, out)
+    if later:
+        p.op("aten.clone.default", w, None, kept)
+    p.op("wgx.paged_attention.default", q, kc, vc, t, ln, None, None, None, kept, w2, out2)
+    wt, w2t = T(ctx, hw), ctx.tensor("float32", list(hw.shape))
+    ctx.recordProgram(p.program([q, kc, vc, t, ln, w], [out, out2, w2]), b"",
+                      [T(ctx, hq), T(ctx, c.k), T(ctx, c.v), T(ctx, table), T(ctx, c.lengths), wt,
+                       ctx.tensor("float16", list(hq.shape)), ctx.tensor("float16", list(hq.shape)), w2t])
+    ctx.submit()
+    ctx.sync()
+    _, once = ref.paged_attention(hq, c.k, c.v, table, c.lengths, D ** -0.5, weights=hw)
+    _, twice = ref.paged_attention(hq, c.k, c.v, table, c.lengths, D ** -0.5, weights=once)
+    np.testing.assert_allclose(w2t.numpy()[..., :30], (twice if later else once)[..., :30], atol=8e-5)
+    np.testing.assert_allclose(wt.numpy()[..., :30], once[..., :30], atol=8e-5)
+
+
+@pytest.mark.parametrize("outputs", [False, True])
+def test_state_written_in_place_stays_from_submit_to_submit(ctx, outputs):
+    """Append, attend with accumulated weights and evict, all of whose state
+    (caches, weights, positions, lengths, seen) is written in place: the
+    caller's tensors hold it after every submit and the next one goes on from
+    there, whether they are the Program's outputs too or not."""
+    B, H, G, D, page, steps, budget = 2, 2, 2, 64, 16, 6, 24
+    c = Cache([22, 10], H, D, page, F16, room=steps)
+    rng = np.random.default_rng(3)
+    table = np.where(c.table < 0, 0, c.table)
+    slots = c.width * page
+    hk, hv = (rng.standard_normal((B, 1, H, D)).astype(np.float16) for _ in range(2))
+    hq = rng.standard_normal((B, H * G, D)).astype(np.float16)
+    weights = rng.random((B, H, slots)).astype(np.float32)
+    pos = np.tile(np.arange(slots, dtype=np.int32), (B, H, 1))
+    lengths, seen = c.lengths.copy(), c.lengths.copy()
+    p = Builder()
+    k, v, q, kc, vc, t, ln, sn, w, ps = (p.like(a) for a in (hk, hv, hq, c.k, c.v, table, lengths, seen, weights, pos))
+    out = p.like(hq)
+    p.op("wgx.kv_append.default", k, v, t, ln, ps, sn, w, kc, vc, sn, ln)
+    p.op("wgx.paged_attention.default", q, kc, vc, t, ln, None, None, None, w, w, out)
+    p.op("wgx.cache_evict.default", t, ln, sn, w, ps, (budget,), (4,), (2,), kc, vc, w, ps, ln)
+    kt, vt, qt = T(ctx, hk), T(ctx, hv), T(ctx, hq)
+    state = [T(ctx, a) for a in (c.k, c.v, table, lengths, seen, weights, pos)]
+    ot = ctx.tensor("float16", list(hq.shape))
+    more = ([ln, sn, w, ps], state[3:]) if outputs else ([], [])
+    ctx.recordProgram(p.program([k, v, q, kc, vc, t, ln, sn, w, ps], [out] + more[0]), b"",
+                      [kt, vt, qt] + state + [ot] + more[1])
+    for _ in range(steps):
+        hk, hv = (rng.standard_normal((B, 1, H, D)).astype(np.float16) for _ in range(2))
+        hq = rng.standard_normal((B, H * G, D)).astype(np.float16)
+        kt.setData(hk), vt.setData(hv), qt.setData(hq)
+        ctx.submit()
+        ctx.sync()
+        for b in range(B):
+            for h in range(H):
+                ref.slot_row(c.k, table, b, h, lengths[b])[:] = hk[b, 0, h]
+                ref.slot_row(c.v, table, b, h, lengths[b])[:] = hv[b, 0, h]
+            weights[b, :, lengths[b]], pos[b, :, lengths[b]] = 0, seen[b]
+        lengths, seen = lengths + 1, seen + 1
+        want, added = ref.paged_attention(hq, c.k, c.v, table, lengths, D ** -0.5, weights=weights)
+        attention_close(ot.numpy(), want, 6.0, True)
+        before = lengths
+        weights = added.astype(np.float32)
+        lengths = ref.cache_evict(c.k, c.v, table, lengths, weights, pos, seen, budget, 4, 2)
+        assert state[3].numpy().tolist() == lengths.tolist() and state[4].numpy().tolist() == seen.tolist()
+        gw, gp = state[5].numpy(), state[6].numpy()
+        for b in range(B):
+            n = lengths[b]
+            np.testing.assert_array_equal(gp[b, :, :n], pos[b, :, :n])
+            np.testing.assert_allclose(gw[b, :, :n], weights[b, :, :n], atol=4e-5 * G * steps)
+        # (slots behind the lengths hold what the eviction left there)
+        np.testing.assert_array_equal(state[0].numpy(), c.k)
+        np.testing.assert_array_equal(state[1].numpy(), c.v)
+    assert (before > lengths).any()
+
+
+def test_two_programs_hand_state_over(ctx):
+    """The lengths that one Program advances in place are another's input."""
+    B, H, D, page = 1, 1, 64, 16
+    c = Cache([3], H, D, page, F16, room=4)
+    rng = np.random.default_rng(4)
+    hk, hv = (rng.standard_normal((B, 1, H, D)).astype(np.float16) for _ in range(2))
+    hq = rng.standard_normal((B, H, D)).astype(np.float16)
+    kt, vt, tt, lt = T(ctx, c.k), T(ctx, c.v), T(ctx, np.where(c.table < 0, 0, c.table)), T(ctx, c.lengths)
+    a = Builder()
+    k, v, t, ln, kc, vc = (a.like(x) for x in (hk, hv, c.table, c.lengths, c.k, c.v))
+    a.op("wgx.kv_append.default", k, v, t, ln, None, None, None, kc, vc, None, ln)
+    ctx.recordProgram(a.program([k, v, t, ln, kc, vc], []), b"", [T(ctx, hk), T(ctx, hv), tt, lt, kt, vt])
+    b = Builder()
+    q, t, ln, kc, vc = (b.like(x) for x in (hq, c.table, c.lengths, c.k, c.v))
+    out = b.like(hq)
+    b.op("wgx.paged_attention.default", q, kc, vc, t, ln, None, None, None, None, None, out)
+    ot = ctx.tensor("float16", [B, H, D])
+    ctx.recordProgram(b.program([q, t, ln, kc, vc], [out]), b"", [T(ctx, hq), tt, lt, kt, vt, ot])
+    for step in range(2):
+        ctx.submit()
+        ctx.sync()
+        n = c.lengths + step
+        for h in range(H):
+            ref.slot_row(c.k, c.table, 0, h, n[0])[:] = hk[0, 0, h]
+            ref.slot_row(c.v, c.table, 0, h, n[0])[:] = hv[0, 0, h]
+        want, _ = ref.paged_attention(hq, c.k, c.v, c.table, n + 1, D ** -0.5)
+        attention_close(ot.numpy(), want, 6.0, True)
+        assert lt.numpy().tolist() == (n + 1).tolist()
+
+
+def test_state_of_another_size_is_refused(ctx):
+    c = Cache([3], 1, 64, 16, F16, room=4)
+    new = np.zeros((1, 1, 1, 64), np.float16)
+    p = Builder()
+    k, v, t, ln, kc, vc = (p.like(x) for x in (new, new, c.table, c.lengths, c.k, c.v))
+    p.op("wgx.kv_append.default", k, v, t, ln, None, None, None, kc, vc, None, ln)
+    small = T(ctx, c.k[:1])
+    with pytest.raises(wgx.WgxError, match="updated in place"):
+        ctx.recordProgram(p.program([k, v, t, ln, kc, vc], []), b"", [T(ctx, new), T(ctx, new), T(ctx, c.table),
+                                                                      T(ctx, c.lengths), small, T(ctx, c.v)])
+    assert ctx.stats()["commands"] == 0

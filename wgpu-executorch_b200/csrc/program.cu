@@ -887,8 +887,15 @@ static void record_program_impl(wgx_context *ctx, const char *text, uint64_t len
   // the last two arguments of every operator (and the items of tensor lists
   // there); a caller tensor that is both an input and an output, or whose
   // dtype or shape differs from the value's, keeps the copy.
-  std::set<int64_t> written;
+  // What a decoding operator writes of the inputs is state that it updates in
+  // place (caches, lengths, weights, positions): it is bound too, so that the
+  // caller's tensor holds it from submit to submit. (Where one tensor is given
+  // for two inputs, a value among an operator's last two arguments keeps its
+  // copy.)
+  std::set<int64_t> written, state;
   for (const POp &op : P.chain) {
+    if (!decode_written_args(op.name).empty())
+      for (int64_t v : values_written(P, op)) state.insert(v);
     const size_t na = op.args.size();
     for (size_t k = na >= 2 ? na - 2 : 0; k < na; ++k) {
       const int64_t v = op.args[k];
@@ -898,7 +905,8 @@ static void record_program_impl(wgx_context *ctx, const char *text, uint64_t len
         for (auto t : P.values[v].items) written.insert(t);
     }
   }
-  std::set<const wgx_buffer *> in_bufs, out_bufs;
+  std::multiset<const wgx_buffer *> in_bufs;
+  std::set<const wgx_buffer *> out_bufs;
   for (size_t i = 0; i < n_in; ++i)
     if (args[i].kind == WGX_ARG_TENSOR) in_bufs.insert(args[i].v.tensor->buffer);
   for (size_t i = 0; i < n_out; ++i)
@@ -941,8 +949,13 @@ static void record_program_impl(wgx_context *ctx, const char *text, uint64_t len
     if (it == tensors.end())
       fail("program: no tensor for input value " + std::to_string(P.input_ids[i]));
     const int64_t v = P.input_ids[i];
-    if (!written.count(v) && !out_bufs.count(args[i].v.tensor->buffer) &&
-        same_layout(it->second, args[i].v.tensor)) {
+    const bool held = state.count(v) && (!written.count(v) || in_bufs.count(args[i].v.tensor->buffer) == 1);
+    if (held && it->second->byte_length() != args[i].v.tensor->byte_length())
+      fail("program: input " + std::to_string(i) + " is updated in place: it needs " +
+           std::to_string(it->second->byte_length()) + " bytes, got " +
+           std::to_string(args[i].v.tensor->byte_length()));
+    if ((held || (!written.count(v) && same_layout(it->second, args[i].v.tensor))) &&
+        !out_bufs.count(args[i].v.tensor->buffer)) {
       it->second->buffer = args[i].v.tensor->buffer;
       for (const auto &alias : aliases.of)
         if (alias.second == v) tensors.at(alias.first)->buffer = it->second->buffer;
