@@ -22,6 +22,10 @@ uint64_t paged_attention_scratch_bytes(const wgx_paged_attention_args &a);
 void launch_paged_attention(const wgx_paged_attention_args &a, cudaStream_t stream);
 void launch_kv_append(const wgx_kv_append_args &a, cudaStream_t stream);
 void launch_cache_evict(const wgx_cache_evict_args &a, cudaStream_t stream);
+// Kernels that a call launches.
+int paged_attention_launches(const wgx_paged_attention_args &a);
+int kv_append_launches(const wgx_kv_append_args &a);
+int cache_evict_launches(const wgx_cache_evict_args &a);
 uint64_t beam_search_scratch_bytes(const wgx_beam_search_args &a);
 void launch_beam_search_step(const wgx_beam_search_args &a, cudaStream_t stream);
 

@@ -1752,6 +1752,7 @@ Layout layout_of(const wgx_paged_attention_args &a, bool for_launch) {
 }  // namespace
 
 uint64_t paged_attention_scratch_bytes(const wgx_paged_attention_args &a) { return layout_of(a, false).bytes; }
+int paged_attention_launches(const wgx_paged_attention_args &a) { return layout_of(a, false).p.row_blocks ? 1 : 2; }
 
 void launch_paged_attention(const wgx_paged_attention_args &a, cudaStream_t stream) {
   Layout l = layout_of(a, true);

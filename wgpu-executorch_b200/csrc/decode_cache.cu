@@ -22,6 +22,7 @@ struct AppendArgs {
   wgx_kv_append_args a;
   int64_t capacity;
   int block_tokens;
+  int vec;       // rows move in 16-byte units
   int counters;  // this kernel writes the counters (their outputs are not its inputs, or one
                  // block per sequence)
   uint32_t *err;
@@ -460,35 +461,50 @@ __global__ void evict_lengths_kernel(const __grid_constant__ EvictArgs p) {
 
 }  // namespace
 
-void launch_kv_append(const wgx_kv_append_args &a, cudaStream_t stream) {
+// A call's kernel arguments but for the error word, and its grid.
+static AppendArgs append_plan(const wgx_kv_append_args &a, dim3 &grid) {
   AppendArgs p{};
   const wgx_kv_cache &c = a.cache;
   p.a = a;
   p.capacity = cache_capacity(c);
-  p.err = device_error_word(current_device());
   const int es = dtype_size(c.dtype);
-  bool vec = cache_rows_16b(c);
+  p.vec = cache_rows_16b(c);
   const int64_t strides[] = {a.k_batch_stride, a.k_token_stride, a.k_head_stride,
                              a.v_batch_stride, a.v_token_stride, a.v_head_stride};
-  for (int64_t s : strides) vec = vec && (s * es) % 16 == 0;
-  vec = vec && ((reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v)) & 15) == 0;
+  for (int64_t s : strides) p.vec = p.vec && (s * es) % 16 == 0;
+  p.vec = p.vec && ((reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v)) & 15) == 0;
   // tokens a block takes: AP_UNITS units a thread, and more where that would be
   // over sixteen blocks per SM
-  const int all = c.kv_heads * (vec ? c.head_dim * es / 16 : c.head_dim);
+  const int all = c.kv_heads * (p.vec ? c.head_dim * es / 16 : c.head_dim);
   const int64_t most = std::max<int64_t>(1, int64_t(device_sm_count()) * 16 / c.batch);
   p.block_tokens = int(std::max<int64_t>(int64_t(std::max(1, AP_THREADS / all)) * AP_UNITS, (a.tokens + most - 1) / most));
-  const dim3 grid(unsigned((a.tokens + p.block_tokens - 1) / p.block_tokens), unsigned(c.batch));
+  grid = dim3(unsigned((a.tokens + p.block_tokens - 1) / p.block_tokens), unsigned(c.batch));
   p.counters = grid.x == 1 || (a.lengths_out != a.lengths && (!a.seen || a.seen_out != a.seen));
+  return p;
+}
+
+int kv_append_launches(const wgx_kv_append_args &a) {
+  dim3 grid;
+  return append_plan(a, grid).counters ? 1 : 2;
+}
+
+void launch_kv_append(const wgx_kv_append_args &a, cudaStream_t stream) {
+  dim3 grid;
+  AppendArgs p = append_plan(a, grid);
+  p.err = device_error_word(current_device());
+  const int es = dtype_size(a.cache.dtype);
   const int th = timer_begin("append_kernel", stream);
-  launch_dependent(vec ? (es == 2 ? append_kernel<uint4, 8> : append_kernel<uint4, 4>)
-                       : (es == 2 ? append_kernel<uint16_t, 1> : append_kernel<uint32_t, 1>),
+  launch_dependent(p.vec ? (es == 2 ? append_kernel<uint4, 8> : append_kernel<uint4, 4>)
+                         : (es == 2 ? append_kernel<uint16_t, 1> : append_kernel<uint32_t, 1>),
                    grid, AP_THREADS, 0, stream, "kv_append launch", p);
   timer_end(th, stream);
   if (!p.counters) {
-    advance_kernel<<<unsigned(c.batch + 127) / 128, 128, 0, stream>>>(p);
+    advance_kernel<<<unsigned(a.cache.batch + 127) / 128, 128, 0, stream>>>(p);
     check_cuda(cudaGetLastError(), "kv_append counters launch");
   }
 }
+
+int cache_evict_launches(const wgx_cache_evict_args &a) { return a.lengths_out != a.lengths ? 1 : 2; }
 
 void launch_cache_evict(const wgx_cache_evict_args &a, cudaStream_t stream) {
   EvictArgs p{};
@@ -509,7 +525,7 @@ void launch_cache_evict(const wgx_cache_evict_args &a, cudaStream_t stream) {
   p.quads = a.slots % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.weights) | reinterpret_cast<uintptr_t>(a.weights_out) |
                                   reinterpret_cast<uintptr_t>(a.positions) |
                                   reinterpret_cast<uintptr_t>(a.positions_out)) & 15) == 0;
-  p.counters = a.lengths_out != a.lengths;
+  p.counters = cache_evict_launches(a) == 1;
   const int dev = current_device();
   p.err = device_error_word(dev);
   {

@@ -318,7 +318,7 @@ void record_kv_append(wgx_context *ctx, const std::vector<wgx_arg> &args) {
   a.seen_out = ptr<int32_t>(r.opt(9, "seen_out", {WGX_INT32}, {c.batch}));
   a.lengths_out = ptr<int32_t>(r.tensor(10, "lengths_out", {WGX_INT32}, {c.batch}));
   check_append(&a);
-  push(ctx, name, 2, 0, [a](const ExecEnv &env) { launch_kv_append(a, env.stream); });
+  push(ctx, name, kv_append_launches(a), 0, [a](const ExecEnv &env) { launch_kv_append(a, env.stream); });
 }
 
 // [q, k_cache, v_cache, page_table, lengths, mask?, scale?, window?, weights?,
@@ -352,7 +352,7 @@ void record_paged_attention(wgx_context *ctx, const std::vector<wgx_arg> &args) 
   a.q_head_stride = a.out_head_stride = c.head_dim;
   a.q_batch_stride = a.out_batch_stride = int64_t(a.q_heads) * c.head_dim;
   check_attention(&a);
-  push(ctx, name, 2, paged_attention_scratch_bytes(a), [a](const ExecEnv &env) {
+  push(ctx, name, paged_attention_launches(a), paged_attention_scratch_bytes(a), [a](const ExecEnv &env) {
     wgx_paged_attention_args x = a;
     x.scratch = env.workspace;
     x.scratch_bytes = env.workspace_bytes;
@@ -383,7 +383,7 @@ void record_cache_evict(wgx_context *ctx, const std::vector<wgx_arg> &args) {
       ptr<int32_t>(r.tensor(11, "positions_out", {WGX_INT32}, {c.batch, c.kv_heads, a.slots}));
   a.lengths_out = ptr<int32_t>(r.tensor(12, "lengths_out", {WGX_INT32}, {c.batch}));
   check_evict(&a);
-  push(ctx, name, 2, 0, [a](const ExecEnv &env) { launch_cache_evict(a, env.stream); });
+  push(ctx, name, cache_evict_launches(a), 0, [a](const ExecEnv &env) { launch_cache_evict(a, env.stream); });
 }
 
 // [logits, scores, finished, eos, lengths?, page_table?, spare?, k_cache?,
