@@ -129,3 +129,14 @@ def test_evict_moves_a_slots_label_only_with_its_row(dec, in_place, bad):  # noq
     np.testing.assert_array_equal(host(wo)[0, 0, :budget], ww[:budget])
     np.testing.assert_array_equal(host(po)[0, 0, :budget], pw[:budget])
     assert host(lo).tolist() == [budget] and dec.device_error(0) == 32
+
+
+@pytest.mark.parametrize("B", [1, 3])
+def test_append_of_more_tokens_than_any_table_holds(dec, B):  # noqa: F811
+    c = Cache([5] * B, 1, 16, 16, F16)
+    k0, lo = host(c.dk).copy(), torch.zeros(B, dtype=torch.int32, device="cuda")
+    new = torch.zeros(1, 1, 1, 16, dtype=F16, device="cuda").expand(B, 2 ** 31 - 1, 1, 16)
+    dec.kv_append(new, new, c.dk, c.dv, c.dtable, c.dlengths, lo)
+    assert host(lo).tolist() == [5] * B
+    np.testing.assert_array_equal(host(c.dk), k0)
+    assert dec.device_error(0) == 32

@@ -477,8 +477,8 @@ static AppendArgs append_plan(const wgx_kv_append_args &a, dim3 &grid) {
   // over sixteen blocks per SM
   const int all = c.kv_heads * (p.vec ? c.head_dim * es / 16 : c.head_dim);
   const int64_t most = std::max<int64_t>(1, int64_t(device_sm_count()) * 16 / c.batch);
-  p.block_tokens = int(std::max<int64_t>(int64_t(std::max(1, AP_THREADS / all)) * AP_UNITS, (a.tokens + most - 1) / most));
-  grid = dim3(unsigned((a.tokens + p.block_tokens - 1) / p.block_tokens), unsigned(c.batch));
+  p.block_tokens = int(std::max<int64_t>(int64_t(std::max(1, AP_THREADS / all)) * AP_UNITS, (int64_t(a.tokens) + most - 1) / most));
+  grid = dim3(unsigned((int64_t(a.tokens) + p.block_tokens - 1) / p.block_tokens), unsigned(c.batch));
   p.counters = grid.x == 1 || (a.lengths_out != a.lengths && (!a.seen || a.seen_out != a.seen));
   return p;
 }
