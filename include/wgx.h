@@ -339,7 +339,8 @@ WGX_API int wgx_kv_append(const wgx_kv_append_args *a, void *stream);
  * and an infinite K or V may (with more than 8 query heads, fp32 numbers within
  * 2^-12 of the largest too). The same inputs give the same bits. scratch:
  * wgx_paged_attention_scratch_bytes(), 256-byte aligned (its contents need no
- * preparation). Limits: batch <= 2048, 128 query heads per K/V head, weights
+ * preparation); with weights it holds 4 bytes per query head and slot that the
+ * table, or the window, can name. Limits: batch <= 2048, 128 query heads per K/V head, weights
  * over 2^25 slots. */
 typedef struct wgx_paged_attention_args {
   wgx_kv_cache cache;

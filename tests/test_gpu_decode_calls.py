@@ -1,10 +1,16 @@
 """What the decoding operators' calls say beside their results: the launch counts
-of recorded commands."""
+of recorded commands, and the scratch they ask for."""
+import ctypes
+import struct
+
 import numpy as np
 import pytest
+import torch
 
 import wgx
-from test_gpu_decode import F16, T, Cache
+from test_decode_cpu import FORMATS, GOOD
+from test_gpu_decode import F16, T, Cache, dec  # noqa: F401
+from wgx import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -57,3 +63,52 @@ def test_launch_count_of_a_recorded_beam_step(ctx):
                                                  t(np.zeros((1, 2), bool)), 0, None, None, None, None, None,
                                                  e("float32"), e("int32"), e("int32"), e("bool"), None, None])
     same_launches(ctx, 2)
+
+
+def scratch_bytes(**fields):
+    fmt, names = FORMATS["attention"]
+    fields = dict(GOOD["attention"], **fields)
+    packed = struct.Struct("@" + fmt).pack(*(fields.get(n, 0.0 if n == "scale" else 0) for n in names))
+    buf, n = ctypes.create_string_buffer(packed, len(packed)), ctypes.c_uint64()
+    _lib.check(_lib.lib.wgx_paged_attention_scratch_bytes(ctypes.addressof(buf), ctypes.byref(n)))
+    return n.value
+
+
+def test_scratch_of_a_window_goes_by_the_window():
+    """Scores are kept for the weights: of the slots a window can hold, not of
+    all that a wide table can name."""
+    case = dict(batch=64, kv_heads=8, q_heads=32, head_dim=128, page_size=16, table_width=8192, table_stride=8192,
+                weights=4096, weights_out=4096, slots=131072)
+    scores = 64 * 32 * 4096 * 4
+    most = 1.02 * scores + 2 ** 24  # and the partial results of the cut rows
+    assert scores <= scratch_bytes(window=4096, **case) <= most
+    assert scratch_bytes(window=0, **case) >= 32 * scores
+    assert scratch_bytes(window=4096, **dict(case, table_width=256, table_stride=256)) <= most
+
+
+@pytest.mark.parametrize("dtype,G", [(torch.float16, 2), (torch.float32, 2), (torch.float32, 12)])
+@pytest.mark.parametrize("window", [1, 17, 250, 1000, 4097])
+def test_window_weights_within_their_scratch(dec, dtype, G, window):  # noqa: F811
+    """The result with a workspace of exactly the size asked for, poisoned
+    around it; slots on both sides of a step's edge."""
+    import decode_reference as ref
+    lengths = [3, 1000, 2063, 4100]
+    c = Cache(lengths, 2, 64, 16, dtype, width=300)
+    slots = c.width * 16
+    rng = np.random.default_rng(window)
+    q = rng.standard_normal((4, 2 * G, 64)).astype(c.k.dtype)
+    w = rng.random((4, 2, slots)).astype(np.float32)
+    dq, dw = torch.from_numpy(q).cuda(), torch.from_numpy(w).cuda()
+    wo = torch.full_like(dw, -5.0)
+    n = scratch_bytes(batch=4, kv_heads=2, q_heads=2 * G, head_dim=64, dtype=1 if dtype == torch.float16 else 0,
+                      pages=c.k.shape[0], page_size=16, table_width=c.width, table_stride=c.width, window=window,
+                      weights=4096, weights_out=8192, slots=slots)
+    room = torch.full((n + 4096,), 0xff, dtype=torch.uint8, device="cuda")
+    dec.paged_attention(dq, c.dk, c.dv, c.dtable, c.dlengths, window=window, weights=dw, weights_out=wo,
+                        workspace=room[:n])
+    _, want = ref.paged_attention(q, c.k, c.v, c.table, c.lengths, 0.125, window, None, w)
+    got = wo.cpu().numpy()
+    for b, m in enumerate(lengths):
+        np.testing.assert_allclose(got[b, :, :m], want[b, :, :m], rtol=1e-6, atol=4e-5 * G)
+        assert (got[b, :, m:] == -5).all()
+    assert (room[n:] == 0xff).all() and dec.device_error(0) == 0

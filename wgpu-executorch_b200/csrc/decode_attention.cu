@@ -94,8 +94,8 @@ struct AttnArgs {
   int part_stride;    // head_dim rounded up to 4
   float2 *part_ml;    // [worker][2][heads] (max, sum)
   float2 *stats;      // [row][heads]: of rows finished by one warp (accumulation only)
-  float *scores;      // [batch][q_heads][score_stride] (accumulation only)
-  int64_t score_stride;
+  float *scores;      // [batch][q_heads][score_stride], from a row's first step (accumulation only)
+  int64_t score_stride;  // slots of the steps that a row can have
   int weights_quads;  // weights move four slots at a time
   int heads;          // min(group, PA_HEADS): rows a partial result has
   uint32_t *prefix;   // [batch + 1] steps of a row before each sequence (for the join)
@@ -582,7 +582,8 @@ __device__ void finish_row(const AttnArgs &p, int b, int row, const Span &s, flo
       float w = p.a.weights[at + t];
       if (t >= s.first * TOK && (!odd || slot_is_live(p, b, s, t)))
 #pragma unroll 4
-        for (int g = 0; g < nh; ++g) w += exp2_approx(sc[int64_t(g) * p.score_stride + t] - head_m[g]) * head_inv[g];
+        for (int g = 0; g < nh; ++g)
+          w += exp2_approx(sc[int64_t(g) * p.score_stride + (t - s.first * TOK)] - head_m[g]) * head_inv[g];
       p.a.weights_out[at + t] = w;
     }
   }
@@ -912,7 +913,7 @@ __global__ void __launch_bounds__(MmaShape<T, DP>::THREADS)
             if (!((live >> (t * 8 + 2 * (lane & 3) + (e & 1))) & 1)) s[t][e] = -INFINITY;
       }
       if (p.scores) {
-        const int t0 = (cur.s.first + cur.step + int(i)) * TOK + 2 * (lane & 3);
+        const int t0 = (cur.step + int(i)) * TOK + 2 * (lane & 3);
         if (part == 0) {
 #pragma unroll
           for (int x = 0; x < HALVES; ++x) {
@@ -1291,7 +1292,7 @@ __global__ void __launch_bounds__(SimtShape<DP, G>::THREADS)
       if (p.scores) {
         if (quarter == 0) {
           float *w = p.scores + (int64_t(cur.b) * p.a.q_heads + h * nh) * p.score_stride +
-                     (cur.s.first + cur.step + int(i)) * TOK + ks;
+                     (cur.step + int(i)) * TOK + ks;
           for (int g = 0; g < G; ++g)
             if (g < nh) w[int64_t(g) * p.score_stride] = s[g];
         }
@@ -1577,7 +1578,7 @@ __global__ void __launch_bounds__(PA_JOIN_THREADS) join_kernel(const __grid_cons
     // (slots in front of the window have scores of -infinity)
     if (t >= s.first * TOK && (!odd || slot_is_live(p, b, s, t)))
       for (int g = 0; g < p.group; ++g)
-        w += exp2_approx(sc[int64_t(g) * p.score_stride + t] - head_m[g]) * head_inv[g];
+        w += exp2_approx(sc[int64_t(g) * p.score_stride + (t - s.first * TOK)] - head_m[g]) * head_inv[g];
     p.a.weights_out[at + t] = w;
   };
   int t = t0 + 4 * tid;
@@ -1588,7 +1589,7 @@ __global__ void __launch_bounds__(PA_JOIN_THREADS) join_kernel(const __grid_cons
       if (t >= s.first * TOK) {
 #pragma unroll 4
         for (int g = 0; g < p.group; ++g) {
-          const float4 x = __ldcs(reinterpret_cast<const float4 *>(sc + int64_t(g) * p.score_stride + t));
+          const float4 x = __ldcs(reinterpret_cast<const float4 *>(sc + int64_t(g) * p.score_stride + (t - s.first * TOK)));
           const float m = head_m[g], inv = head_inv[g];
           w.x += exp2_approx(x.x - m) * inv;
           w.y += exp2_approx(x.y - m) * inv;
@@ -1740,7 +1741,7 @@ Layout layout_of(const wgx_paged_attention_args &a, bool for_launch) {
   p.o_blocks = int((int64_t(c.batch) * a.q_heads + per_block - 1) / per_block);
   if (a.weights_out) {
     p.stats = reinterpret_cast<float2 *>(take(uint64_t(c.batch) * c.kv_heads * p.chunks * PA_HEADS * 8));
-    p.score_stride = (p.capacity + 15) / 16 * 16;
+    p.score_stride = (row_steps * l.cfg->tok + 15) / 16 * 16;
     p.weights_quads = a.slots % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.weights) |
                                             reinterpret_cast<uintptr_t>(a.weights_out)) & 15) == 0;
     p.scores = reinterpret_cast<float *>(take(uint64_t(c.batch) * a.q_heads * p.score_stride * 4));
