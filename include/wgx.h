@@ -284,9 +284,9 @@ WGX_API int wgx_conv2d_noalloc(const wgx_conv2d_params *p, const void *in, const
  * names is left out and the device error word gets a bit, which the next
  * wgx_sync reports as WGX_ERR_DEVICE. Of such a length wgx_paged_attention
  * reads the slots that the table has; the calls that write leave the sequence
- * as it is and hand its length on unchanged. Limits: head_dim <= 256, batch <= 65535,
- * 2^30 slots per sequence. All calls enqueue on `stream` of the current device
- * and return; scratch memory is in use until the enqueued work is done. */
+ * as it is and hand its length on unchanged. Limits: head_dim <= 256, batch <=
+ * 65535, 2^30 slots per sequence. All calls enqueue on `stream` of the current
+ * device and return; scratch memory is in use until the enqueued work is done. */
 typedef struct wgx_kv_cache {
   void *k, *v;
   const int32_t *page_table; /* [batch][table_width] */
@@ -340,8 +340,8 @@ WGX_API int wgx_kv_append(const wgx_kv_append_args *a, void *stream);
  * 2^-12 of the largest too). The same inputs give the same bits. scratch:
  * wgx_paged_attention_scratch_bytes(), 256-byte aligned (its contents need no
  * preparation); with weights it holds 4 bytes per query head and slot that the
- * table, or the window, can name. Limits: batch <= 2048, 128 query heads per K/V head, weights
- * over 2^25 slots. */
+ * table, or the window, can name. Limits: batch <= 2048, 128 query heads per K/V
+ * head, weights over 2^25 slots. */
 typedef struct wgx_paged_attention_args {
   wgx_kv_cache cache;
   const void *q; /* [batch][q_heads][head_dim] */

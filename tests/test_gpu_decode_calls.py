@@ -1,5 +1,5 @@
 """What the decoding operators' calls say beside their results: the launch counts
-of recorded commands, and the scratch they ask for."""
+of recorded commands, the scratch they ask for, and what autograd sees."""
 import ctypes
 import struct
 
@@ -112,3 +112,55 @@ def test_window_weights_within_their_scratch(dec, dtype, G, window):  # noqa: F8
         np.testing.assert_allclose(got[b, :, :m], want[b, :, :m], rtol=1e-6, atol=4e-5 * G)
         assert (got[b, :, m:] == -5).all()
     assert (room[n:] == 0xff).all() and dec.device_error(0) == 0
+
+
+def test_autograd_sees_what_the_calls_write(dec):  # noqa: F811
+    """The operators are outside autograd (results carry no graph), but what
+    they write counts as written: backward over a tensor saved before and
+    overwritten since is refused instead of silently wrong."""
+    c = Cache([20, 10], 2, 64, 16, F16)
+    q = torch.zeros(2, 4, 64, dtype=F16, device="cuda", requires_grad=True)
+    slots = c.width * 16
+    w, wo = torch.zeros(2, 2, slots, device="cuda"), torch.zeros(2, 2, slots, device="cuda")
+    out = torch.empty(2, 4, 64, dtype=F16, device="cuda")
+    count = lambda *ts: [t._version for t in ts]  # noqa: E731
+    v0 = count(out, wo)
+    r = dec.paged_attention(q, c.dk, c.dv, c.dtable, c.dlengths, out, weights=w, weights_out=wo)
+    assert r is out or r.data_ptr() == out.data_ptr()
+    assert not r.requires_grad and r.grad_fn is None
+    assert count(out, wo) == [n + 1 for n in v0]
+    k = torch.zeros(2, 1, 2, 64, dtype=F16, device="cuda")
+    lo, so, seen = torch.zeros_like(c.dlengths), torch.zeros_like(c.dlengths), torch.zeros_like(c.dlengths)
+    pos = torch.zeros(2, 2, slots, dtype=torch.int32, device="cuda")
+    written, read = [c.dk, c.dv, lo, so, pos, w], [k, c.dtable, c.dlengths, seen]
+    v0, r0 = count(*written), count(*read)
+    dec.kv_append(k, k, c.dk, c.dv, c.dtable, c.dlengths, lo, seen=seen, seen_out=so, positions=pos, weights=w)
+    assert count(*written) == [n + 1 for n in v0] and count(*read) == r0
+    po = torch.zeros_like(pos)
+    written, read = [c.dk, c.dv, lo, wo, po], [c.dtable, c.dlengths, w, pos, seen]
+    v0, r0 = count(*written), count(*read)
+    dec.cache_evict(c.dk, c.dv, c.dtable, c.dlengths, lo, w, wo, pos, po, seen, budget=8)
+    assert count(*written) == [n + 1 for n in v0] and count(*read) == r0
+    x, s = torch.zeros(1, 2, 50, device="cuda"), torch.zeros(1, 2, device="cuda")
+    f = torch.zeros(1, 2, dtype=torch.bool, device="cuda")
+    outs = [torch.zeros(1, 2, device="cuda"), torch.zeros(1, 2, dtype=torch.int32, device="cuda"),
+            torch.zeros(1, 2, dtype=torch.int32, device="cuda"), torch.zeros(1, 2, dtype=torch.bool, device="cuda")]
+    table, to = torch.zeros(2, 3, dtype=torch.int32, device="cuda"), torch.zeros(2, 3, dtype=torch.int32, device="cuda")
+    spare = torch.tensor([1, 2], dtype=torch.int32, device="cuda")
+    written, read = outs + [c.dk, c.dv, to, lo], [x, s, f, table, c.dlengths, spare]
+    v0, r0 = count(*written), count(*read)
+    dec.beam_search_step(x, s, f, *outs, eos=0, k_cache=c.dk, v_cache=c.dv, page_table=table, lengths=c.dlengths,
+                         spare=spare, page_table_out=to, lengths_out=lo)
+    assert count(*written) == [n + 1 for n in v0] and count(*read) == r0
+    # a saved tensor that was overwritten
+    a = torch.randn(2, 4, 64, device="cuda", requires_grad=True)
+    saved = torch.randn(2, 4, 64, device="cuda")
+    y = (a * saved).sum()
+    dec.paged_attention(torch.zeros(2, 4, 64, device="cuda"), c.dk.float(), c.dv.float(), c.dtable, c.dlengths, saved)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    # tensors made under inference mode have no versions to count
+    with torch.inference_mode():
+        t = torch.zeros(2, 4, 64, dtype=F16, device="cuda")
+        dec.paged_attention(t, c.dk, c.dv, c.dtable, c.dlengths, t.clone())
+    dec.paged_attention(q.detach(), c.dk, c.dv, c.dtable, c.dlengths, t)

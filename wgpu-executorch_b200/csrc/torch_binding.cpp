@@ -14,6 +14,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
+#include <initializer_list>
 #include <optional>
 #include <string>
 
@@ -152,6 +153,15 @@ struct Call {
       fail("workspace must be a contiguous uint8 tensor on the cache's device");
     return t;
   }
+  // what a call has written counts as written for autograd: saved tensors that
+  // were overwritten are noticed
+  void written(std::initializer_list<int> at) const {
+    for (int i : at) {
+      if (none(i)) continue;
+      const at::Tensor &t = THPVariable_Unpack(args[i]);
+      if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    }
+  }
   void *stream() const { return c10::cuda::getCurrentCUDAStream(dev).stream(); }
 };
 
@@ -208,6 +218,7 @@ PyObject *kv_append(PyObject *, PyObject *const *args, Py_ssize_t n) {
     c10::cuda::OptionalCUDAGuard guard;
     if (c10::cuda::current_device() != c.dev) guard.set_index(c.dev);
     c.check(f_append(&a, c.stream()));
+    c.written({2, 3, 6, 8, 9, 10});
     Py_RETURN_NONE;
   });
 }
@@ -274,6 +285,7 @@ PyObject *paged_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
     a.scratch = ws.data_ptr();
     a.scratch_bytes = uint64_t(ws.numel());
     c.check(f_attention(&a, c.stream()));
+    c.written({5, 10});
     return THPVariable_Wrap(out);
   });
 }
@@ -300,6 +312,7 @@ PyObject *cache_evict(PyObject *, PyObject *const *args, Py_ssize_t n) {
     c10::cuda::OptionalCUDAGuard guard;
     if (c10::cuda::current_device() != c.dev) guard.set_index(c.dev);
     c.check(f_evict(&a, c.stream()));
+    c.written({0, 1, 4, 6, 8});
     Py_RETURN_NONE;
   });
 }
@@ -347,6 +360,7 @@ PyObject *beam_search_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
     a.scratch = ws.data_ptr();
     a.scratch_bytes = uint64_t(ws.numel());
     c.check(f_beam(&a, c.stream()));
+    c.written({3, 4, 5, 6, 8, 9, 13, 14});
     Py_RETURN_NONE;
   });
 }

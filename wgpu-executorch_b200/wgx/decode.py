@@ -13,11 +13,14 @@ or float32, with any strides but a unit last one (a slot-major pool is passed
 as ``pool.transpose(1, 2)``). ``page_table[b, s // page_size]`` is the page of
 slot ``s`` of sequence ``b``; ``lengths[b]`` slots are in use. Lengths and page
 tables stay on the device: a call never waits for them. A page id or length
-that lies outside the cache is left out and noted (``device_error``).
+that lies outside the cache is left out and noted (``device_error``); the calls
+that write leave a sequence of such a length as it is.
 
 Calls are enqueued on the tensors' device's current stream. Outputs are
 arguments; nothing is kept between calls. Scratch memory comes from torch's
-allocator unless ``workspace`` (a uint8 tensor) is given.
+allocator unless ``workspace`` (a uint8 tensor) is given. The operators are for
+inference: results carry no gradient, whatever the inputs require; what a call
+writes counts as modified in place.
 """
 from __future__ import annotations
 
