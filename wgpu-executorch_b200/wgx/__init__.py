@@ -291,9 +291,13 @@ class _Shaders:
     # reference's registry); wgx.decode has the same operators as direct calls
     kvAppend = _native_shader("wgx.kv_append.default", {"vec16": "16-byte rows", "generic": ""})
     pagedAttention = _native_shader("wgx.paged_attention.default",
-                                    {"f16": "split over the cache, joined", "f32": "3xTF32"})
+                                    {"f16": "mma.sync, split over the cache and joined",
+                                     "f32": "CUDA cores up to 8 query heads per K/V head, 3xTF32 above",
+                                     "row": "a block or a cluster per short row"})
     cacheEvict = _native_shader("wgx.cache_evict.default", {"cluster": "radix selection"})
-    beamSearchStep = _native_shader("wgx.beam_search_step.default", {"chunked": ""})
+    beamSearchStep = _native_shader("wgx.beam_search_step.default",
+                                    {"scan": "segments of the vocabulary, then a selection per item",
+                                     "reorder": "page tables and partly filled pages"})
 
     def __iter__(self):
         for k, v in vars(type(self)).items():
