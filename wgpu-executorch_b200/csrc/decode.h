@@ -50,7 +50,25 @@ inline int current_device() {
   return dev;
 }
 
+inline uint64_t align256(uint64_t x) { return (x + 255) / 256 * 256; }  // parts of a scratch buffer
+
 #ifdef __CUDACC__
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+  for (int d = 16; d; d /= 2) x = fmaxf(x, __shfl_xor_sync(~0u, x, d));
+  return x;
+}
+__device__ __forceinline__ float warp_sum(float x) {
+#pragma unroll
+  for (int d = 16; d; d /= 2) x += __shfl_xor_sync(~0u, x, d);
+  return x;
+}
+
 // Programmatic dependent launch: the next kernel's blocks may be set up while
 // this one's work ends (every block of this kernel has started); wait returns
 // when all of the prior kernel's work is done and visible. Every kernel here

@@ -200,11 +200,6 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool l
                "r"(live ? 16 : 0)
                : "memory");
 }
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t *r) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -1405,17 +1400,6 @@ __global__ void __launch_bounds__(SimtShape<DP, G>::THREADS)
     finish_row<float, TOK, true>(p, cur.b, cur.row, cur.s, row_ml, rings, M::RING, DP);
 }
 
-__device__ __forceinline__ float warp_max(float x) {
-#pragma unroll
-  for (int d = 16; d; d /= 2) x = fmaxf(x, __shfl_xor_sync(~0u, x, d));
-  return x;
-}
-__device__ __forceinline__ float warp_sum(float x) {
-#pragma unroll
-  for (int d = 16; d; d /= 2) x += __shfl_xor_sync(~0u, x, d);
-  return x;
-}
-
 // Rows cut between workers: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i.
 // Blocks below o_blocks join query heads, join_warps warps each (one where a
 // row has few partial results, the whole block for a lone long row that most
@@ -1668,8 +1652,6 @@ const Config &config_for(int dtype, int head_dim, int heads) {
   }
   return table[dev][dt][dp][hk];
 }
-
-uint64_t align256(uint64_t x) { return (x + 255) / 256 * 256; }
 
 struct Layout {
   AttnArgs p;

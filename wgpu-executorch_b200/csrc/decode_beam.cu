@@ -60,16 +60,6 @@ __device__ __forceinline__ float unordered(uint32_t k) {
   return __uint_as_float(k ^ (k >> 31 ? 0x80000000u : 0xffffffffu));
 }
 
-__device__ __forceinline__ float warp_max(float x) {
-#pragma unroll
-  for (int d = 16; d; d /= 2) x = fmaxf(x, __shfl_xor_sync(~0u, x, d));
-  return x;
-}
-__device__ __forceinline__ float warp_sum(float x) {
-#pragma unroll
-  for (int d = 16; d; d /= 2) x += __shfl_xor_sync(~0u, x, d);
-  return x;
-}
 // The lanes' keys in descending order (bitonic), each with its tag.
 __device__ __forceinline__ void warp_sort(uint64_t &x, int &tag) {
   const int lane = threadIdx.x & 31;
@@ -98,11 +88,6 @@ __device__ __forceinline__ float warp_sort(float x) {
       x = ((lane & k) == 0) == ((lane & j) == 0) ? fmaxf(x, y) : fminf(x, y);
     }
   return x;
-}
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 
 // Key of a logit: larger logits first, equal ones by token. No two are equal.
@@ -527,8 +512,6 @@ __global__ void __launch_bounds__(BM_COPY_THREADS) reorder_kernel(const __grid_c
     }
   }
 }
-
-uint64_t align256(uint64_t x) { return (x + 255) / 256 * 256; }
 
 uint64_t layout(const wgx_beam_search_args &a, BeamArgs *p) {
   const uint64_t rows = uint64_t(a.batch) * a.beams;
