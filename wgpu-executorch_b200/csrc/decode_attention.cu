@@ -585,6 +585,11 @@ __device__ void finish_row(const AttnArgs &p, int b, int row, const Span &s, flo
   if constexpr (CLUSTER) cluster.sync();  // a block's results are read by the others until here
 }
 
+// ROW: row mode, a kernel of its own. In one kernel for both, the registers that
+// the end of a row needs were held through the steps: 54.2 against 52 us at 48
+// sequences x 4096 slots x 16 heads x 256, 5.14 against 5.02 at one of 77 slots x
+// 8 x 64, 63.8 against 60.8 at 16 sequences of 3000-5000 slots x 2 x 16 x 128 in
+// fp32; one row of 131072 slots x 8 x 4 x 128 is 0.9 us slower (96.1, 97).
 // Tensor-core form: the worker's heads are the 16 rows of an mma tile. A step of
 // 16 slots costs a warp about 48 mma of 128 channels and as many other
 // instructions; with operand addresses computed in full it was 450 instructions
@@ -607,8 +612,8 @@ struct MmaShape {
   static_assert(PA_BLOCK_WORKERS * (RING + EXTRA) + 1024 + (2 * 2048 + 1) * 4 + 10 * 1024 <= 227 * 1024, "shared memory of a block");
 };
 
-template <typename T, int DP, bool HALF_ROWS>
-__global__ void __launch_bounds__(MmaShape<T, DP>::THREADS)
+template <typename T, int DP, bool HALF_ROWS, bool ROW>
+__global__ void __launch_bounds__(MmaShape<T, DP>::THREADS, DP > 128 ? 1 : 2)
     paged_attention_kernel(const __grid_constant__ AttnArgs p) {
   using L = Tile<T, DP>;
   using M = MmaShape<T, DP>;
@@ -662,7 +667,7 @@ __global__ void __launch_bounds__(MmaShape<T, DP>::THREADS)
   const int rows = c.kv_heads * p.chunks;
   Walk<TOK> cur;
   uint32_t to_do, me = 0;
-  if (p.row_blocks) {
+  if constexpr (ROW) {
     // this cluster's row, this block's part of it, a quarter of that per worker
     const int unit = int(blockIdx.x) / p.row_blocks, rank = int(blockIdx.x) - unit * p.row_blocks;
     cur.b = unit / rows;
@@ -791,6 +796,7 @@ __global__ void __launch_bounds__(MmaShape<T, DP>::THREADS)
       __syncwarp();
     }
     const uint32_t here = min(uint32_t(cur.s.steps - cur.step), to_do);
+    const bool whole = from_begin && cur.step + int(here) == cur.s.steps;
 #pragma unroll 1
     for (uint32_t i = 0; i < here; ++i) {
       const uint32_t live = loader.oldest();
@@ -1040,8 +1046,7 @@ __global__ void __launch_bounds__(MmaShape<T, DP>::THREADS)
       }
     }
     to_do -= here;
-    const bool whole = from_begin && cur.step + int(here) == cur.s.steps;
-    if (p.row_blocks) worker_all(true);  // (the ring becomes the result's place)
+    if (ROW) worker_all(true);  // (the ring becomes the result's place)
 #pragma unroll
     for (int x = 0; x < HALVES; ++x) {
       float sum = l[x];
@@ -1049,7 +1054,7 @@ __global__ void __launch_bounds__(MmaShape<T, DP>::THREADS)
       sum += __shfl_xor_sync(~0u, sum, 2);
       const int g = (lane >> 2) + 8 * x;
       if (g >= nh || !ok) continue;
-      if (p.row_blocks) {
+      if (ROW) {
         float *ro = reinterpret_cast<float *>(sm.ring) + g * DP;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -1081,16 +1086,16 @@ __global__ void __launch_bounds__(MmaShape<T, DP>::THREADS)
         if (part == 0 && (lane & 3) == 0) p.part_ml[at] = make_float2(m[x], sum);
       }
     }
-    if (p.row_blocks || !to_do) break;
+    if (ROW || !to_do) break;
     cur.next_row(p, sm.lens, rows);
     load_q();
   }
   if (!ok) drain<STAGES>(loader.live_ring, bars, stage, phase);
-  uint8_t *rings = sm.ring - size_t(worker) * M::RING;
-  if (p.row_blocks == 1)
-    finish_row<T, TOK, false>(p, cur.b, cur.row, cur.s, row_ml, rings, M::RING, DP);
-  else if (p.row_blocks > 1)
-    finish_row<T, TOK, true>(p, cur.b, cur.row, cur.s, row_ml, rings, M::RING, DP);
+  if constexpr (ROW) {
+    uint8_t *rings = sm.ring - size_t(worker) * M::RING;
+    if (p.row_blocks == 1) finish_row<T, TOK, false>(p, cur.b, cur.row, cur.s, row_ml, rings, M::RING, DP);
+    else finish_row<T, TOK, true>(p, cur.b, cur.row, cur.s, row_ml, rings, M::RING, DP);
+  }
 }
 
 // CUDA-core form for fp32 caches and groups of at most 8 heads (G: the group
@@ -1120,7 +1125,7 @@ __device__ __forceinline__ float4 lds128(uint32_t addr) {
   return v;
 }
 
-template <int DP, int G>
+template <int DP, int G, bool ROW>
 __global__ void __launch_bounds__(SimtShape<DP, G>::THREADS)
     paged_attention_simt_kernel(const __grid_constant__ AttnArgs p) {
   using L = Tile<float, DP>;
@@ -1156,7 +1161,7 @@ __global__ void __launch_bounds__(SimtShape<DP, G>::THREADS)
   const int rows = c.kv_heads;  // (p.chunks is 1)
   Walk<TOK> cur;
   uint32_t to_do, me = 0;
-  if (p.row_blocks) {
+  if constexpr (ROW) {
     // this cluster's row, this block's part of it, a quarter of that per worker
     const int unit = int(blockIdx.x) / p.row_blocks, rank = int(blockIdx.x) - unit * p.row_blocks;
     cur.b = unit / rows;
@@ -1352,7 +1357,7 @@ __global__ void __launch_bounds__(SimtShape<DP, G>::THREADS)
     }
     to_do -= here;
     const bool whole = from_begin && cur.step + int(here) == cur.s.steps;
-    if (p.row_blocks) __syncwarp();  // (the ring becomes the result's place)
+    if (ROW) __syncwarp();  // (the ring becomes the result's place)
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       float sum = l[g];
@@ -1367,8 +1372,8 @@ __global__ void __launch_bounds__(SimtShape<DP, G>::THREADS)
       }
       if (g >= nh || !ok) continue;
       const int64_t at = (int64_t(me) * 2 + (from_begin ? 1 : 0)) * p.heads + g;
-      const float inv = p.row_blocks || !whole ? 1.f : sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-      float *to = p.row_blocks ? reinterpret_cast<float *>(sm.ring) + g * DP
+      const float inv = ROW || !whole ? 1.f : sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+      float *to = ROW ? reinterpret_cast<float *>(sm.ring) + g * DP
                   : whole ? static_cast<float *>(p.a.out) + int64_t(cur.b) * p.a.out_batch_stride +
                               int64_t(h * nh + g) * p.a.out_head_stride
                         : p.part_o + at * p.part_stride;
@@ -1383,21 +1388,21 @@ __global__ void __launch_bounds__(SimtShape<DP, G>::THREADS)
         }
       }
       if (lane == 0) {
-        if (p.row_blocks) row_ml[worker][g] = make_float2(m[g], sum);
+        if (ROW) row_ml[worker][g] = make_float2(m[g], sum);
         else if (!whole) p.part_ml[at] = make_float2(m[g], sum);
         else if (p.stats) p.stats[(int64_t(cur.b) * rows + cur.row) * PA_HEADS + g] = make_float2(m[g], sum);
       }
     }
-    if (p.row_blocks || !to_do) break;
+    if (ROW || !to_do) break;
     cur.next_row(p, sm.lens, rows);
     load_q();
   }
   if (!ok) drain<STAGES>(loader.live_ring, bars, stage, phase);
-  uint8_t *rings = sm.ring - size_t(worker) * M::RING;
-  if (p.row_blocks == 1)
-    finish_row<float, TOK, false>(p, cur.b, cur.row, cur.s, row_ml, rings, M::RING, DP);
-  else if (p.row_blocks > 1)
-    finish_row<float, TOK, true>(p, cur.b, cur.row, cur.s, row_ml, rings, M::RING, DP);
+  if constexpr (ROW) {
+    uint8_t *rings = sm.ring - size_t(worker) * M::RING;
+    if (p.row_blocks == 1) finish_row<float, TOK, false>(p, cur.b, cur.row, cur.s, row_ml, rings, M::RING, DP);
+    else finish_row<float, TOK, true>(p, cur.b, cur.row, cur.s, row_ml, rings, M::RING, DP);
+  }
 }
 
 // Rows cut between workers: out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i.
@@ -1591,14 +1596,15 @@ __global__ void __launch_bounds__(PA_JOIN_THREADS) join_kernel(const __grid_cons
 }
 
 struct Config {
-  void (*kernel)(AttnArgs);
+  void (*kernel)(AttnArgs), (*row_kernel)(AttnArgs);  // shares of the line; row mode
   int ring, tok, threads, ctas_per_sm;
 };
 
 template <typename T, int DP, bool HALF_ROWS>
 Config mma_config() {
   Config c{};
-  c.kernel = paged_attention_kernel<T, DP, HALF_ROWS>;
+  c.kernel = paged_attention_kernel<T, DP, HALF_ROWS, false>;
+  c.row_kernel = paged_attention_kernel<T, DP, HALF_ROWS, true>;
   c.ring = PA_BLOCK_WORKERS * (MmaShape<T, DP>::RING + MmaShape<T, DP>::EXTRA) + 1024;  // + alignment
   c.tok = Tile<T, DP>::TOK;
   c.threads = MmaShape<T, DP>::THREADS;
@@ -1607,7 +1613,8 @@ Config mma_config() {
 template <int DP, int G>
 Config simt_config() {
   Config c{};
-  c.kernel = paged_attention_simt_kernel<DP, G>;
+  c.kernel = paged_attention_simt_kernel<DP, G, false>;
+  c.row_kernel = paged_attention_simt_kernel<DP, G, true>;
   c.ring = PA_BLOCK_WORKERS * (SimtShape<DP, G>::RING + SimtShape<DP, G>::EXTRA) + 1024;
   c.tok = 8;
   c.threads = SimtShape<DP, G>::THREADS;
@@ -1640,9 +1647,10 @@ const Config &config_for(int dtype, int head_dim, int heads) {
   if (!ready[dev][dt][dp][hk]) {
     Config c = dp == 0 ? config_of<64>(dtype, heads)
                        : dp == 1 ? config_of<128>(dtype, heads) : config_of<256>(dtype, heads);
-    check_cuda(cudaFuncSetAttribute(c.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    c.ring + prefix_bytes(kPaMaxBatch)),
-               "paged_attention smem attr");
+    for (auto *kernel : {c.kernel, c.row_kernel})
+      check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      c.ring + prefix_bytes(kPaMaxBatch)),
+                 "paged_attention smem attr");
     check_cuda(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&c.ctas_per_sm, c.kernel, c.threads,
                                                              c.ring + prefix_bytes(256)),
                "paged_attention occupancy");
@@ -1745,8 +1753,8 @@ void launch_paged_attention(const wgx_paged_attention_args &a, cudaStream_t stre
   const wgx_kv_cache &c = a.cache;
   const int pre = prefix_bytes(c.batch);
   const int th = timer_begin("paged_attention_kernel", stream);
-  launch_dependent(l.cfg->kernel, dim3(unsigned(l.grid)), l.cfg->threads, size_t(l.cfg->ring + pre), stream,
-                   "paged_attention launch", l.p, l.p.row_blocks);
+  launch_dependent(l.p.row_blocks ? l.cfg->row_kernel : l.cfg->kernel, dim3(unsigned(l.grid)), l.cfg->threads,
+                   size_t(l.cfg->ring + pre), stream, "paged_attention launch", l.p, l.p.row_blocks);
   timer_end(th, stream);
   if (l.p.row_blocks) return;
   int64_t blocks = l.p.o_blocks;
