@@ -33,11 +33,12 @@
 //
 // Measured (fp16, K and V bytes over the time of the kernel, then the whole
 // call): 8 K/V heads x 128 channels, 131071 slots: 84.5 us, 6.35 TB/s, call 97
-// us; 64 sequences of 17-8192 slots with weights: 190 us, 5.7 TB/s, call 207;
+// us; 64 sequences of 17-8192 slots with weights: 190 us, 5.7 TB/s, call 208;
 // 48 sequences of one head of 256 channels x 16, 4096 slots each: steps run at
-// 6.4 TB/s, but start, cut rows and join are 20 us of the call's 52. What is
-// left is the chain lengths -> page table -> rows at the start (about 4 us)
-// and the join (5 us).
+// 6.4 TB/s, but start, cut rows and join are 20 us of the call's 52:
+// neighbouring shares lie in different blocks, and each of some 640 cut rows of
+// 16 KB goes through memory. What is left besides is the chain lengths -> page
+// table -> rows at the start (about 4 us) and the join (5 us).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -589,7 +590,7 @@ __device__ void finish_row(const AttnArgs &p, int b, int row, const Span &s, flo
 // the end of a row needs were held through the steps: 54.2 against 52 us at 48
 // sequences x 4096 slots x 16 heads x 256, 5.14 against 5.02 at one of 77 slots x
 // 8 x 64, 63.8 against 60.8 at 16 sequences of 3000-5000 slots x 2 x 16 x 128 in
-// fp32; one row of 131072 slots x 8 x 4 x 128 is 0.9 us slower (96.1, 97).
+// fp32; one row of 131072 slots x 8 x 4 x 128 the same within 1 %.
 // Tensor-core form: the worker's heads are the 16 rows of an mma tile. A step of
 // 16 slots costs a warp about 48 mma of 128 channels and as many other
 // instructions; with operand addresses computed in full it was 450 instructions
@@ -1103,8 +1104,9 @@ __global__ void __launch_bounds__(MmaShape<T, DP>::THREADS, DP > 128 ? 1 : 2)
 // products. On the tensor cores a step of 8 slots costs the same whatever the
 // group (about 450 instructions, most of them the operands' splitting); here
 // about 100 and 64 * G more at 128 channels. 12 sequences of 129-2001 slots x 5
-// heads x 80 channels, 2 query heads each: 23.5 us on the tensor cores, 19 here
-// (34 MB; the rest is latency: six steps per worker). 116 sequences x 2 heads x
+// heads x 80 channels, 2 query heads each: a call takes 32.4 us on the tensor
+// cores, 22.4 here (34 MB; the rest is latency: six or seven steps per worker,
+// whose masks are fetched one step ahead). 116 sequences x 2 heads x
 // 128 channels, 762-1525 slots: 52 us a call, 5.2 TB/s.
 template <int DP, int G>
 struct SimtShape {

@@ -12,7 +12,8 @@
 // in one launch.
 //
 // Measured: 32 x 1 beam x 50257 fp16 logits 10 us a call (two launches, 3 MB:
-// latency); 16 x 8 beams x 131072 fp32 logits and 24 layers of tails 59 us: the
+// latency, part of it the order of the threads' maxima and the second look at
+// the logits, which one beam does not need); 16 x 8 beams x 131072 fp32 logits and 24 layers of tails 59 us: the
 // scan 20 (60 MB; one wave of blocks with 3 or 4 per SM), the selection 7, the
 // copies 31 (226 MB moved, part of it within L2).
 //
