@@ -1,5 +1,5 @@
 """What the decoding operators' calls say beside their results: the launch counts
-of recorded commands, the scratch they ask for, and what autograd sees."""
+of recorded commands, the scratch they ask for, refusals at recording, and what autograd sees."""
 import ctypes
 import struct
 
@@ -164,3 +164,19 @@ def test_autograd_sees_what_the_calls_write(dec):  # noqa: F811
         t = torch.zeros(2, 4, 64, dtype=F16, device="cuda")
         dec.paged_attention(t, c.dk, c.dv, c.dtable, c.dlengths, t.clone())
     dec.paged_attention(q.detach(), c.dk, c.dv, c.dtable, c.dlengths, t)
+
+
+def test_an_eviction_of_too_many_slots_is_refused_when_recorded(ctx):
+    """Not at the first submit: a recorded command can run."""
+    t = lambda dt, *s: ctx.tensor(dt, list(s))  # noqa: E731
+
+    def record(width):
+        slots = width * 16
+        w, pos, ln = t("float32", 1, 1, slots), t("int32", 1, 1, slots), t("int32", 1)
+        ctx.recordShader(wgx.shaders.cacheEvict, [t("int32", 1, width), ln, ln, w, pos, 8, 0, 0, t("float16", 2, 1, 16, 8),
+                                                  t("float16", 2, 1, 16, 8), w, pos, ln])
+    with pytest.raises(wgx.WgxError, match="262144 slots"):
+        record(16385)
+    assert ctx.stats()["commands"] == 0
+    record(16384)
+    assert ctx.stats()["commands"] == 1

@@ -29,6 +29,8 @@ int cache_evict_launches(const wgx_cache_evict_args &a);
 uint64_t beam_search_scratch_bytes(const wgx_beam_search_args &a);
 void launch_beam_search_step(const wgx_beam_search_args &a, cudaStream_t stream);
 
+constexpr int64_t kEvictMaxSlots = 262144;  // of a sequence that cache_evict can order
+
 // Slots one sequence's table can name.
 inline int64_t cache_capacity(const wgx_kv_cache &c) { return int64_t(c.table_width) * c.page_size; }
 

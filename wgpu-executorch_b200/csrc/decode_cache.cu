@@ -135,6 +135,7 @@ __global__ void advance_kernel(const __grid_constant__ AppendArgs p) {
 constexpr int EV_THREADS = 512;
 constexpr int EV_MAX_CLUSTER = 8;
 constexpr int EV_MAX_CHUNK = 32768;  // slots per CTA: 6 bytes of shared memory each
+static_assert(kEvictMaxSlots == int64_t(EV_MAX_CLUSTER) * EV_MAX_CHUNK, "the checks' limit");
 constexpr int EV_BINS = 2048, EV_BITS = 11;
 constexpr int EV_CLASS = 128;        // slots of a class that are ranked by counting
 static_assert(EV_CLASS <= EV_THREADS, "one thread ranks one member");
@@ -517,9 +518,6 @@ void launch_cache_evict(const wgx_cache_evict_args &a, cudaStream_t stream) {
   while (S < EV_MAX_CLUSTER &&
          (slots > int64_t(S) * EV_MAX_CHUNK || (rows * S < device_sm_count() && slots > int64_t(S) * 2048)))
     S *= 2;
-  if (slots > int64_t(S) * EV_MAX_CHUNK)
-    fail("cache_evict: more than " + std::to_string(EV_MAX_CLUSTER * EV_MAX_CHUNK) +
-         " slots per sequence are not supported");
   p.chunk = int(((slots + S - 1) / S + 7) / 8 * 8);
   p.vec = cache_rows_16b(c);
   p.quads = a.slots % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.weights) | reinterpret_cast<uintptr_t>(a.weights_out) |

@@ -98,6 +98,7 @@ void check_evict(const wgx_cache_evict_args *a) {
        "recent + sinks must be in [0, budget]");
   need(a->slots >= cache_capacity(a->cache), op,
        "weights and positions must cover every slot of the page table");
+  need(cache_capacity(a->cache) <= kEvictMaxSlots, op, "more than 262144 slots per sequence are not supported");
 }
 
 void check_beam(const wgx_beam_search_args *a) {
